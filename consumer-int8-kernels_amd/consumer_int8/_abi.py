@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in include/consumer_int8_amd.h (libci8_amd.so).
+"""ctypes binding of the C ABI in include/consumer_int8_amd.h and
+include/consumer_int8_attention.h (libci8_amd.so).
 
 This is the binding an FFI caller would write; the torch ops do not use it (they call
 the same entry points from C++). Tests use it to reach the C ABI directly.
@@ -43,6 +44,42 @@ SIGNATURES = {
                               ctypes.c_int),
 }
 
+# include/consumer_int8_attention.h: descriptors are passed by address.
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", _p), ("heads", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class HeadNorm(ctypes.Structure):
+    _fields_ = [("q_weight", _p), ("k_weight", _p), ("eps", ctypes.c_double)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("table", _p), ("rows", _i64), ("rot", _i64), ("positions", _p), ("axes", _i64),
+                ("axis_of", _p), ("interleaved", _i64)]
+
+
+class Fp4CacheView(ctypes.Structure):
+    _fields_ = [("k_codes", _p), ("k_scales", _p), ("v_codes", _p), ("v_scales", _p),
+                ("k_code_page_stride", _i64), ("k_scale_page_stride", _i64),
+                ("v_code_page_stride", _i64), ("v_scale_page_stride", _i64), ("pages", _i64),
+                ("heads", _i64), ("page_size", _i64)]
+
+
+_heads, _norm, _rotation, _cache = (ctypes.POINTER(t)
+                                    for t in (Heads, HeadNorm, Rotation, Fp4CacheView))
+
+ATTENTION_SIGNATURES = {
+    "ci8_qk_norm_rope": ([_heads, _heads, _heads, _heads, _norm, _rotation, _i64, _i64, _p],
+                         ctypes.c_int),
+    "ci8_append_fp4": ([_heads, _heads, _heads, _heads, _norm, _rotation, _p, _cache, _i64, _i64,
+                        _p], ctypes.c_int),
+    "ci8_unpack_fp4": ([_cache, _p, _p, _p, _i64, _i64, _p], ctypes.c_int),
+    "ci8_attention_fp4": ([_heads, _cache, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p,
+                           ctypes.c_double, _i64, _i64, _p], ctypes.c_int),
+}
+
 _lib = None
 
 
@@ -50,7 +87,7 @@ def load(path: Path | str = LIB_PATH) -> ctypes.CDLL:
     global _lib
     if _lib is None:
         lib = ctypes.CDLL(str(path))
-        for name, (args, res) in SIGNATURES.items():
+        for name, (args, res) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes = args
             fn.restype = res

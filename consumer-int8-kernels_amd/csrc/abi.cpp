@@ -10,38 +10,19 @@
 #include <cstdio>
 #include <string>
 
+#include "abi_checks.h"
 #include "launch.h"
 
 namespace {
 
 thread_local std::string g_last_error;
 
-int fail(int status, const char* message) {
-  g_last_error = message;
-  return status;
-}
+using ci8::aligned;
+using ci8::as_stream;
+using ci8::overlap;
 
-int launched(hipError_t error) {
-  if (error != hipSuccess) {
-    g_last_error = std::string("HIP launch failed: ") + hipGetErrorString(error);
-    return CI8_ERR_LAUNCH;
-  }
-  g_last_error.clear();
-  return CI8_OK;
-}
-
-bool aligned(const void* p, uintptr_t bytes) {
-  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
-}
-
-bool overlap(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
-  const auto first = reinterpret_cast<uintptr_t>(a);
-  const auto second = reinterpret_cast<uintptr_t>(b);
-  return bytes_a > 0 && bytes_b > 0 && first < second + uint64_t(bytes_b) &&
-         second < first + uint64_t(bytes_a);
-}
-
-hipStream_t as_stream(void* stream) { return static_cast<hipStream_t>(stream); }
+int fail(int status, const char* message) { return ci8::abi_fail(status, message); }
+int launched(hipError_t error) { return ci8::abi_launched(error); }
 
 // Shared GEMM geometry (csrc/bindings.cpp:402-408 for the signed ops,
 // csrc/bindings.cpp:252-258 for channel_mm).
@@ -63,6 +44,24 @@ int check_q8(int64_t m, int64_t n, int64_t k) {
 }
 
 }  // namespace
+
+namespace ci8 {
+
+int abi_fail(int status, const char* message) {
+  g_last_error = message;
+  return status;
+}
+
+int abi_launched(hipError_t error) {
+  if (error != hipSuccess) {
+    g_last_error = std::string("HIP launch failed: ") + hipGetErrorString(error);
+    return CI8_ERR_LAUNCH;
+  }
+  g_last_error.clear();
+  return CI8_OK;
+}
+
+}  // namespace ci8
 
 extern "C" {
 
