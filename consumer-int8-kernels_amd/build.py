@@ -34,7 +34,7 @@ ARCH = "gfx950"
 HIP_SOURCES = ["quantize.hip", "gemm.hip", "gemm_small.hip", "gemm_ring.hip", "gemm_pp.hip", "gemv.hip", "gemv_stream.hip", "silu.hip",
                "allspark.hip", "q8block.hip", "gguf_q8.hip", "gguf_ring.hip",
                "gemm_grouped.hip", "grouped_ring.hip", "noalloc.hip", "gemm_bytes.hip",
-               "norm_rope.hip", "attention_split.hip"]
+               "norm_rope.hip", "attention_split.hip", "attention_prompt.hip"]
 HOST_SOURCES = ["abi.cpp", "attention_abi.cpp"]
 
 # -packed-fp32-ops: keep packed FP32 (v_pk_*_f32) out of the generated code.

@@ -64,6 +64,11 @@ struct AttentionArgs {
   float scale_log2;  // scale * log2(e)
   int table_width, seqs, tokens, group, max_q, window;
 };
+// Sequences of at most `rows` (16 or 32) rows, and those of more than `few`.
+hipError_t launch_attention_split(const AttentionArgs& args, int dim, int rows,
+                                  hipStream_t stream);
+hipError_t launch_attention_prompt(const AttentionArgs& args, int dim, int few,
+                                   hipStream_t stream);
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream);
 
 }  // namespace ci8

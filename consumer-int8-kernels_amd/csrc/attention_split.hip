@@ -1,11 +1,12 @@
-// attention_fp4 (include/consumer_int8_attention.h): causal attention of BF16 queries over a
-// paged cache of E2M1 values with power-of-two scales.
+// attention_fp4 for few query rows a sequence (include/consumer_int8_attention.h): causal
+// attention of BF16 queries over a paged cache of E2M1 values with power-of-two scales.
 //
 //   o = sum_t p_t v_t / sum_t p_t,   p_t = exp2(s_t - m),   s_t = q.k_t * scale * log2(e)
 //
-// in one pass with a running m. Rows are (token, query head of one key head) pairs, 16 a tile,
-// so that the cache is read once for all heads that share it. A wave works alone on 32 tokens
-// at a time:
+// in one pass with a running reference m. Rows are (token, query head of one key head) pairs,
+// 16 or 32, so that the cache is read once for all heads that share it: bound by HBM, whose
+// stream the conversions (half an instruction a value) and MFMAs have to stay under. A wave
+// works alone on 32 tokens at a time, the next 32 on their way:
 //
 //   S^T = K Q^T      v_mfma_f32_16x16x32_bf16, K as the row operand: lane l holds token l % 16
 //                    and the channels of its own scale block, 16 bytes of codes as they lie in
@@ -16,17 +17,26 @@
 //                    loads it, stored to the wave's own LDS tile and read transposed
 //                    (ds_read_b64_tr_b16) with the tokens in that order.
 //
-// All statistics of a row sit in the lanes of its column. Waves of a workgroup take parts of
-// the context and are joined in LDS.
+// All statistics of a row sit in the lanes of its column. m moves only when a score passes it by
+// 2^8 in weight, so most tiles exchange nothing between lanes and rescale nothing.
+//
+// Contexts differ and only the device knows them, so the work is cut there: all tiles of all
+// sequences and key heads are laid end to end and each workgroup takes an equal run of them.
+// A run that covers a whole context writes its output; parts of one go to the workspace, two
+// at most a workgroup, and a second kernel joins them in a fixed order.
 #include "attention_launch.h"
 #include "fp4_device.h"
+#include "launch.h"
 
 namespace ci8 {
 namespace {
 
-constexpr int kRows = 16;    // query rows of a tile
 constexpr int kTokens = 32;  // tokens a wave takes at once
+constexpr int kWaves = 8;
 constexpr float kLowest = -3.402823466e38f;
+// How far a score may pass the reference, as a power of two of its weight: sums of 2^31 such
+// weights stay in FP32, and BF16 weights are as exact at any size.
+constexpr float kSlack = 8.f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -39,6 +49,13 @@ __device__ __forceinline__ u32x2 lds_read_transposed(const char* p) {
                  (lds_s16x4*)reinterpret_cast<const s16x4*>(p)));
 }
 
+// Keeps LDS accesses of a wave's lanes in program order; the LDS itself does.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int D>
 struct Layout {
   // Channels a lane holds of a chunk: its own 16 bytes of codes (8 at D = 64).
@@ -49,266 +66,618 @@ struct Layout {
   static constexpr int kScaleBytes = D / kFp4Block;
 };
 
-// The codes and scales of 16 tokens' rows: this lane's token l % 16 and its chunks.
+// Codes and scales of 16 tokens' rows: this lane's token l % 16 and its chunks.
 template <int D>
 struct Raw {
   uint32_t codes[Layout<D>::kChunks][Layout<D>::kChunk / 8];
   uint32_t scales[Layout<D>::kChunks];
 };
 
+// `code_at`, `scale_at`: this lane's byte offsets from the first row.
 template <int D>
-__device__ __forceinline__ Raw<D> load_rows(const uint8_t* codes, const uint8_t* scales, int lane,
-                                            bool live) {
+__device__ __forceinline__ void load_rows(Raw<D>& r, const uint8_t* codes, const uint8_t* scales,
+                                          uint32_t code_at, uint32_t scale_at) {
   using L = Layout<D>;
-  Raw<D> r = {};
-  if (!live) return r;
-  const uint8_t* c = codes + (lane % 16) * (D / 2);
-  const uint8_t* s = scales + (lane % 16) * L::kScaleBytes;
-  const int group = lane / 16;
 #pragma unroll
   for (int u = 0; u < L::kChunks; ++u) {
-    const uint32_t* src =
-        reinterpret_cast<const uint32_t*>(c + (4 * u + group) * (L::kChunk / 2));
+    typedef uint32_t Words __attribute__((ext_vector_type(L::kChunk / 8)));
+    const Words w = *reinterpret_cast<const Words*>(codes + (code_at + u * 2 * L::kChunk));
 #pragma unroll
-    for (int w = 0; w < L::kChunk / 8; ++w) r.codes[u][w] = src[w];
-    r.scales[u] = s[(4 * u + group) * L::kChunk / kFp4Block];
+    for (int j = 0; j < L::kChunk / 8; ++j) r.codes[u][j] = w[j];
+    r.scales[u] = scales[scale_at + u * 4 * L::kChunk / kFp4Block];
   }
-  return r;
 }
 
-template <int D, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves) attention_kernel(const AttentionArgs p) {
+// What one sequence asks for.
+struct Sequence {
+  int q_begin, rows;        // first query row, and rows of (query, head) computed
+  int context, shift;       // tokens; position of query 0
+  int low, high;            // tokens that any row attends to
+  int first_high, last_low; // every row attends to [last_low, first_high)
+  __device__ int first_tile() const { return low / kTokens; }
+  __device__ int tiles() const { return (high + kTokens - 1) / kTokens - first_tile(); }
+};
+
+__device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int seq) {
+  Sequence s;
+  s.q_begin = seq;
+  int count = 1;
+  if (p.q_starts) {
+    s.q_begin = min(max(p.q_starts[seq], 0), p.tokens);
+    count = min(max(p.q_starts[seq + 1], s.q_begin), p.tokens) - s.q_begin;
+  }
+  const int shown = min(count, p.max_q);
+  s.rows = shown * p.group;
+  const int64_t capacity = int64_t(p.table_width) << p.cache.page_shift;
+  s.context = int(min(int64_t(max(p.context_lens[seq], 0)), capacity));
+  s.shift = s.context - count;
+  s.high = max(s.shift + shown, 0);
+  s.first_high = s.shift + 1;
+  s.low = p.window ? max(s.first_high - p.window, 0) : 0;
+  s.last_low = p.window ? max(s.high - p.window, 0) : 0;
+  return s;
+}
+
+// Tiles of a sequence that the split kernel has, at least one (it writes the rows that attend
+// to nothing): 0 without rows, or with more than `most`, which are the prompt kernel's.
+__device__ __forceinline__ int split_tiles(const Sequence& s, int most) {
+  return s.rows == 0 || s.rows > most ? 0 : max(s.tiles(), 1);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return int64_t(uint64_t(uint32_t(uniform(int(v)))) | uint64_t(uint32_t(uniform(int(v >> 32)))) << 32);
+}
+
+// Inclusive sums over the lanes.
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    const int below = __shfl_up(v, step, 64);
+    if (lane >= step) v += below;
+  }
+  return v;
+}
+
+// A run of tiles: [begin, end) of the row of all sequences' tiles, one after the other for each
+// key head.
+struct Run {
+  int64_t begin, end, quota;
+};
+struct Place {
+  int seq, head, tile, tiles;  // tile: from the sequence's first
+};
+
+__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int lane) {
+  int64_t total = 0;
+  for (int base = 0; base < p.seqs; base += 64) {
+    int n = 0;
+    if (base + lane < p.seqs) n = split_tiles(sequence(p, base + lane), most);
+#pragma unroll
+    for (int step = 32; step >= 1; step /= 2) n += __shfl_xor(n, step, 64);
+    total += n;
+  }
+  return uniform(total * p.cache.heads);
+}
+
+// Where tile `at` of all lies; at is less than their number. Continues from `seq0`, which has
+// `before` tiles of all in front.
+__device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int lane, int64_t at,
+                                           int seq0, int64_t before) {
+  Place place = {};
+  const int heads = p.cache.heads;
+  for (int base = seq0; base < p.seqs; base += 64) {
+    int n = 0;
+    if (base + lane < p.seqs) n = split_tiles(sequence(p, base + lane), most);
+    const int sum = wave_scan(n, lane);
+    const bool past = before + int64_t(sum) * heads > at;
+    const uint64_t hit = __ballot(past);
+    if (hit) {
+      const int which = __builtin_ctzll(hit);
+      place.seq = base + which;
+      place.tiles = uniform(__shfl(n, which, 64));
+      const int in_front = uniform(__shfl(sum, which, 64)) - place.tiles;
+      const int64_t inside = at - before - int64_t(in_front) * heads;
+      place.head = int(inside / place.tiles);
+      place.tile = int(inside % place.tiles);
+      return place;
+    }
+    before += int64_t(uniform(__shfl(sum, 63, 64))) * heads;
+  }
+  return place;
+}
+
+// Parts in the workspace: of workgroup w, part 2w continues a context, part 2w + 1 begins one.
+// Sums of rows [part][row][D] first, then their [reference, sum], then what each workgroup that
+// begins a context says of it.
+struct Joint {
+  int parts, q_begin, rows, head;
+};
+template <int D, int kTiles>
+__device__ __forceinline__ float* part_sums(const AttentionArgs& p, int part) {
+  return p.workspace + int64_t(part) * (16 * kTiles * D);
+}
+template <int D, int kTiles>
+__device__ __forceinline__ float* part_stats(const AttentionArgs& p, int part) {
+  return p.workspace + int64_t(kAttentionWorkspaceRows) * D + part * (16 * kTiles * 2);
+}
+template <int D>
+__device__ __forceinline__ Joint* joints(const AttentionArgs& p) {
+  // the last 64 KiB of the [rows, 2] region
+  return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 4096;
+}
+
+__device__ __forceinline__ void write_row4(const AttentionArgs& p, int dim, int q_begin, int row,
+                                           int kv_head, int channel, const f32x4& x, float top,
+                                           float sum) {
+  const float inv = sum == 0 ? 0.f : 1.f / sum;
+  const int64_t at = int64_t(q_begin + row / p.group) * p.q.heads + kv_head * p.group +
+                     row % p.group;
+  *reinterpret_cast<u32x2*>(p.out + at * dim + channel) =
+      u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+  if (p.lse && channel == 0)
+    p.lse[at] =
+        sum == 0 ? -__builtin_inff() : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
+}
+
+// Workgroups of a CU, by their registers and LDS.
+constexpr int groups_per_cu(int dim, int tiles) {
+  return dim == 64 ? (tiles == 1 ? 3 : 2) : dim == 128 && tiles == 1 ? 2 : 1;
+}
+
+// kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
+template <int D, int kTiles, bool kSplit>
+__global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
+    attention_split_kernel(const AttentionArgs p, int min_quota) {
   using L = Layout<D>;
+  constexpr int kRows = 16 * kTiles;
   constexpr int kTileBytes = kTokens * L::kPitch;
   constexpr int kJoinPitch = D + 4;  // floats
-  constexpr int kJoinBytes = kRows * kJoinPitch * 4;
+  constexpr int kJoinBytes = 16 * kJoinPitch * 4;
   constexpr int kWaveBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
   __shared__ __align__(16) char shared[kWaves * kWaveBytes];
-  __shared__ float top[kWaves][kRows], total[kWaves][kRows];
+  __shared__ float tops[kWaves][kRows], sums[kWaves][kRows];
+  // The queries' operands stay in registers, or in LDS where those are taken.
+  constexpr bool kQueriesInLds = D == 256 && kTiles == 2;
+  constexpr int kSteps = L::kChunks * L::kSteps;
+  __shared__ u32x4 queries[kQueriesInLds ? kTiles * kSteps * 64 : 1];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane % 16, group4 = lane / 16;
-  const int seq = blockIdx.y, kv_head = blockIdx.z;
 
-  int q_begin = seq, q_count = 1;
-  if (p.q_starts) {
-    q_begin = min(max(p.q_starts[seq], 0), p.tokens);
-    q_count = min(max(p.q_starts[seq + 1], q_begin), p.tokens) - q_begin;
+  Run run;
+  Place place;
+  if constexpr (kSplit) {
+    const int64_t total = all_tiles(p, kRows, lane);
+    run.quota = max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota));
+    run.begin = blockIdx.x * run.quota;
+    run.end = min(run.begin + run.quota, total);
+    if (threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
+    if (run.begin >= total) return;
+    place = find_tile(p, kRows, lane, run.begin, 0, 0);
+  } else {
+    place.seq = blockIdx.x / p.cache.heads;
+    place.head = blockIdx.x % p.cache.heads;
+    place.tile = 0;
+    place.tiles = split_tiles(sequence(p, place.seq), kRows);
+    if (place.tiles == 0) return;
+    run = {0, place.tiles, place.tiles};
   }
-  const int row0 = blockIdx.x * kRows, rows = min(q_count, p.max_q) * p.group;
-  if (row0 >= rows) return;
-  const int page_size = 1 << p.cache.page_shift;
-  const int64_t capacity = int64_t(p.table_width) << p.cache.page_shift;
-  const int context = int(min(int64_t(max(p.context_lens[seq], 0)), capacity));
+  // Where this lane's rows of 16 tokens start, and its place in the LDS tile.
+  const uint32_t code_at = column * (D / 2) + group4 * (L::kChunk / 2);
+  const uint32_t scale_at = column * L::kScaleBytes + group4 * L::kChunk / kFp4Block;
+  char* const tile = shared + wave * kWaveBytes;
+  char* const to = tile + column * L::kPitch + group4 * L::kChunk * 2;
+  const char* const from = tile + (4 * group4 + column / 4) * L::kPitch + (column % 4) * 8;
+  const int page_mask = (1 << p.cache.page_shift) - 1;
 
-  // The lane's row: its query, and the tokens [low, high) that it attends to.
-  const int row = row0 + column;
-  const bool live_row = row < rows;
-  const int query = live_row ? row / p.group : 0;
-  const int head = kv_head * p.group + (live_row ? row % p.group : 0);
-  const int high = live_row ? context - q_count + query + 1 : 0;
-  const int low = p.window ? max(high - p.window, 0) : 0;
-  // Tokens that any row of the tile attends to.
-  const int last_query = min(row0 + kRows - 1, rows - 1) / p.group;
-  const int tile_high = max(context - q_count + last_query + 1, 0);
-  const int first_high = context - q_count + row0 / p.group + 1;
-  const int tile_low = p.window ? max(first_high - p.window, 0) : 0;
-  const int last_low = p.window ? max(tile_high - p.window, 0) : 0;
+  for (int64_t at = run.begin; at < run.end;) {
+    const int seq = place.seq, kv_head = place.head;
+    const Sequence s = sequence(p, seq);
+    const int take = int(min(int64_t(place.tiles - place.tile), run.end - at));
+    const int t_begin = s.first_tile() + place.tile, t_end = t_begin + take;
 
-  u32x4 q[L::kChunks][L::kSteps];
+    // The lane's rows: their queries, and the tokens [low, high) that each attends to.
+    int low[kTiles], high[kTiles];
+    u32x4 q[kTiles][L::kChunks][L::kSteps];
+    if (kQueriesInLds) __syncthreads();  // the last ones are read
 #pragma unroll
-  for (int u = 0; u < L::kChunks; ++u)
-#pragma unroll
-    for (int j = 0; j < L::kSteps; ++j) {
-      q[u][j] = u32x4{0, 0, 0, 0};
-      if (live_row)
-        q[u][j] = *reinterpret_cast<const u32x4*>(
-            p.q.data + int64_t(q_begin + query) * p.q.token_stride + head * p.q.head_stride +
-            (4 * u + group4) * L::kChunk + 8 * j);
-    }
-
-  char* tile = shared + wave * kWaveBytes;
-  f32x4 o[D / 16];
-#pragma unroll
-  for (int m = 0; m < D / 16; ++m) o[m] = f32x4{0, 0, 0, 0};
-  float reference = kLowest, sum = 0;
-
-  const int first_tile = tile_low / kTokens, tiles = (tile_high + kTokens - 1) / kTokens;
-  for (int t = first_tile + wave; t < tiles; t += kWaves) {
-    Raw<D> k[2], v[2];
-    bool there[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int token = t * kTokens + 16 * h;
-      int page = -1;
-      if (token < context) page = p.page_table[int64_t(seq) * p.table_width +
-                                               (token >> p.cache.page_shift)];
-      there[h] = page >= 0 && page < p.cache.pages;
-      const bool live = there[h] && token + lane % 16 < context;
-      const int64_t row_in_page =
-          (int64_t(kv_head) << p.cache.page_shift) + (token & (page_size - 1));
-      const int64_t at = there[h] ? page : 0;
-      k[h] = load_rows<D>(p.cache.k.codes + at * p.cache.k.code_stride + row_in_page * (D / 2),
-                          p.cache.k.scales + at * p.cache.k.scale_stride +
-                              row_in_page * L::kScaleBytes,
-                          lane, live);
-      v[h] = load_rows<D>(p.cache.v.codes + at * p.cache.v.code_stride + row_in_page * (D / 2),
-                          p.cache.v.scales + at * p.cache.v.scale_stride +
-                              row_in_page * L::kScaleBytes,
-                          lane, live);
-    }
-    // Scores, lane: row `column`, tokens 4 * group4 + i of each half.
-    f32x4 s[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] = f32x4{0, 0, 0, 0};
+    for (int n = 0; n < kTiles; ++n) {
+      const int row = 16 * n + column;
+      const bool live = row < s.rows;
+      const int query = live ? row / p.group : 0;
+      high[n] = live ? s.shift + query + 1 : 0;
+      low[n] = p.window ? max(high[n] - p.window, 0) : 0;
+      const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
+                            int64_t(kv_head * p.group + (live ? row % p.group : 0)) *
+                                p.q.head_stride;
 #pragma unroll
       for (int u = 0; u < L::kChunks; ++u)
 #pragma unroll
-        for (int j = 0; j < L::kSteps; ++j)
-          s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8,
-                                 fp4_to_bf16x8(k[h].codes[u][j], fp4_scale(k[h].scales[u]))),
-              __builtin_bit_cast(bf16x8, q[u][j]), s[h], 0, 0, 0);
+        for (int j = 0; j < L::kSteps; ++j) {
+          const int step = (n * L::kChunks + u) * L::kSteps + j;
+          const u32x4* at =
+              reinterpret_cast<const u32x4*>(src + (4 * u + group4) * L::kChunk + 8 * j);
+          if constexpr (!kQueriesInLds)
+            q[n][u][j] = *at;
+          else if (step % kWaves == wave)
+            queries[step * 64 + lane] = *at;
+        }
+      // Rows that are not there repeat a row that is; their results go nowhere.
     }
-    // V into the LDS tile; rows that are not there hold zeros, and so do blocks that are NaN where
-    // some row does not see their token: its weight of 0 would not keep them out.
-    const bool edge = (t + 1) * kTokens > first_high || t * kTokens < last_low;
-    uint32_t poisoned[2] = {0, 0};
-    if (edge) {
+    if (kQueriesInLds) __syncthreads();
+
+    f32x4 o[kTiles][D / 16];
+    float reference[kTiles], sum[kTiles];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) o[n][m] = f32x4{0, 0, 0, 0};
+      reference[n] = kLowest;
+      sum[n] = 0;
+    }
+
+    // This wave's tiles are t_begin + wave, + kWaves, ...; lane 2i + h holds the page of half h
+    // of the i-th, for 32 of them.
+    int pages = -1;
+    auto load_pages = [&](int first) {
+      const int t = first + (lane >> 1) * kWaves;
+      const int token = t * kTokens + 16 * (lane & 1);
+      pages = -1;
+      if (t < t_end && token < s.context)
+        pages = p.page_table[int64_t(seq) * p.table_width + (token >> p.cache.page_shift)];
+      if (uint32_t(pages) >= uint32_t(p.cache.pages)) pages = -1;
+    };
+    // Pages of the i-th tile's halves: their places in the cache, and whether they are there.
+    struct Place2 {
+      int64_t page[2];
+      uint32_t row[2];
+      bool there[2];
+    };
+    auto place_of = [&](int tile_index, int i) {
+      Place2 x;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int page = __builtin_amdgcn_readlane(pages, 2 * i + h);
+        x.there[h] = page >= 0;
+        x.page[h] = max(page, 0);
+        x.row[h] = uint32_t(tile_index * kTokens + 16 * h) & page_mask;
+      }
+      return x;
+    };
+    auto load = [&](Raw<D>(&raw)[2], const Fp4Rows& rows, const Place2& x) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = (int64_t(kv_head) << p.cache.page_shift) + x.row[h];
+        load_rows<D>(raw[h], rows.codes + x.page[h] * rows.code_stride + row * (D / 2),
+                     rows.scales + x.page[h] * rows.scale_stride + row * L::kScaleBytes, code_at,
+                     scale_at);
+      }
+    };
+
+    // Keys and values of a tile each take the registers of the last as soon as those are used.
+    Raw<D> k[2], v[2];
+    Place2 now = {}, next = {};
+    int t = t_begin + wave, i = 0;
+    if (t < t_end) {
+      load_pages(t);
+      now = place_of(t, 0);
+      load(k, p.cache.k, now);
+      load(v, p.cache.v, now);
+    }
+    while (t < t_end) {
+      const int t_next = t + kWaves;
+      const bool more = t_next < t_end;
+      if (++i == 32) {
+        load_pages(t_next);
+        i = 0;
+      }
+      next = place_of(t_next, i);
+
+      // Tiles that some row sees in part, or that are not whole.
+      const bool edge = (t + 1) * kTokens > s.first_high || t * kTokens < s.last_low ||
+                        !now.there[0] || !now.there[1];
+      // Scores, lane: row `column`, tokens 4 * group4 + i of each half.
+      f32x4 score[kTiles][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
+        for (int n = 0; n < kTiles; ++n) score[n][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
         for (int u = 0; u < L::kChunks; ++u)
-          if (v[h].scales[u] >= 253) {
-            poisoned[h] |= 1u << ((4 * u + group4) * L::kChunk / kFp4Block);
 #pragma unroll
-            for (int j = 0; j < L::kSteps; ++j) v[h].codes[u][j] = 0;
-            v[h].scales[u] = 0;
+          for (int j = 0; j < L::kSteps; ++j) {
+            const bf16x8 a = __builtin_bit_cast(
+                bf16x8, fp4_to_bf16x8(k[h].codes[u][j], fp4_scale(k[h].scales[u])));
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+              score[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  a,
+                  __builtin_bit_cast(
+                      bf16x8, kQueriesInLds
+                                  ? queries[((n * L::kChunks + u) * L::kSteps + j) * 64 + lane]
+                                  : q[n][u][j]),
+                  score[n][h], 0, 0, 0);
           }
-        poisoned[h] |= uint32_t(__shfl_xor(int(poisoned[h]), 16, 64));
-        poisoned[h] |= uint32_t(__shfl_xor(int(poisoned[h]), 32, 64));
       }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int u = 0; u < L::kChunks; ++u)
-#pragma unroll
-        for (int j = 0; j < L::kSteps; ++j)
-          *reinterpret_cast<u32x4*>(tile + (16 * h + lane % 16) * L::kPitch +
-                                    ((4 * u + group4) * L::kChunk + 8 * j) * 2) =
-              fp4_to_bf16x8(v[h].codes[u][j], fp4_scale(v[h].scales[u]));
+      if (more) load(k, p.cache.k, next);
 
-    float most = kLowest;
+      uint32_t poisoned[2] = {0, 0};
+      if (edge) {
+        // Values of tokens past the context or of no page are zeros, and so are blocks that are
+        // NaN, since some row may not see their token and its weight of 0 would not keep them out.
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const int token = t * kTokens + 16 * h + column;
+          const bool real = now.there[h] && token < s.context;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int token = t * kTokens + 16 * h + 4 * group4 + i;
-        const bool seen = there[h] && token >= low && token < high;
-        s[h][i] = seen ? s[h][i] * p.scale_log2 : -__builtin_inff();
-        most = fmaxf(most, s[h][i]);
+          for (int u = 0; u < L::kChunks; ++u) {
+            if (!real || v[h].scales[u] >= 253) {
+              if (real) poisoned[h] |= 1u << ((4 * u + group4) * L::kChunk / kFp4Block);
+#pragma unroll
+              for (int j = 0; j < L::kSteps; ++j) v[h].codes[u][j] = 0;
+              v[h].scales[u] = 0;
+            }
+          }
+          poisoned[h] |= uint32_t(__shfl_xor(int(poisoned[h]), 16, 64));
+          poisoned[h] |= uint32_t(__shfl_xor(int(poisoned[h]), 32, 64));
+        }
       }
-    most = fmaxf(most, __shfl_xor(most, 16, 64));
-    most = fmaxf(most, __shfl_xor(most, 32, 64));
-    if (__any(most > reference)) {
-      const float next = fmaxf(most, reference);
-      const float factor = __builtin_amdgcn_exp2f(reference - next);
-      reference = next;
-      sum *= factor;
+      wave_order();
 #pragma unroll
-      for (int m = 0; m < D / 16; ++m) o[m] *= factor;
-    }
-    float w[8];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int u = 0; u < L::kChunks; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[4 * h + i] = __builtin_amdgcn_exp2f(s[h][i] - reference);
-        sum += w[4 * h + i];
-      }
-    const u32x4 weights = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]),
+          for (int j = 0; j < L::kSteps; ++j)
+            *reinterpret_cast<u32x4*>(to + 16 * h * L::kPitch + (4 * u * L::kChunk + 8 * j) * 2) =
+                fp4_to_bf16x8(v[h].codes[u][j], fp4_scale(v[h].scales[u]));
+      wave_order();
+      if (more) load(v, p.cache.v, next);
+
+      u32x4 weights[kTiles];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        float most = kLowest;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) score[n][h][j] *= p.scale_log2;
+        if (edge) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int token = t * kTokens + 16 * h + 4 * group4 + j;
+              if (!(now.there[h] && token >= low[n] && token < high[n]))
+                score[n][h][j] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most = fmaxf(most, score[n][h][j]);
+        if (__any(most > reference[n] + kSlack)) {
+          most = fmaxf(most, __shfl_xor(most, 16, 64));
+          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          most = fmaxf(most, reference[n]);
+          const float factor = __builtin_amdgcn_exp2f(reference[n] - most);
+          reference[n] = most;
+          sum[n] *= factor;
+#pragma unroll
+          for (int m = 0; m < D / 16; ++m) o[n][m] *= factor;
+        }
+        float w[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[4 * h + j] = __builtin_amdgcn_exp2f(score[n][h][j] - reference[n]);
+            sum[n] += w[4 * h + j];
+          }
+        weights[n] = u32x4{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]),
                            pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])};
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const char* from = tile + (4 * group4 + column / 4) * L::kPitch + (column % 4) * 8;
+      }
 #pragma unroll
-    for (int m = 0; m < D / 16; ++m) {
-      const u32x2 a = lds_read_transposed(from + 32 * m);
-      const u32x2 b = lds_read_transposed(from + 16 * L::kPitch + 32 * m);
-      o[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]}),
-          __builtin_bit_cast(bf16x8, weights), o[m], 0, 0, 0);
+      for (int m = 0; m < D / 16; ++m) {
+        const u32x2 a = lds_read_transposed(from + 32 * m);
+        const u32x2 b = lds_read_transposed(from + 16 * L::kPitch + 32 * m);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+          o[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]}),
+              __builtin_bit_cast(bf16x8, weights[n]), o[n][m], 0, 0, 0);
+      }
+      if (edge && __any(poisoned[0] | poisoned[1])) {
+        for (int token = 0; token < kTokens; ++token) {
+          const uint32_t blocks = uint32_t(__shfl(int(poisoned[token / 16]), token % 16, 64));
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+            if (t * kTokens + token >= low[n] && t * kTokens + token < high[n]) {
+#pragma unroll
+              for (int m = 0; m < D / 16; ++m)
+                o[n][m] += blocks >> (m / 2) & 1 ? __builtin_nanf("") : 0.f;
+            }
+        }
+      }
+      now = next;
+      t = t_next;
     }
-    if (edge && __any(poisoned[0] | poisoned[1])) {
-      for (int i = 0; i < kTokens; ++i) {
-        const uint32_t blocks = uint32_t(__shfl(int(poisoned[i / 16]), i % 16, 64));
-        const int token = t * kTokens + i;
-        if (token < low || token >= high) continue;
+
+    // Joins the waves: one tile of rows at a time through LDS. Lane numbers are taken anew, so
+    // that nothing of this is computed ahead and held through the loop above.
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, column = lane % 16, group4 = lane / 16;
 #pragma unroll
-        for (int m = 0; m < D / 16; ++m)
-          if (blocks >> (m / 2) & 1) o[m] += __builtin_nanf("");
+    for (int n = 0; n < kTiles; ++n) {
+      sum[n] += __shfl_xor(sum[n], 16, 64);
+      sum[n] += __shfl_xor(sum[n], 32, 64);
+      if (lane < 16) {
+        tops[wave][16 * n + lane] = reference[n];
+        sums[wave][16 * n + lane] = sum[n];
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
-
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  if (lane < kRows) {
-    top[wave][lane] = reference;
-    total[wave][lane] = sum;
-  }
-  __syncthreads();
-  float highest = kLowest;
+    __syncthreads();
+    const bool whole = place.tile == 0 && take == place.tiles;
+    const int part = 2 * blockIdx.x + (place.tile == 0 ? 1 : 0);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) highest = fmaxf(highest, top[w][column]);
-  const float factor = __builtin_amdgcn_exp2f(reference - highest);
-  float* join = reinterpret_cast<float*>(shared + wave * kWaveBytes);
+    for (int n = 0; n < kTiles; ++n) {
+      float top = kLowest;
 #pragma unroll
-  for (int m = 0; m < D / 16; ++m)
-    *reinterpret_cast<f32x4*>(join + column * kJoinPitch + 16 * m + 4 * group4) = o[m] * factor;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * D / 4; i += 64 * kWaves) {
-    const int r = i / (D / 4), channel = i % (D / 4) * 4;
-    if (row0 + r >= rows) continue;
-    float m = kLowest, l = 0;
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w][16 * n + column]);
+      const float factor = __builtin_amdgcn_exp2f(reference[n] - top);
+      float* join = reinterpret_cast<float*>(tile) + column * kJoinPitch + 4 * group4;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, top[w][r]);
-    f32x4 x = {0, 0, 0, 0};
+      for (int m = 0; m < D / 16; ++m) *reinterpret_cast<f32x4*>(join + 16 * m) = o[n][m] * factor;
+      __syncthreads();
+      for (int i = thread; i < 16 * D / 4; i += 64 * kWaves) {
+        const int r = i / (D / 4), row = 16 * n + r, channel = i % (D / 4) * 4;
+        if (row >= s.rows) continue;
+        float all = kLowest, l = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      l += total[w][r] * __builtin_amdgcn_exp2f(top[w][r] - m);
-      x += *reinterpret_cast<const f32x4*>(shared + w * kWaveBytes +
-                                           (r * kJoinPitch + channel) * 4);
+        for (int w = 0; w < kWaves; ++w) all = fmaxf(all, tops[w][row]);
+        f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          l += sums[w][row] * __builtin_amdgcn_exp2f(tops[w][row] - all);
+          x += *reinterpret_cast<const f32x4*>(shared + w * kWaveBytes +
+                                               (r * kJoinPitch + channel) * 4);
+        }
+        if (!kSplit || whole) {
+          write_row4(p, D, s.q_begin, row, kv_head, channel, x, all, l);
+        } else {
+          *reinterpret_cast<f32x4*>(part_sums<D, kTiles>(p, part) + row * D + channel) = x;
+          if (channel == 0) {
+            float* stats = part_stats<D, kTiles>(p, part) + row * 2;
+            stats[0] = all;
+            stats[1] = l;
+          }
+        }
+      }
+      __syncthreads();
     }
-    const float inv = l == 0 ? 0.f : 1.f / l;
-    const int64_t at = int64_t(q_begin + (row0 + r) / p.group) * p.q.heads + kv_head * p.group +
-                       (row0 + r) % p.group;
-    u32x2 packed = {pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
-    *reinterpret_cast<u32x2*>(p.out + at * D + channel) = packed;
-    if (p.lse && channel == 0)
-      p.lse[at] = l == 0 ? -__builtin_inff()
-                         : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+    if (kSplit && !whole && place.tile == 0 && threadIdx.x == 0) {
+      const int64_t last = at + place.tiles - 1;
+      joints<D>(p)[blockIdx.x] = {int(last / run.quota) - int(blockIdx.x) + 1, s.q_begin, s.rows,
+                                  kv_head};
+    }
+    // On to the next key head or sequence.
+    at += take;
+    if (at < run.end) {
+      place.tile = 0;
+      if (place.head + 1 < p.cache.heads) {
+        ++place.head;
+      } else {
+        place = find_tile(p, kRows, lane, at, place.seq + 1, at);
+      }
+    }
   }
+}
+
+// Joins the parts of the context that workgroup blockIdx.x of the split kernel began. Slices of
+// the channels go to blockIdx.y; groups of threads take every so many parts.
+template <int D, int kTiles>
+__global__ void __launch_bounds__(512) attention_join_kernel(const AttentionArgs p) {
+  constexpr int kSlices = D / 64, kRows = 16 * kTiles, kLanes = 16;  // lanes of a row's slice
+  const Joint joint = joints<D>(p)[blockIdx.x];
+  if (joint.parts == 0) return;
+  static_assert(kSlices * 64 == D);
+  __shared__ f32x4 sums[512];
+  __shared__ float tops[kRows], totals[kRows];
+  auto part = [&](int i) { return i == 0 ? 2 * int(blockIdx.x) + 1 : 2 * (int(blockIdx.x) + i); };
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int row = wave; row < joint.rows; row += 8) {
+    float top = kLowest, total = 0;
+    for (int i = lane; i < joint.parts; i += 64)
+      top = fmaxf(top, part_stats<D, kTiles>(p, part(i))[2 * row]);
+#pragma unroll
+    for (int step = 32; step >= 1; step /= 2) top = fmaxf(top, __shfl_xor(top, step, 64));
+    for (int i = lane; i < joint.parts; i += 64) {
+      const float* stats = part_stats<D, kTiles>(p, part(i)) + 2 * row;
+      total += stats[1] * __builtin_amdgcn_exp2f(stats[0] - top);
+    }
+#pragma unroll
+    for (int step = 32; step >= 1; step /= 2) total += __shfl_xor(total, step, 64);
+    if (lane == 0) {
+      tops[row] = top;
+      totals[row] = total;
+    }
+  }
+  __syncthreads();
+  // rows * 16 lanes are one group; as many groups as fit.
+  const int width = joint.rows * kLanes, groups = 512 / width, group = threadIdx.x / width;
+  const int row = threadIdx.x % width / kLanes;
+  const int channel = blockIdx.y * 64 + threadIdx.x % kLanes * 4;
+  f32x4 x = {0, 0, 0, 0};
+  if (group < groups) {
+    const float top = tops[row];
+#pragma unroll 4
+    for (int i = group; i < joint.parts; i += groups)
+      x += *reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel) *
+           __builtin_amdgcn_exp2f(part_stats<D, kTiles>(p, part(i))[2 * row] - top);
+  }
+  sums[threadIdx.x] = x;
+  __syncthreads();
+  if (group == 0) {
+    for (int g = 1; g < groups; ++g) x += sums[g * width + threadIdx.x];
+    write_row4(p, D, joint.q_begin, row, joint.head, channel, x, tops[row], totals[row]);
+  }
+}
+
+// Up to this many tiles of the longest context a workgroup takes a whole context.
+constexpr int kWholeTiles = 64;
+
+template <int D, int kTiles>
+hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
+  const int64_t longest = (int64_t(args.table_width) << args.cache.page_shift) / kTokens;
+  const int64_t span = args.window ? (args.window + args.max_q) / kTokens + 2 : longest;
+  if ((longest < span ? longest : span) <= kWholeTiles) {
+    attention_split_kernel<D, kTiles, false>
+        <<<uint32_t(args.seqs) * args.cache.heads, 64 * kWaves, 0, stream>>>(args, 0);
+    return hipGetLastError();
+  }
+  const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
+  const int groups = cus * groups_per_cu(D, kTiles);
+  static_assert(2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
+                    kAttentionWorkspaceRows * 2 - 4096 * 4,
+                "parts, statistics and descriptions fit the workspace");
+  attention_split_kernel<D, kTiles, true><<<groups, 64 * kWaves, 0, stream>>>(args, kWaves);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  attention_join_kernel<D, kTiles><<<dim3(groups, D / 64), 512, 0, stream>>>(args);
+  return hipGetLastError();
 }
 
 }  // namespace
 
+hipError_t launch_attention_split(const AttentionArgs& args, int dim, int rows,
+                                  hipStream_t stream) {
+  if (rows <= 16) {
+    switch (dim) {
+      case 64: return launch_split<64, 1>(args, stream);
+      case 128: return launch_split<128, 1>(args, stream);
+      default: return launch_split<256, 1>(args, stream);
+    }
+  }
+  switch (dim) {
+    case 64: return launch_split<64, 2>(args, stream);
+    case 128: return launch_split<128, 2>(args, stream);
+    default: return launch_split<256, 2>(args, stream);
+  }
+}
+
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  const int64_t rows = int64_t(args.max_q < args.tokens ? args.max_q : args.tokens) * args.group;
-  const dim3 grid(uint32_t((rows + kRows - 1) / kRows), args.seqs, args.cache.heads);
-  switch (dim) {
-    case 64: attention_kernel<64, 4><<<grid, 256, 0, stream>>>(args); break;
-    case 128: attention_kernel<128, 4><<<grid, 256, 0, stream>>>(args); break;
-    default: attention_kernel<256, 4><<<grid, 256, 0, stream>>>(args); break;
+  // Sequences of at most `few` rows go to the split kernel, the others to the prompt kernel;
+  // 16 or 32 so that the usual decode fits.
+  const int64_t most = int64_t(args.max_q) * args.group;
+  const int few = most <= 16 || (most > 32 && args.group <= 16) ? 16 : 32;
+  if (args.group <= few) {
+    if (const hipError_t e = launch_attention_split(args, dim, few, stream); e != hipSuccess)
+      return e;
   }
-  return hipGetLastError();
+  return most > few ? launch_attention_prompt(args, dim, few, stream) : hipSuccess;
 }
 
 }  // namespace ci8
