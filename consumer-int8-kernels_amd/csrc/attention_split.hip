@@ -24,8 +24,7 @@
 // sequences and key heads are laid end to end and each workgroup takes an equal run of them.
 // A run that covers a whole context writes its output; parts of one go to the workspace, two
 // at most a workgroup, and a second kernel joins them in a fixed order.
-#include "attention_launch.h"
-#include "fp4_device.h"
+#include "attention_device.h"
 #include "launch.h"
 
 namespace ci8 {
@@ -33,21 +32,6 @@ namespace {
 
 constexpr int kTokens = 32;  // tokens a wave takes at once
 constexpr int kWaves = 8;
-constexpr float kLowest = -3.402823466e38f;
-// How far a score may pass the reference, as a power of two of its weight: sums of 2^31 such
-// weights stay in FP32, and BF16 weights are as exact at any size.
-constexpr float kSlack = 8.f;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// Four values of one channel from four token rows, transposed on the way out of LDS: of each 16
-// lanes, lanes 4j .. 4j+3 address row j (8 bytes each) and lane i gets column i of the rows.
-__device__ __forceinline__ u32x2 lds_read_transposed(const char* p) {
-  return __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                 (lds_s16x4*)reinterpret_cast<const s16x4*>(p)));
-}
 
 // Keeps LDS accesses of a wave's lanes in program order; the LDS itself does.
 __device__ __forceinline__ void wave_order() {
@@ -88,55 +72,10 @@ __device__ __forceinline__ void load_rows(Raw<D>& r, const uint8_t* codes, const
   }
 }
 
-// What one sequence asks for.
-struct Sequence {
-  int q_begin, rows;        // first query row, and rows of (query, head) computed
-  int context, shift;       // tokens; position of query 0
-  int low, high;            // tokens that any row attends to
-  int first_high, last_low; // every row attends to [last_low, first_high)
-  __device__ int first_tile() const { return low / kTokens; }
-  __device__ int tiles() const { return (high + kTokens - 1) / kTokens - first_tile(); }
-};
-
-__device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int seq) {
-  Sequence s;
-  s.q_begin = seq;
-  int count = 1;
-  if (p.q_starts) {
-    s.q_begin = min(max(p.q_starts[seq], 0), p.tokens);
-    count = min(max(p.q_starts[seq + 1], s.q_begin), p.tokens) - s.q_begin;
-  }
-  const int shown = min(count, p.max_q);
-  s.rows = shown * p.group;
-  const int64_t capacity = int64_t(p.table_width) << p.cache.page_shift;
-  s.context = int(min(int64_t(max(p.context_lens[seq], 0)), capacity));
-  s.shift = s.context - count;
-  s.high = max(s.shift + shown, 0);
-  s.first_high = s.shift + 1;
-  s.low = p.window ? max(s.first_high - p.window, 0) : 0;
-  s.last_low = p.window ? max(s.high - p.window, 0) : 0;
-  return s;
-}
-
 // Tiles of a sequence that the split kernel has, at least one (it writes the rows that attend
 // to nothing): 0 without rows, or with more than `most`, which are the prompt kernel's.
 __device__ __forceinline__ int split_tiles(const Sequence& s, int most) {
-  return s.rows == 0 || s.rows > most ? 0 : max(s.tiles(), 1);
-}
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return int64_t(uint64_t(uint32_t(uniform(int(v)))) | uint64_t(uint32_t(uniform(int(v >> 32)))) << 32);
-}
-
-// Inclusive sums over the lanes.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    const int below = __shfl_up(v, step, 64);
-    if (lane >= step) v += below;
-  }
-  return v;
+  return s.rows == 0 || s.rows > most ? 0 : max(s.tiles(kTokens), 1);
 }
 
 // A run of tiles: [begin, end) of the row of all sequences' tiles, one after the other for each
@@ -207,19 +146,6 @@ __device__ __forceinline__ Joint* joints(const AttentionArgs& p) {
   return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 4096;
 }
 
-__device__ __forceinline__ void write_row4(const AttentionArgs& p, int dim, int q_begin, int row,
-                                           int kv_head, int channel, const f32x4& x, float top,
-                                           float sum) {
-  const float inv = sum == 0 ? 0.f : 1.f / sum;
-  const int64_t at = int64_t(q_begin + row / p.group) * p.q.heads + kv_head * p.group +
-                     row % p.group;
-  *reinterpret_cast<u32x2*>(p.out + at * dim + channel) =
-      u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
-  if (p.lse && channel == 0)
-    p.lse[at] =
-        sum == 0 ? -__builtin_inff() : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
-}
-
 // Workgroups of a CU, by their registers and LDS.
 constexpr int groups_per_cu(int dim, int tiles) {
   return dim == 64 ? (tiles == 1 ? 3 : 2) : dim == 128 && tiles == 1 ? 2 : 1;
@@ -276,7 +202,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
     const int seq = place.seq, kv_head = place.head;
     const Sequence s = sequence(p, seq);
     const int take = int(min(int64_t(place.tiles - place.tile), run.end - at));
-    const int t_begin = s.first_tile() + place.tile, t_end = t_begin + take;
+    const int t_begin = s.first_tile(kTokens) + place.tile, t_end = t_begin + take;
 
     // The lane's rows: their queries, and the tokens [low, high) that each attends to.
     int low[kTiles], high[kTiles];
@@ -672,7 +598,10 @@ hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t 
   // Sequences of at most `few` rows go to the split kernel, the others to the prompt kernel;
   // 16 or 32 so that the usual decode fits.
   const int64_t most = int64_t(args.max_q) * args.group;
-  const int few = most <= 16 || (most > 32 && args.group <= 16) ? 16 : 32;
+  int few = most <= 16 || (most > 32 && args.group <= 16) ? 16 : 32;
+  // No sequence can be that short where all others at their longest leave more than that: then
+  // the prompt kernel has them all.
+  if (most > few && (args.tokens - int64_t(args.seqs - 1) * args.max_q) * args.group > few) few = 0;
   if (args.group <= few) {
     if (const hipError_t e = launch_attention_split(args, dim, few, stream); e != hipSuccess)
       return e;
