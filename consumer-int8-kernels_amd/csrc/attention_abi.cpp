@@ -2,6 +2,7 @@
 // validation, then the launch. Pure host code up to the launch.
 #include "consumer_int8_attention.h"
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -356,7 +357,8 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
   args.workspace = static_cast<float*>(workspace);
   args.out = static_cast<uint16_t*>(out);
   args.lse = lse;
-  args.scale_log2 = float(scale * 1.4426950408889634);
+  args.scale_log2 = std::fmax(std::fabs(float(scale * 1.4426950408889634)), FLT_MIN);
+  args.q_sign = scale < 0 ? 0x80008000u : 0;
   args.table_width = int(table_width);
   args.seqs = int(seqs);
   args.tokens = int(tokens);

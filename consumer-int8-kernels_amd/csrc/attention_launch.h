@@ -61,7 +61,10 @@ struct AttentionArgs {
   float* workspace;
   uint16_t* out;
   float* lse;  // may be null
-  float scale_log2;  // scale * log2(e)
+  // |scale| * log2(e), at least the smallest normal number (scores of -inf stay that, and finite
+  // ones become 0), and the sign bits of a BF16 pair where scale is negative.
+  float scale_log2;
+  uint32_t q_sign;
   int table_width, seqs, tokens, group, max_q, window;
 };
 // Sequences of at most `rows` (16 or 32) rows, and those of more than `few`.

@@ -30,12 +30,24 @@ struct Shape {
   static constexpr int kRows = 32 * kTiles * kWaves;
   static constexpr int kTokens = D == 64 ? 128 : D == 128 ? 64 : 32;
   static constexpr int kBlocks = D / kFp4Block;
-  // Byte pitches of LDS rows: reads of 8 lanes' 16 bytes, and of 4 rows' 32 bytes transposed,
-  // fall on different banks.
-  static constexpr int kKeyPitch = 2 * D + 16, kValuePitch = 2 * D + 32;
+  // Byte pitch of LDS rows of keys: 16 of them, 16 bytes each, fall on different banks. Rows of
+  // values are not padded; their pieces trade places instead (value_at), so that transposed
+  // reads of 64 bytes of 4 tokens, and writes of 16 lanes' pieces, fall on different banks.
+  static constexpr int kKeyPitch = 2 * D + 16, kValuePitch = 2 * D;
   static constexpr int kKeyBytes = kTokens * kKeyPitch, kValueBytes = kTokens * kValuePitch;
   static constexpr int kPacks = 2 * kTokens * kBlocks / kThreads;  // 16 bytes of codes a thread
   static_assert(2 * kTokens * kBlocks % kThreads == 0);
+  static constexpr int kKeyBuffers = 3;
+  static constexpr int kLdsBytes = kKeyBuffers * kKeyBytes + 2 * kValueBytes;
+  static_assert(kKeyBuffers * kKeyBytes % 256 == 0);
+  // Byte of piece j (8 channels) of a token's block in a buffer of values: among the 256 bytes
+  // that hold it, blocks are XORed by the token, and in a block the pieces are.
+  __device__ static constexpr int value_at(int token, int block, int j) {
+    return D == 64 ? token * kValuePitch + 64 * (block ^ (token >> 1 & 1)) +
+                         16 * (j ^ (token >> 1 & 3))
+                   : token * kValuePitch + 256 * (block / 4) + 64 * (block % 4 ^ token % 4) +
+                         16 * (j ^ (D == 128 ? token % 4 : token % 2 * 2 + block / 4));
+  }
 };
 
 // Row tiles of a sequence that this kernel has.
@@ -78,10 +90,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   using S = Shape<D>;
   constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = kTokens / 32;
   constexpr int kSteps = D / 16, kChannels = D / 32;
-  // Keys of tile t are read in the steps of tiles t - 1 and t, values in that of t.
-  __shared__ __align__(16) char keys[3][S::kKeyBytes];
-  __shared__ __align__(16) char values[2][S::kValueBytes];
-  __shared__ uint32_t there_words[3][kTokens / 16];       // whether 16 tokens' page is
+  constexpr bool kTwoGroups = S::kWaves == 8, kAhead = kTwoGroups;
+  // Three buffers of keys, then two of values.
+  __shared__ __align__(256) char lds[S::kLdsBytes];
+  constexpr int kValues = S::kKeyBuffers * S::kKeyBytes;
   __shared__ uint8_t poison[2][kTokens][S::kBlocks];      // NaN blocks of edge tiles
   __shared__ int poisoned[2];                             // the last such tile that has any
 
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
                           int64_t(kv_head * p.group + (live ? row % p.group : 0)) * p.q.head_stride;
 #pragma unroll
     for (int j = 0; j < kSteps; ++j)
-      q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half);
+      q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
   }
   // Tokens that all, or any, of the wave's live rows attend to.
   const int wave_last = min(wave_row + 32 * kTiles - 1, s.rows - 1);
@@ -145,116 +157,169 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     sum[n] = 0;
   }
 
-  // Staging. Pack c of a thread is 32 channels of one token, of the keys first, then of the
-  // values. `page` is loaded a tile ahead of the codes, these a tile ahead of their use.
-  constexpr int kPerTile = kTokens * S::kBlocks;
-  struct Staged {
-    u32x4 codes;
-    uint32_t scale;
-    int page;
+  // Pages outside the cache are rare: whether there are any is found once.
+  const int context_page = max(s.context - 1, 0) >> p.cache.page_shift;
+  const int32_t* const table = p.page_table + int64_t(where.seq) * p.table_width;
+  bool missing = false;
+  if (t_begin < t_end) {
+    const int last = min((t_end * kTokens - 1) >> p.cache.page_shift, context_page);
+    for (int i = (t_begin * kTokens >> p.cache.page_shift) + thread; i <= last; i += S::kThreads)
+      missing = missing || uint32_t(table[i]) >= uint32_t(p.cache.pages);
+  }
+  if (thread < 2) poisoned[thread] = -1;
+  const bool any_missing = __syncthreads_or(missing);
+
+  // Staging. A thread converts 32 channels of one token a pack; a wave's packs are all of the keys
+  // or all of the values, of one page or two. Pages are looked up a tile ahead of the codes, these
+  // are loaded a tile ahead of their use. Past the last tile this goes on with tokens that are
+  // there, into buffers that nobody reads, since branches would cost more.
+  constexpr int kPerTile = kTokens * S::kBlocks, kWaveTokens = 64 / S::kBlocks;
+  constexpr bool kTwoPages = kWaveTokens > 16;
+  static_assert(kPerTile % 64 == 0 && kWaveTokens <= 32);
+  u32x4 staged_codes[S::kPacks];
+  uint32_t staged_scales[S::kPacks];
+  int pages[S::kPacks];
+  const int lane_token = lane / S::kBlocks, block = lane % S::kBlocks;
+  const int page_mask = (1 << p.cache.page_shift) - 1;
+  // Scales are loaded as the words that hold them: a loop-carried byte would be masked, and so
+  // waited for, at the loop's end.
+  const uint32_t scale_byte = lane_token % 16 * S::kBlocks + block, scale_shift = scale_byte % 4 * 8;
+  struct Pack {
+    bool value;
+    int token;                // the wave's first in a tile
+    const uint8_t *codes, *scales;  // of this head's rows in page 0, at the lane's place
+    int64_t code_stride, scale_stride;
+    int to[4];                // LDS bytes of the lane's four pieces in the first buffer
   };
-  Staged staged[S::kPacks];
-  auto is_value = [&](int c) __attribute__((always_inline)) { return c * S::kThreads + thread >= kPerTile; };
-  auto token_of = [&](int c) __attribute__((always_inline)) { return (c * S::kThreads + thread) % kPerTile / S::kBlocks; };
-  auto block_of = [&](int c) __attribute__((always_inline)) { return thread % S::kBlocks; };
-  auto page_of = [&](int t, int c) __attribute__((always_inline)) {
-    const int token = t * kTokens + token_of(c);
-    int page = -1;
-    if (t < t_end && token < s.context)
-      page = p.page_table[int64_t(where.seq) * p.table_width + (token >> p.cache.page_shift)];
-    return uint32_t(page) < uint32_t(p.cache.pages) ? page : -1;
+  auto pack = [&](int c) __attribute__((always_inline)) {
+    Pack x;
+    x.value = c * S::kThreads + 64 * wave >= kPerTile;
+    x.token = (c * S::kThreads + 64 * wave) % kPerTile / S::kBlocks;
+    const Fp4Rows& rows = x.value ? p.cache.v : p.cache.k;
+    const int64_t row = int64_t(kv_head) << p.cache.page_shift;
+    x.codes = rows.codes + row * (D / 2) + lane_token % 16 * (D / 2) + 16 * block;
+    x.scales = rows.scales + row * S::kBlocks + (scale_byte & ~3u);
+    x.code_stride = rows.code_stride;
+    x.scale_stride = rows.scale_stride;
+    const int token = x.token + lane_token;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x.to[j] = x.value ? kValues + S::value_at(token, block, j)
+                        : token * S::kKeyPitch + 64 * block + 16 * j;
+    return x;
   };
-  int next_page[S::kPacks];
+  Pack packs[S::kPacks];
+#pragma unroll
+  for (int c = 0; c < S::kPacks; ++c) packs[c] = pack(c);
+  // Makes page lookups vector loads: scalar ones would be waited for with every LDS read.
+  int lane_zero = 0;
+  asm volatile("" : "+v"(lane_zero));
   // Tiles of the keys and of the values.
   auto load_pages = [&](int tk, int tv) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < S::kPacks; ++c) next_page[c] = page_of(is_value(c) ? tv : tk, c);
+    for (int c = 0; c < S::kPacks; ++c) {
+      const int token = (packs[c].value ? tv : tk) * kTokens + packs[c].token;
+      const int at = (kTwoPages ? token + (lane_token & 16) : token + lane_zero) >> p.cache.page_shift;
+      pages[c] = table[min(at, context_page)];
+    }
   };
   auto load_codes = [&](int tk, int tv) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
-      const int t = is_value(c) ? tv : tk;
-      staged[c].page = next_page[c];
-      staged[c].codes = u32x4{0, 0, 0, 0};
-      staged[c].scale = 0;
-      if (staged[c].page >= 0) {
-        const Fp4Rows& rows = is_value(c) ? p.cache.v : p.cache.k;
-        const int64_t row = (int64_t(kv_head) << p.cache.page_shift) +
-                            ((t * kTokens + token_of(c)) & ((1 << p.cache.page_shift) - 1));
-        staged[c].codes = *reinterpret_cast<const u32x4*>(
-            rows.codes + staged[c].page * rows.code_stride + row * (D / 2) + 16 * block_of(c));
-        staged[c].scale = rows.scales[staged[c].page * rows.scale_stride + row * S::kBlocks + block_of(c)];
+      const Pack& x = packs[c];
+      const int token = (x.value ? tv : tk) * kTokens + x.token;
+      auto offsets = [&](int page, int first, int64_t& code, int64_t& scale)
+          __attribute__((always_inline)) {
+        // Loads stay in the cache.
+        const int64_t at = uint32_t(page) < uint32_t(p.cache.pages) ? page : 0;
+        const int row = first & page_mask;
+        code = at * x.code_stride + row * (D / 2);
+        scale = at * x.scale_stride + row * S::kBlocks;
+      };
+      int64_t code, scale;
+      offsets(uniform(pages[c]), token, code, scale);
+      if constexpr (kTwoPages) {
+        int64_t code2, scale2;
+        offsets(__builtin_amdgcn_readlane(pages[c], 16 * S::kBlocks), token + 16, code2, scale2);
+        code = lane_token >= 16 ? code2 : code;
+        scale = lane_token >= 16 ? scale2 : scale;
       }
+      staged_codes[c] = *reinterpret_cast<const u32x4*>(x.codes + code);
+      staged_scales[c] = *reinterpret_cast<const uint32_t*>(x.scales + scale);
     }
+  };
+  auto there = [&](int token) __attribute__((always_inline)) {
+    return uint32_t(table[min(token >> p.cache.page_shift, context_page)]) < uint32_t(p.cache.pages);
   };
   auto edge_tile = [&](int t) __attribute__((always_inline)) {
     return (t + 1) * kTokens > first_high || t * kTokens < last_low;
   };
-  auto store_tiles = [&](int tk, int tv) __attribute__((always_inline)) {
+  // key_buffer: where tile tk goes, t % 3 of some count.
+  auto store_tiles = [&](int key_buffer, int tv) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
-      const int token = token_of(c), block = block_of(c);
-      const bool value = is_value(c);
-      const int t = value ? tv : tk, buffer = value ? t & 1 : t % 3;
-      if (t >= t_end) continue;
-      Staged x = staged[c];
-      if (value && edge_tile(t)) {
-        const bool nan = x.scale >= 253;
-        poison[buffer][token][block] = nan;
-        if (nan) {
-          poisoned[buffer] = t;
-          x.codes = u32x4{0, 0, 0, 0};
-          x.scale = 0;
-        }
+      const Pack& x = packs[c];
+      u32x4 codes = staged_codes[c];
+      uint32_t scale = staged_scales[c] >> scale_shift & 0xFF;
+      if (x.value && (edge_tile(tv) || any_missing)) {
+        // Values of no page or past the context are zeros, and so are an edge tile's NaN blocks.
+        const int token = tv * kTokens + x.token + lane_token;
+        const bool real = token < s.context && (!any_missing || there(token));
+        const bool nan = real && scale >= 253 && edge_tile(tv);
+        poison[tv & 1][x.token + lane_token][block] = nan;
+        if (nan) poisoned[tv & 1] = tv;
+        codes = nan || !real ? u32x4{0, 0, 0, 0} : codes;
+        scale = nan || !real ? 0 : scale;
       }
-      if (!value && block == 0 && token % 16 == 0) there_words[buffer][token / 16] = x.page >= 0;
-      char* to = value ? values[buffer] + token * S::kValuePitch : keys[buffer] + token * S::kKeyPitch;
+      const int buffer = x.value ? (tv & 1) * S::kValueBytes : key_buffer * S::kKeyBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<u32x4*>(to + 64 * block + 16 * j) =
-            fp4_to_bf16x8(x.codes[j], fp4_scale(x.scale));
+        *reinterpret_cast<u32x4*>(lds + (x.to[j] + buffer)) =
+            fp4_to_bf16x8(codes[j], fp4_scale(scale));
     }
   };
 
-  // Half b of tile t is 32 tokens; its scores are computed while the half before is weighed.
-  auto multiply = [&](int t, int b, f32x16(&score)[kTiles], uint32_t& holes)
-      __attribute__((always_inline)) {
-    const char* from = keys[t % 3] + (32 * b + column) * S::kKeyPitch + 16 * half;
-    holes = (there_words[t % 3][2 * b] ? 0u : 1u) | (there_words[t % 3][2 * b + 1] ? 0u : 2u);
+  // Half b of tile t is 32 tokens.
+  u32x4 key[kSteps];
+  auto read_keys = [&](int buffer, int b) __attribute__((always_inline)) {
+    const char* from = lds + buffer * S::kKeyBytes + (32 * b + column) * S::kKeyPitch + 16 * half;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) key[j] = *reinterpret_cast<const u32x4*>(from + 32 * j);
+  };
+  auto multiply = [&](f32x16(&score)[kTiles]) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) score[n][i] = 0;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(from + 32 * j);
+    for (int j = 0; j < kSteps; ++j)
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
         score[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, q[n][j]), score[n], 0, 0, 0);
-    }
+            __builtin_bit_cast(bf16x8, key[j]), __builtin_bit_cast(bf16x8, q[n][j]), score[n], 0,
+            0, 0);
   };
 
-  u32x4 weights[kTiles][2];
-  auto weigh = [&](int first, f32x16(&score)[kTiles], uint32_t holes)
-      __attribute__((always_inline)) {
-    const bool edge = first + 32 > all_high || first < all_low || holes;
+  // Hides what rows do not attend to, and moves their references where scores pass them.
+  auto settle = [&](int first, f32x16(&score)[kTiles]) __attribute__((always_inline)) {
+    const bool edge = first > all_high - 32 || first < all_low || any_missing;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) score[n][i] *= p.scale_log2;
       if (edge) {
+        const bool low_there = !any_missing || there(first);
+        const bool high_there = !any_missing || there(first + 16);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int at = 8 * (i / 4) + i % 4, token = first + at + 4 * half;
-          const bool hidden =
-              (token < row_low[n]) | (token >= row_high[n]) | ((holes >> (at / 16) & 1) != 0);
-          score[n][i] = hidden ? -__builtin_inff() : score[n][i];
+          const bool seen = (token >= row_low[n]) & (token < row_high[n]) &
+                            (at < 16 ? low_there : high_there);
+          score[n][i] = seen ? score[n][i] : -__builtin_inff();
         }
       }
-      float most = kLowest;
+      float most = score[n][0];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) most = fmaxf(most, score[n][i]);
+      for (int i = 1; i < 16; ++i) most = fmaxf(most, score[n][i]);
+      most *= p.scale_log2;
       if (__any(most > reference[n] + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         most = fmaxf(most, reference[n]);
@@ -264,10 +329,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 #pragma unroll
         for (int m = 0; m < kChannels; ++m) o[n][m] *= factor;
       }
+    }
+  };
+  u32x4 weights[kTiles][2];
+  auto weigh = [&](f32x16(&score)[kTiles]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
       float total[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        score[n][i] = __builtin_amdgcn_exp2f(score[n][i] - reference[n]);
+        score[n][i] = __builtin_amdgcn_exp2f(fmaf(score[n][i], p.scale_log2, -reference[n]));
         total[i % 2] += score[n][i];
       }
       sum[n] += total[0] + total[1];
@@ -278,22 +349,33 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
           weights[n][c][i] = pack_bf16x2(score[n][8 * c + 2 * i], score[n][8 * c + 2 * i + 1]);
     }
   };
-  auto add_values = [&](int t, int half_tile) __attribute__((always_inline)) {
-    const char* from = values[t & 1] +
-                       (32 * half_tile + 4 * half + lane % 16 / 4) * S::kValuePitch +
-                       (16 * (lane / 16 % 2) + 4 * (lane % 4)) * 2;
+  u32x4 value[2][kChannels];
+  auto read_values = [&](int t, int b) __attribute__((always_inline)) {
+    // The lane's row of four and its 8 bytes of the 64 that two groups of 16 lanes read: piece
+    // 2 * (lane / 16 % 2) + lane % 4 / 2. Tokens of other fours keep its place in the row.
+    const int row = 4 * half + lane % 16 / 4, piece = 2 * (lane / 16 % 2) + lane % 4 / 2;
+    const char* from = lds + (kValues + (t & 1) * S::kValueBytes + 32 * b * S::kValuePitch) +
+                       lane % 2 * 8;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int m = 0; m < kChannels; ++m) {
-        const u32x2 a = lds_read_transposed(from + 16 * c * S::kValuePitch + 64 * m);
-        const u32x2 b = lds_read_transposed(from + (16 * c + 8) * S::kValuePitch + 64 * m);
+        const char* at = from + S::value_at(row, m, piece) + 16 * c * S::kValuePitch;
+        const u32x2 x = lds_read_transposed(at);
+        const u32x2 y = lds_read_transposed(at + 8 * S::kValuePitch);
+        value[c][m] = u32x4{x[0], x[1], y[0], y[1]};
+      }
+  };
+  auto add_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int m = 0; m < kChannels; ++m)
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
           o[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]}),
-              __builtin_bit_cast(bf16x8, weights[n][c]), o[n][m], 0, 0, 0);
-      }
+              __builtin_bit_cast(bf16x8, value[c][m]), __builtin_bit_cast(bf16x8, weights[n][c]),
+              o[n][m], 0, 0, 0);
   };
   // NaN blocks of an edge tile's values stand as zeros; rows that see their token get the NaN.
   auto add_poison = [&](int t) __attribute__((always_inline)) {
@@ -308,54 +390,83 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         }
   };
 
-  f32x16 scores[2][kTiles];
-  uint32_t holes[2];
-  if (thread < 2) poisoned[thread] = -1;
-  __syncthreads();
+  f32x16 scores[kTiles];
+  // A phase ends where all waves meet; nothing is moved over that.
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (t_begin < t_end) {
-    // Keys run a tile ahead of values.
-    load_pages(t_begin, t_end);
-    load_codes(t_begin, t_end);
+    // In a tile's step the keys of the next tile but one are staged, and the values of the next.
+    load_pages(t_begin, t_begin);
+    load_codes(t_begin, t_begin);
     load_pages(t_begin + 1, t_begin);
-    store_tiles(t_begin, t_end);
+    store_tiles(0, t_begin);
     load_codes(t_begin + 1, t_begin);
     load_pages(t_begin + 2, t_begin + 1);
-    store_tiles(t_begin + 1, t_begin);
+    store_tiles(1, t_begin);
     load_codes(t_begin + 2, t_begin + 1);
     load_pages(t_begin + 3, t_begin + 2);
     __syncthreads();
-    multiply(t_begin, 0, scores[0], holes[0]);
-    __syncthreads();
+    read_keys(0, 0);
+    multiply(scores);
+    if (kAhead) {
+      read_keys(1 / kHalves, 1 % kHalves);
+      read_values(t_begin, 0);
+    }
   }
-  // Scores alternate between two sets of registers; tiles of one half are unrolled in pairs.
-  auto step = [&](int t, auto parity) __attribute__((always_inline)) {
-    constexpr int first = kHalves % 2 == 0 ? 0 : decltype(parity)::value;
+  // The second half of the waves is one phase behind the first.
+  const bool behind = kTwoGroups && wave >= S::kWaves / 2;
+  if (behind) meet();
+  int buffer[3] = {0, 1, 2};  // of the keys of this tile and the next two
+  for (int t = t_begin; t < t_end; ++t) {
 #pragma unroll
     for (int b = 0; b < kHalves; ++b) {
-      const int now = (first + b) % 2, after = 1 - now;
-      if (b + 1 < kHalves)
-        multiply(t, b + 1, scores[after], holes[after]);
-      else if (t + 1 < t_end)
-        multiply(t + 1, 0, scores[after], holes[after]);
-      weigh(t * kTokens + 32 * b, scores[now], holes[now]);
-      if (b == 0) {
-        store_tiles(t + 2, t + 1);
+      // Vector phase: weighs this half's scores.
+      if (!kAhead) read_keys(buffer[1], 0);
+      settle(t * kTokens + 32 * b, scores);
+      weigh(scores);
+      if (kTwoGroups) meet();
+      // Matrix phase: this half's values, the next half's scores (past the last tile those of old
+      // keys, which nothing reads), the operands after those, and the staging.
+      __builtin_amdgcn_s_setprio(1);
+      if (!kAhead) read_values(t, b);
+      multiply(scores);
+      if (kAhead) read_keys(buffer[(b + 2) / kHalves], (b + 2) % kHalves);
+      add_values();
+      if (kAhead) read_values(t + (b + 1) / kHalves, (b + 1) % kHalves);
+      if (b == 0) store_tiles(buffer[2], t + 1);
+      if (b == kHalves - 1) {
         load_codes(t + 3, t + 2);
         load_pages(t + 4, t + 3);
       }
-      add_values(t, b);
+      // Two waves of a SIMD are in different phases, and inside this one LDS reads and vector
+      // instructions go between the MFMAs.
+      if (kAhead) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x006, 4, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * kChannels; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x006, 4, 0);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if (b + 1 == kHalves && edge_tile(t) && poisoned[t & 1] == t) add_poison(t);
+      if (kTwoGroups || b + 1 == kHalves) meet();
     }
-    if (edge_tile(t) && poisoned[t & 1] == t) add_poison(t);
-    __syncthreads();
-  };
-  for (int t = t_begin; t < t_end;) {
-    step(t, std::integral_constant<int, 0>{});
-    ++t;
-    if (kHalves % 2 == 0) continue;
-    if (t >= t_end) break;
-    step(t, std::integral_constant<int, 1>{});
-    ++t;
+    const int first = buffer[0];
+    buffer[0] = buffer[1];
+    buffer[1] = buffer[2];
+    buffer[2] = first;
   }
+  if (kTwoGroups && !behind) meet();
 
   // A row's two lanes hold the sums of their own tokens.
 #pragma unroll

@@ -226,9 +226,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
           const u32x4* at =
               reinterpret_cast<const u32x4*>(src + (4 * u + group4) * L::kChunk + 8 * j);
           if constexpr (!kQueriesInLds)
-            q[n][u][j] = *at;
+            q[n][u][j] = *at ^ p.q_sign;
           else if (step % kWaves == wave)
-            queries[step * 64 + lane] = *at;
+            queries[step * 64 + lane] = *at ^ p.q_sign;
         }
       // Rows that are not there repeat a row that is; their results go nowhere.
     }
@@ -365,11 +365,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
       u32x4 weights[kTiles];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
-        float most = kLowest;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) score[n][h][j] *= p.scale_log2;
+        float most = -__builtin_inff();
         if (edge) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -384,6 +380,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) most = fmaxf(most, score[n][h][j]);
+        most *= p.scale_log2;
         if (__any(most > reference[n] + kSlack)) {
           most = fmaxf(most, __shfl_xor(most, 16, 64));
           most = fmaxf(most, __shfl_xor(most, 32, 64));
@@ -399,7 +396,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            w[4 * h + j] = __builtin_amdgcn_exp2f(score[n][h][j] - reference[n]);
+            w[4 * h + j] =
+                __builtin_amdgcn_exp2f(fmaf(score[n][h][j], p.scale_log2, -reference[n]));
             sum[n] += w[4 * h + j];
           }
         weights[n] = u32x4{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]),
