@@ -55,10 +55,21 @@ __device__ __forceinline__ int row_tiles(const Sequence& s, int few, int rows) {
   return s.rows <= few ? 0 : (s.rows + rows - 1) / rows;
 }
 
-// Which sequence and row tile: `index` counts all sequences' tiles.
+// Row tiles of all sequences, and the one that `index` counts to.
 struct RowTile {
   int seq, tile, tiles;  // seq < 0: past the last
 };
+__device__ __forceinline__ int all_row_tiles(const AttentionArgs& p, int few, int rows, int lane) {
+  int total = 0;
+  for (int base = 0; base < p.seqs; base += 64) {
+    int n = 0;
+    if (base + lane < p.seqs) n = row_tiles(sequence(p, base + lane), few, rows);
+#pragma unroll
+    for (int step = 32; step >= 1; step /= 2) n += __shfl_xor(n, step, 64);
+    total += n;
+  }
+  return uniform(total);
+}
 __device__ __forceinline__ RowTile find_row_tile(const AttentionArgs& p, int few, int rows,
                                                  int index, int lane) {
   for (int base = 0; base < p.seqs; base += 64) {
@@ -76,7 +87,26 @@ __device__ __forceinline__ RowTile find_row_tile(const AttentionArgs& p, int few
   return {-1, 0, 0};
 }
 
-// Parts of the workspace: [unit][split][row][D] and the statistics after them.
+// Units of work are (row tile, key head). One a CU, they run in rounds; those of a last round that
+// does not fill the GPU have their contexts cut, so that it does.
+struct Cut {
+  int units, whole, splits;  // units from `whole` on are cut
+};
+__device__ __forceinline__ Cut cut_units(const AttentionArgs& p, int few, int rows, int cus,
+                                         int most_splits, int lane) {
+  Cut c;
+  c.units = all_row_tiles(p, few, rows, lane) * p.cache.heads;
+  const int rest = c.units % cus;
+  c.whole = c.units - rest;
+  c.splits = rest ? min(cus / rest, most_splits) : 1;
+  if (c.splits <= 1) {
+    c.splits = 1;
+    c.whole = c.units;
+  }
+  return c;
+}
+
+// Parts of the workspace: [cut unit][split][row][D] and the statistics after them.
 __device__ __forceinline__ float* part_sums(const AttentionArgs& p, int64_t row, int dim) {
   return p.workspace + row * dim;
 }
@@ -86,7 +116,7 @@ __device__ __forceinline__ float* part_stats(const AttentionArgs& p, int64_t row
 
 template <int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads)
-    attention_prompt_kernel(const AttentionArgs p, int few, int splits) {
+    attention_prompt_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
   using S = Shape<D>;
   constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = kTokens / 32;
   constexpr int kSteps = D / 16, kChannels = D / 32;
@@ -100,7 +130,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6);
   const int column = lane & 31, half = lane >> 5;
   const int heads = p.cache.heads;
-  const int split = blockIdx.x % splits, unit = blockIdx.x / splits;
+  int unit = blockIdx.x, split = 0, splits = 1, part = 0;
+  if (most_splits > 1) {
+    const Cut c = cut_units(p, few, S::kRows, cus, most_splits, lane);
+    if (unit >= c.whole) {
+      splits = c.splits;
+      part = unit - c.whole;
+      unit = c.whole + part / splits;
+      split = part % splits;
+    }
+  }
   const int kv_head = unit % heads;
   const RowTile where = find_row_tile(p, few, S::kRows, unit / heads, lane);
   if (where.seq < 0) return;
@@ -115,10 +154,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   const int last_low = p.window ? max(high - p.window, 0) : 0;
   int t_begin = tile_low / kTokens, t_end = (high + kTokens - 1) / kTokens;
   if (splits > 1) {
-    const int n = max(t_end - t_begin, 0), part = (n + splits - 1) / splits;
+    const int n = max(t_end - t_begin, 0), each = (n + splits - 1) / splits;
     const int end = t_end;
-    t_begin = min(t_begin + split * part, end);
-    t_end = min(t_begin + part, end);
+    t_begin = min(t_begin + split * each, end);
+    t_end = min(t_begin + each, end);
   }
 
   // The lane's rows and their tokens [low, high).
@@ -146,14 +185,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   const int all_low = p.window ? max(any_high - p.window, 0) : 0;
 
   f32x16 o[kTiles][kChannels];
-  float reference[kTiles], sum[kTiles];
+  float reference[kTiles], limit[kTiles], sum[kTiles];
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
     for (int m = 0; m < kChannels; ++m)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[n][m][i] = 0;
-    reference[n] = kLowest;
+    reference[n] = 0;
+    limit[n] = kLowest;
     sum[n] = 0;
   }
 
@@ -300,8 +340,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
             0, 0);
   };
 
-  // Hides what rows do not attend to, and moves their references where scores pass them.
-  auto settle = [&](int first, f32x16(&score)[kTiles]) __attribute__((always_inline)) {
+  // Scores become exponents x = s * scale - reference; most: the lane's largest.
+  float most[kTiles];
+  auto largest = [&](const f32x16& x) __attribute__((always_inline)) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, x[i]);
+    return m;
+  };
+  auto scale = [&](f32x16(&score)[kTiles]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) score[n][i] = fmaf(score[n][i], p.scale_log2, -reference[n]);
+      most[n] = largest(score[n]);
+    }
+  };
+  // Hides what rows do not attend to, and moves their references where exponents pass the limit:
+  // kSlack, and anything for a row that has seen nothing.
+  auto settle = [&](int first, f32x16(&x)[kTiles]) __attribute__((always_inline)) {
     const bool edge = first > all_high - 32 || first < all_low || any_missing;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
@@ -313,40 +370,43 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
           const int at = 8 * (i / 4) + i % 4, token = first + at + 4 * half;
           const bool seen = (token >= row_low[n]) & (token < row_high[n]) &
                             (at < 16 ? low_there : high_there);
-          score[n][i] = seen ? score[n][i] : -__builtin_inff();
+          x[n][i] = seen ? x[n][i] : -__builtin_inff();
         }
+        most[n] = largest(x[n]);
       }
-      float most = score[n][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) most = fmaxf(most, score[n][i]);
-      most *= p.scale_log2;
-      if (__any(most > reference[n] + kSlack)) {
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        most = fmaxf(most, reference[n]);
-        const float factor = __builtin_amdgcn_exp2f(reference[n] - most);
-        reference[n] = most;
+      if (__any(most[n] > limit[n])) {
+        const float m = fmaxf(most[n], __shfl_xor(most[n], 32, 64));
+        const bool fresh = limit[n] < 0;
+        float next = reference[n];
+        if (fresh ? m > kLowest : m > 0) next += m;
+        const float up = next - reference[n];
+        const float factor = fresh ? 1.f : __builtin_amdgcn_exp2f(-up);
+        if (m > kLowest) limit[n] = kSlack;
+        reference[n] = next;
         sum[n] *= factor;
 #pragma unroll
-        for (int m = 0; m < kChannels; ++m) o[n][m] *= factor;
+        for (int i = 0; i < 16; ++i) x[n][i] -= up;
+#pragma unroll
+        for (int c = 0; c < kChannels; ++c) o[n][c] *= factor;
       }
     }
   };
   u32x4 weights[kTiles][2];
-  auto weigh = [&](f32x16(&score)[kTiles]) __attribute__((always_inline)) {
+  auto weigh = [&](f32x16(&x)[kTiles]) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       float total[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        score[n][i] = __builtin_amdgcn_exp2f(fmaf(score[n][i], p.scale_log2, -reference[n]));
-        total[i % 2] += score[n][i];
+        x[n][i] = __builtin_amdgcn_exp2f(x[n][i]);
+        total[i % 2] += x[n][i];
       }
       sum[n] += total[0] + total[1];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          weights[n][c][i] = pack_bf16x2(score[n][8 * c + 2 * i], score[n][8 * c + 2 * i + 1]);
+          weights[n][c][i] = pack_bf16x2(x[n][8 * c + 2 * i], x[n][8 * c + 2 * i + 1]);
     }
   };
   u32x4 value[2][kChannels];
@@ -411,6 +471,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     __syncthreads();
     read_keys(0, 0);
     multiply(scores);
+    scale(scores);
     if (kAhead) {
       read_keys(1 / kHalves, 1 % kHalves);
       read_values(t_begin, 0);
@@ -427,6 +488,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       if (!kAhead) read_keys(buffer[1], 0);
       settle(t * kTokens + 32 * b, scores);
       weigh(scores);
+      if (b == 0) store_tiles(buffer[2], t + 1);
       if (kTwoGroups) meet();
       // Matrix phase: this half's values, the next half's scores (past the last tile those of old
       // keys, which nothing reads), the operands after those, and the staging.
@@ -436,8 +498,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       if (kAhead) read_keys(buffer[(b + 2) / kHalves], (b + 2) % kHalves);
       add_values();
       if (kAhead) read_values(t + (b + 1) / kHalves, (b + 1) % kHalves);
-      if (b == 0) store_tiles(buffer[2], t + 1);
-      if (b == kHalves - 1) {
+      scale(scores);
+      if (b == 0) {
         load_codes(t + 3, t + 2);
         load_pages(t + 4, t + 3);
       }
@@ -448,13 +510,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         for (int i = 0; i < kSteps; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x006, 4, 0);
         }
 #pragma unroll
         for (int i = 0; i < 2 * kChannels; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          __builtin_amdgcn_sched_group_barrier(0x006, 4, 0);
         }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -472,6 +532,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
     const float total = sum[n] + __shfl_xor(sum[n], 32, 64);
+    const float top = limit[n] < 0 ? kLowest : reference[n];
     const int row = wave_row + 32 * n + column;
     if (row >= s.rows) continue;
     if (splits == 1) {
@@ -480,10 +541,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x4 x = {o[n][m][4 * i], o[n][m][4 * i + 1], o[n][m][4 * i + 2], o[n][m][4 * i + 3]};
-          write_row4(p, D, s.q_begin, row, kv_head, 32 * m + 8 * i + 4 * half, x, reference[n], total);
+          write_row4(p, D, s.q_begin, row, kv_head, 32 * m + 8 * i + 4 * half, x, top, total);
         }
     } else {
-      const int64_t at = int64_t(blockIdx.x) * S::kRows + (row - row0);
+      const int64_t at = int64_t(part) * S::kRows + (row - row0);
 #pragma unroll
       for (int m = 0; m < kChannels; ++m)
 #pragma unroll
@@ -491,31 +552,35 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
           *reinterpret_cast<f32x4*>(part_sums(p, at, D) + 32 * m + 8 * i + 4 * half) =
               f32x4{o[n][m][4 * i], o[n][m][4 * i + 1], o[n][m][4 * i + 2], o[n][m][4 * i + 3]};
       if (half == 0) {
-        part_stats(p, at, D)[0] = reference[n];
+        part_stats(p, at, D)[0] = top;
         part_stats(p, at, D)[1] = total;
       }
     }
   }
 }
 
-// Joins the splits of each row: D / 4 lanes a row.
+// Joins the parts of the rows of cut units: D / 4 lanes a row.
+constexpr int kJoinThreads = 512;
 template <int D>
-__global__ void __launch_bounds__(256) attention_prompt_join_kernel(const AttentionArgs p, int few,
-                                                                    int splits) {
-  constexpr int kRows = Shape<D>::kRows, kLanes = D / 4, kSlices = kRows * kLanes / 256;
-  const int lane = threadIdx.x & 63, slice = blockIdx.x % kSlices, unit = blockIdx.x / kSlices;
+__global__ void __launch_bounds__(kJoinThreads)
+    attention_prompt_join_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
+  constexpr int kRows = Shape<D>::kRows, kLanes = D / 4, kSlices = kRows * kLanes / kJoinThreads;
+  const int lane = threadIdx.x & 63, slice = blockIdx.x % kSlices, cut = blockIdx.x / kSlices;
+  const Cut c = cut_units(p, few, kRows, cus, most_splits, lane);
+  const int unit = c.whole + cut;
+  if (unit >= c.units) return;
   const RowTile where = find_row_tile(p, few, kRows, unit / p.cache.heads, lane);
-  if (where.seq < 0) return;
   const Sequence s = sequence(p, where.seq);
-  const int r = slice * (256 / kLanes) + int(threadIdx.x) / kLanes;
+  const int r = slice * (kJoinThreads / kLanes) + int(threadIdx.x) / kLanes;
   const int channel = threadIdx.x % kLanes * 4;
   const int row = (where.tiles - 1 - where.tile) * kRows + r;
   if (row >= s.rows) return;
-  const int64_t first = int64_t(unit) * splits * kRows + r;
+  const int64_t first = int64_t(cut) * c.splits * kRows + r;
   float top = kLowest, total = 0;
-  for (int i = 0; i < splits; ++i) top = fmaxf(top, part_stats(p, first + int64_t(i) * kRows, D)[0]);
+  for (int i = 0; i < c.splits; ++i)
+    top = fmaxf(top, part_stats(p, first + int64_t(i) * kRows, D)[0]);
   f32x4 x = {0, 0, 0, 0};
-  for (int i = 0; i < splits; ++i) {
+  for (int i = 0; i < c.splits; ++i) {
     const int64_t at = first + int64_t(i) * kRows;
     const float factor = __builtin_amdgcn_exp2f(part_stats(p, at, D)[0] - top);
     total += part_stats(p, at, D)[1] * factor;
@@ -527,25 +592,30 @@ __global__ void __launch_bounds__(256) attention_prompt_join_kernel(const Attent
 template <int D>
 hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream) {
   using S = Shape<D>;
-  const int found = device_cu_count(), cus = found > 0 ? found : 256;
+  const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
+  static_assert(256 * S::kRows <= kAttentionWorkspaceRows, "one part a CU");
   // Row tiles of all sequences, at most: each but its last is full.
-  const int64_t rows = int64_t(args.tokens) * args.group;
   const int64_t each = (int64_t(args.max_q) * args.group + S::kRows - 1) / S::kRows;
-  const int64_t bound = rows / S::kRows + args.seqs;
+  const int64_t bound = int64_t(args.tokens) * args.group / S::kRows + args.seqs;
   const int64_t units = (bound < each * args.seqs ? bound : each * args.seqs) * args.cache.heads;
-  // Contexts are cut where row tiles alone leave CUs idle, into parts of four tiles or more.
+  // Cut into parts of four tiles or more. After many rounds the last one counts for little, and
+  // the last units of prompts without a context before them are short by themselves.
   const int64_t longest = int64_t(args.table_width) << args.cache.page_shift;
-  const int64_t seen = args.window && args.window + args.max_q < longest ? args.window + args.max_q : longest;
-  int64_t splits = cus / units;
-  if (splits > seen / (4 * S::kTokens)) splits = seen / (4 * S::kTokens);
+  const bool windowed = args.window && int64_t(args.window) + args.max_q < longest;
+  const int64_t seen = windowed ? args.window + args.max_q : longest;
+  const int64_t rounds = windowed || longest >= 2 * int64_t(args.max_q) ? 8 : 1;
+  int64_t splits = units <= rounds * cus ? seen / (4 * S::kTokens) : 1;
+  if (splits > cus) splits = cus;
   if (splits < 1) splits = 1;
-  if (units * splits * S::kRows > kAttentionWorkspaceRows && splits > 1)
-    splits = kAttentionWorkspaceRows / (units * S::kRows);
-  attention_prompt_kernel<D><<<uint32_t(units * splits), S::kThreads, 0, stream>>>(args, few, int(splits));
+  const int64_t grid = units + (splits > 1 ? cus : 0);
+  attention_prompt_kernel<D>
+      <<<uint32_t(grid), S::kThreads, 0, stream>>>(args, few, cus, int(splits));
   if (splits == 1) return hipGetLastError();
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  // A unit that is cut has two parts or more.
+  constexpr int kSlices = S::kRows * (D / 4) / kJoinThreads;
   attention_prompt_join_kernel<D>
-      <<<uint32_t(units * (S::kRows * (D / 4) / 256)), 256, 0, stream>>>(args, few, int(splits));
+      <<<uint32_t(cus / 2 * kSlices), kJoinThreads, 0, stream>>>(args, few, cus, int(splits));
   return hipGetLastError();
 }
 
