@@ -160,28 +160,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     t_end = min(t_begin + each, end);
   }
 
-  // The lane's rows and their tokens [low, high).
+  // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
+  // go nowhere.
   int row_low[kTiles], row_high[kTiles];
   u32x4 q[kTiles][kSteps];
   const int wave_row = row0 + wave * 32 * kTiles;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
-    const int row = wave_row + 32 * n + column;
-    const bool live = row < s.rows;
-    const int query = live ? row / p.group : 0;
-    row_high[n] = live ? s.shift + query + 1 : 0;
+    const int row = min(wave_row + 32 * n + column, s.rows - 1), query = row / p.group;
+    row_high[n] = s.shift + query + 1;
     row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
     const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
-                          int64_t(kv_head * p.group + (live ? row % p.group : 0)) * p.q.head_stride;
+                          int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
 #pragma unroll
     for (int j = 0; j < kSteps; ++j)
       q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
   }
-  // Tokens that all, or any, of the wave's live rows attend to.
-  const int wave_last = min(wave_row + 32 * kTiles - 1, s.rows - 1);
-  const bool wave_live = wave_row < s.rows;
-  const int all_high = wave_live ? s.shift + wave_row / p.group + 1 : 0;
-  const int any_high = wave_live ? s.shift + wave_last / p.group + 1 : 0;
+  // Tokens [all_low, all_high) that all of the wave's rows attend to.
+  const int all_high = s.shift + min(wave_row, s.rows - 1) / p.group + 1;
+  const int any_high = s.shift + min(wave_row + 32 * kTiles - 1, s.rows - 1) / p.group + 1;
   const int all_low = p.window ? max(any_high - p.window, 0) : 0;
 
   f32x16 o[kTiles][kChannels];
