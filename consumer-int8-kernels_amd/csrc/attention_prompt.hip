@@ -120,12 +120,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   using S = Shape<D>;
   constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = kTokens / 32;
   constexpr int kSteps = D / 16, kChannels = D / 32;
-  constexpr bool kTwoGroups = S::kWaves == 8, kAhead = kTwoGroups;
   // Three buffers of keys, then two of values.
   __shared__ __align__(256) char lds[S::kLdsBytes];
   constexpr int kValues = S::kKeyBuffers * S::kKeyBytes;
-  __shared__ uint8_t poison[2][kTokens][S::kBlocks];      // NaN blocks of edge tiles
-  __shared__ int poisoned[2];                             // the last such tile that has any
+  __shared__ uint8_t poison[3][kTokens][S::kBlocks];      // NaN blocks of edge tiles
+  __shared__ int poisoned[3];                             // the last such tile that has any
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6);
   const int column = lane & 31, half = lane >> 5;
@@ -203,7 +202,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     for (int i = (t_begin * kTokens >> p.cache.page_shift) + thread; i <= last; i += S::kThreads)
       missing = missing || uint32_t(table[i]) >= uint32_t(p.cache.pages);
   }
-  if (thread < 2) poisoned[thread] = -1;
+  if (thread < 3) poisoned[thread] = -1;
   const bool any_missing = __syncthreads_or(missing);
 
   // Staging. A thread converts 32 channels of one token a pack; a wave's packs are all of the keys
@@ -303,8 +302,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         const int token = tv * kTokens + x.token + lane_token;
         const bool real = token < s.context && (!any_missing || there(token));
         const bool nan = real && scale >= 253 && edge_tile(tv);
-        poison[tv & 1][x.token + lane_token][block] = nan;
-        if (nan) poisoned[tv & 1] = tv;
+        poison[tv % 3][x.token + lane_token][block] = nan;
+        if (nan) poisoned[tv % 3] = tv;
         codes = nan || !real ? u32x4{0, 0, 0, 0} : codes;
         scale = nan || !real ? 0 : scale;
       }
@@ -316,7 +315,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     }
   };
 
-  // Half b of tile t is 32 tokens.
+  // Half b of tile t is 32 tokens. Where registers allow, operands are read from LDS half a step
+  // before their products.
+  constexpr bool kAhead = kHalves > 1;
   u32x4 key[kSteps];
   auto read_keys = [&](int buffer, int b) __attribute__((always_inline)) {
     const char* from = lds + buffer * S::kKeyBytes + (32 * b + column) * S::kKeyPitch + 16 * half;
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     for (int token = 0; token < kTokens; ++token)
 #pragma unroll
       for (int m = 0; m < kChannels; ++m)
-        if (poison[t & 1][token][m]) {
+        if (poison[t % 3][token][m]) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
             if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n])
@@ -448,12 +449,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   };
 
   f32x16 scores[kTiles];
-  // A phase ends where all waves meet; nothing is moved over that.
-  auto meet = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-  };
   if (t_begin < t_end) {
     // In a tile's step the keys of the next tile but one are staged, and the values of the next.
     load_pages(t_begin, t_begin);
@@ -474,21 +469,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       read_values(t_begin, 0);
     }
   }
-  // The second half of the waves is one phase behind the first.
-  const bool behind = kTwoGroups && wave >= S::kWaves / 2;
-  if (behind) meet();
   int buffer[3] = {0, 1, 2};  // of the keys of this tile and the next two
   for (int t = t_begin; t < t_end; ++t) {
 #pragma unroll
     for (int b = 0; b < kHalves; ++b) {
-      // Vector phase: weighs this half's scores.
+      // Weighs this half's scores, and stages what the next halves read.
       if (!kAhead) read_keys(buffer[1], 0);
       settle(t * kTokens + 32 * b, scores);
       weigh(scores);
       if (b == 0) store_tiles(buffer[2], t + 1);
-      if (kTwoGroups) meet();
-      // Matrix phase: this half's values, the next half's scores (past the last tile those of old
-      // keys, which nothing reads), the operands after those, and the staging.
+      // This half's values, the next half's scores (past the last tile those of old keys, which
+      // nothing reads), and the operands after those.
       __builtin_amdgcn_s_setprio(1);
       if (!kAhead) read_values(t, b);
       multiply(scores);
@@ -500,8 +491,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         load_codes(t + 3, t + 2);
         load_pages(t + 4, t + 3);
       }
-      // Two waves of a SIMD are in different phases, and inside this one LDS reads and vector
-      // instructions go between the MFMAs.
+      // LDS reads and vector instructions go between the MFMAs.
       if (kAhead) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -515,15 +505,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (b + 1 == kHalves && edge_tile(t) && poisoned[t & 1] == t) add_poison(t);
-      if (kTwoGroups || b + 1 == kHalves) meet();
+      if (b + 1 == kHalves && edge_tile(t) && poisoned[t % 3] == t) add_poison(t);
+      // One barrier a tile. Before it, what the first half of step t stores was last read in step
+      // t - 1's first half or before; it is read from step t's second half on (with one half, from
+      // step t + 1 on).
+      if (b == 0) {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     const int first = buffer[0];
     buffer[0] = buffer[1];
     buffer[1] = buffer[2];
     buffer[2] = first;
   }
-  if (kTwoGroups && !behind) meet();
 
   // A row's two lanes hold the sums of their own tokens.
 #pragma unroll
