@@ -18,6 +18,8 @@ using ci8::as_stream;
 using ci8::overlap;
 
 constexpr int64_t kMaxExtent = int64_t(1) << 46;  // bytes; far past any buffer of a GPU
+// Where a page begins is held in 32 bits, in 16 bytes of codes and 8 of scales.
+constexpr int64_t kMaxCacheExtent = int64_t(1) << 35;
 using i128 = __int128;
 
 bool dim_ok(int64_t dim) { return dim == 64 || dim == 128 || dim == 256; }
@@ -123,7 +125,7 @@ int check_cache(const ci8_fp4_cache* c, int64_t dim, Extents& e) {
       return abi_fail(CI8_ERR_ALIGNMENT,
                       "The cache requires codes on 16 and scales on 8 bytes, pages too");
     const i128 bytes = i128(c->pages - 1) * strides[i] + page;
-    if (bytes > kMaxExtent) return abi_fail(CI8_ERR_TOO_LARGE, "Cache too large");
+    if (bytes > kMaxCacheExtent) return abi_fail(CI8_ERR_TOO_LARGE, "Cache too large");
     e.bytes[i] = int64_t(bytes);
   }
   return CI8_OK;
@@ -320,7 +322,8 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
     return abi_fail(CI8_ERR_GEOMETRY,
                     "Invalid attention: expected at most 65535 sequences, max_q >= 1, window >= "
                     "0, a finite scale, and q_starts unless each sequence has one query");
-  if (i128(table_width) * cache->page_size > INT_MAX - 4096 ||
+  // Tiles of 32 tokens of 64 sequences are summed in 32 bits.
+  if (i128(table_width) * cache->page_size >= (1 << 30) ||
       i128(seqs) * table_width * 4 > kMaxExtent)
     return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large");
   if (!aligned(page_table, 4) || !aligned(context_lens, 4) || !aligned(q_starts, 4) ||

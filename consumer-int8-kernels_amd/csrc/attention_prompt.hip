@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   const int page_mask = (1 << p.cache.page_shift) - 1;
   // Scales are loaded as the words that hold them: a loop-carried byte would be masked, and so
   // waited for, at the loop's end.
-  const uint32_t scale_byte = lane_token % 16 * S::kBlocks + block, scale_shift = scale_byte % 4 * 8;
+  const uint32_t scale_byte = lane_token % 16 * S::kBlocks + block;
+  const uint32_t scale_turn = fp4_scale_turn(scale_byte % 4);
   struct Pack {
     bool value;
     int token;                // the wave's first in a tile
@@ -296,22 +297,22 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     for (int c = 0; c < S::kPacks; ++c) {
       const Pack& x = packs[c];
       u32x4 codes = staged_codes[c];
-      uint32_t scale = staged_scales[c] >> scale_shift & 0xFF;
+      uint32_t scales = staged_scales[c];
       if (x.value && (edge_tile(tv) || any_missing)) {
         // Values of no page or past the context are zeros, and so are an edge tile's NaN blocks.
         const int token = tv * kTokens + x.token + lane_token;
         const bool real = token < s.context && (!any_missing || there(token));
-        const bool nan = real && scale >= 253 && edge_tile(tv);
+        const bool nan = real && (scales >> scale_byte % 4 * 8 & 0xFF) >= 253 && edge_tile(tv);
         poison[tv % 3][x.token + lane_token][block] = nan;
         if (nan) poisoned[tv % 3] = tv;
         codes = nan || !real ? u32x4{0, 0, 0, 0} : codes;
-        scale = nan || !real ? 0 : scale;
+        scales = nan || !real ? 0 : scales;
       }
       const int buffer = x.value ? (tv & 1) * S::kValueBytes : key_buffer * S::kKeyBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<u32x4*>(lds + (x.to[j] + buffer)) =
-            fp4_to_bf16x8(codes[j], fp4_scale(scale));
+            fp4_to_bf16x8(codes[j], fp4_scale_in(scales, scale_turn));
     }
   };
 

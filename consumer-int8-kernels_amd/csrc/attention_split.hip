@@ -24,6 +24,11 @@
 // sequences and key heads are laid end to end and each workgroup takes an equal run of them.
 // A run that covers a whole context writes its output; parts of one go to the workspace, two
 // at most a workgroup, and a second kernel joins them in a fixed order.
+//
+// Measured, of the cache's bytes: 64 contexts up to 32768 tokens, 64 query heads on 8 of 128, 265
+// us, 5.4 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 44 us, 3.3 TB/s with
+// the join (6 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
+// the launch.
 #include "attention_device.h"
 #include "launch.h"
 
@@ -31,7 +36,6 @@ namespace ci8 {
 namespace {
 
 constexpr int kTokens = 32;  // tokens a wave takes at once
-constexpr int kWaves = 8;
 
 // Keeps LDS accesses of a wave's lanes in program order; the LDS itself does.
 __device__ __forceinline__ void wave_order() {
@@ -50,7 +54,9 @@ struct Layout {
   static constexpr int kScaleBytes = D / kFp4Block;
 };
 
-// Codes and scales of 16 tokens' rows: this lane's token l % 16 and its chunks.
+// Codes and scales of 16 tokens' rows: this lane's token l % 16 and its chunks. Scales stay the
+// words that hold them until they are used: bytes carried round a loop would be masked, and so
+// waited for, at its end.
 template <int D>
 struct Raw {
   uint32_t codes[Layout<D>::kChunks][Layout<D>::kChunk / 8];
@@ -68,7 +74,7 @@ __device__ __forceinline__ void load_rows(Raw<D>& r, const uint8_t* codes, const
     const Words w = *reinterpret_cast<const Words*>(codes + (code_at + u * 2 * L::kChunk));
 #pragma unroll
     for (int j = 0; j < L::kChunk / 8; ++j) r.codes[u][j] = w[j];
-    r.scales[u] = scales[scale_at + u * 4 * L::kChunk / kFp4Block];
+    r.scales[u] = *reinterpret_cast<const uint32_t*>(scales + (scale_at + 4 * u));
   }
 }
 
@@ -87,43 +93,48 @@ struct Place {
   int seq, head, tile, tiles;  // tile: from the sequence's first
 };
 
-__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int lane) {
-  int64_t total = 0;
-  for (int base = 0; base < p.seqs; base += 64) {
-    int n = 0;
-    if (base + lane < p.seqs) n = split_tiles(sequence(p, base + lane), most);
-#pragma unroll
-    for (int step = 32; step >= 1; step /= 2) n += __shfl_xor(n, step, 64);
-    total += n;
-  }
-  return uniform(total * p.cache.heads);
+// Tiles of 64 sequences from `base` on, one a lane, and their sums up to each lane's.
+struct Counted {
+  int base, tiles, sum;
+};
+__device__ __forceinline__ Counted count_tiles(const AttentionArgs& p, int most, int lane,
+                                               int base) {
+  Counted c = {base, 0, 0};
+  if (base + lane < p.seqs) c.tiles = split_tiles(sequence(p, base + lane), most);
+  c.sum = wave_scan(c.tiles, lane);
+  return c;
+}
+// Tiles of all; `first` are those of the first 64 sequences.
+__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int lane,
+                                             const Counted& first) {
+  int64_t total = uniform(__shfl(first.sum, 63, 64));
+  for (int base = 64; base < p.seqs; base += 64)
+    total += uniform(__shfl(count_tiles(p, most, lane, base).sum, 63, 64));
+  return total * p.cache.heads;
 }
 
-// Where tile `at` of all lies; at is less than their number. Continues from `seq0`, which has
-// `before` tiles of all in front.
+// Where tile `at` of all lies; at is less than their number. `first`: of the first 64 sequences.
 __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int lane, int64_t at,
-                                           int seq0, int64_t before) {
-  Place place = {};
+                                           const Counted& first) {
   const int heads = p.cache.heads;
-  for (int base = seq0; base < p.seqs; base += 64) {
-    int n = 0;
-    if (base + lane < p.seqs) n = split_tiles(sequence(p, base + lane), most);
-    const int sum = wave_scan(n, lane);
-    const bool past = before + int64_t(sum) * heads > at;
-    const uint64_t hit = __ballot(past);
-    if (hit) {
-      const int which = __builtin_ctzll(hit);
-      place.seq = base + which;
-      place.tiles = uniform(__shfl(n, which, 64));
-      const int in_front = uniform(__shfl(sum, which, 64)) - place.tiles;
+  Counted c = first;
+  int64_t before = 0;
+  for (;;) {
+    const uint64_t hit = __ballot(before + int64_t(c.sum) * heads > at);
+    if (hit || c.base + 64 >= p.seqs) {
+      const int which = hit ? __builtin_ctzll(hit) : 0;
+      Place place;
+      place.seq = uniform(c.base + which);
+      place.tiles = max(uniform(__shfl(c.tiles, which, 64)), 1);
+      const int in_front = uniform(__shfl(c.sum, which, 64)) - place.tiles;
       const int64_t inside = at - before - int64_t(in_front) * heads;
-      place.head = int(inside / place.tiles);
-      place.tile = int(inside % place.tiles);
+      place.head = uniform(int(inside / place.tiles));
+      place.tile = uniform(int(inside % place.tiles));
       return place;
     }
-    before += int64_t(uniform(__shfl(sum, 63, 64))) * heads;
+    before += int64_t(uniform(__shfl(c.sum, 63, 64))) * heads;
+    c = count_tiles(p, most, lane, c.base + 64);
   }
-  return place;
 }
 
 // Parts in the workspace: of workgroup w, part 2w continues a context, part 2w + 1 begins one.
@@ -146,15 +157,24 @@ __device__ __forceinline__ Joint* joints(const AttentionArgs& p) {
   return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 4096;
 }
 
+// The kernel's first argument, read anew: what one part of a long kernel needs of it is not held
+// in registers through the others.
+__device__ __forceinline__ const AttentionArgs& arguments() {
+  auto* args =
+      (const __attribute__((address_space(4))) AttentionArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  return *(const AttentionArgs*)args;
+}
+
 // Workgroups of a CU, by their registers and LDS.
 constexpr int groups_per_cu(int dim, int tiles) {
-  return dim == 64 ? (tiles == 1 ? 3 : 2) : dim == 128 && tiles == 1 ? 2 : 1;
+  return dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
 }
 
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
-template <int D, int kTiles, bool kSplit>
-__global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
-    attention_split_kernel(const AttentionArgs p, int min_quota) {
+template <int D, int kTiles, int kWaves, bool kSplit>
+__global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) : kWaves / 4)
+    attention_split_kernel(const AttentionArgs, int min_quota) {
   using L = Layout<D>;
   constexpr int kRows = 16 * kTiles;
   constexpr int kTileBytes = kTokens * L::kPitch;
@@ -175,31 +195,36 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
   Run run;
   Place place;
   if constexpr (kSplit) {
-    const int64_t total = all_tiles(p, kRows, lane);
-    run.quota = max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota));
+    const AttentionArgs& p = arguments();
+    const Counted counted = count_tiles(p, kRows, lane, 0);
+    const int64_t total = all_tiles(p, kRows, lane, counted);
+    run.quota = uniform(max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota)));
     run.begin = blockIdx.x * run.quota;
     run.end = min(run.begin + run.quota, total);
     if (threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
     if (run.begin >= total) return;
-    place = find_tile(p, kRows, lane, run.begin, 0, 0);
+    place = find_tile(p, kRows, lane, run.begin, counted);
   } else {
+    const AttentionArgs& p = arguments();
     place.seq = blockIdx.x / p.cache.heads;
     place.head = blockIdx.x % p.cache.heads;
     place.tile = 0;
-    place.tiles = split_tiles(sequence(p, place.seq), kRows);
+    place.tiles = uniform(split_tiles(sequence(p, place.seq), kRows));
     if (place.tiles == 0) return;
     run = {0, place.tiles, place.tiles};
   }
   // Where this lane's rows of 16 tokens start, and its place in the LDS tile.
   const uint32_t code_at = column * (D / 2) + group4 * (L::kChunk / 2);
-  const uint32_t scale_at = column * L::kScaleBytes + group4 * L::kChunk / kFp4Block;
+  const uint32_t scale_byte = column * L::kScaleBytes + group4 * L::kChunk / kFp4Block;
+  const uint32_t scale_at = scale_byte & ~3u, scale_turn = fp4_scale_turn(scale_byte % 4);
   char* const tile = shared + wave * kWaveBytes;
   char* const to = tile + column * L::kPitch + group4 * L::kChunk * 2;
   const char* const from = tile + (4 * group4 + column / 4) * L::kPitch + (column % 4) * 8;
-  const int page_mask = (1 << p.cache.page_shift) - 1;
 
   for (int64_t at = run.begin; at < run.end;) {
     const int seq = place.seq, kv_head = place.head;
+    const AttentionArgs& p = arguments();
+    const int page_mask = (1 << p.cache.page_shift) - 1;
     const Sequence s = sequence(p, seq);
     const int take = int(min(int64_t(place.tiles - place.tile), run.end - at));
     const int t_begin = s.first_tile(kTokens) + place.tile, t_end = t_begin + take;
@@ -244,66 +269,67 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
       sum[n] = 0;
     }
 
-    // This wave's tiles are t_begin + wave, + kWaves, ...; lane 2i + h holds the page of half h
-    // of the i-th, for 32 of them.
-    int pages = -1;
+    // This wave's tiles are t_begin + wave, + kWaves, ...; lane 2i + h holds where the page of half
+    // h of the i-th begins, for 32 of them: in 16 bytes of codes and 8 of scales. Pages outside the
+    // cache begin at 0 and have no bit in `in_cache`.
+    struct {
+      uint32_t k_codes, k_scales, v_codes, v_scales;
+    } at_page;
+    uint64_t in_cache = 0;
     auto load_pages = [&](int first) {
       const int t = first + (lane >> 1) * kWaves;
       const int token = t * kTokens + 16 * (lane & 1);
-      pages = -1;
+      int page = -1;
       if (t < t_end && token < s.context)
-        pages = p.page_table[int64_t(seq) * p.table_width + (token >> p.cache.page_shift)];
-      if (uint32_t(pages) >= uint32_t(p.cache.pages)) pages = -1;
+        page = p.page_table[int64_t(seq) * p.table_width + (token >> p.cache.page_shift)];
+      const bool there = uint32_t(page) < uint32_t(p.cache.pages);
+      in_cache = __ballot(there);
+      const uint32_t safe = there ? page : 0;
+      at_page = {safe * uint32_t(p.cache.k.code_stride >> 4),
+                 safe * uint32_t(p.cache.k.scale_stride >> 3),
+                 safe * uint32_t(p.cache.v.code_stride >> 4),
+                 safe * uint32_t(p.cache.v.scale_stride >> 3)};
     };
-    // Pages of the i-th tile's halves: their places in the cache, and whether they are there.
-    struct Place2 {
-      int64_t page[2];
-      uint32_t row[2];
-      bool there[2];
-    };
-    auto place_of = [&](int tile_index, int i) {
-      Place2 x;
+    const int64_t head_row = int64_t(kv_head) << p.cache.page_shift;
+    const uint8_t* const k_codes = p.cache.k.codes + head_row * (D / 2);
+    const uint8_t* const v_codes = p.cache.v.codes + head_row * (D / 2);
+    const uint8_t* const k_scales = p.cache.k.scales + head_row * L::kScaleBytes;
+    const uint8_t* const v_scales = p.cache.v.scales + head_row * L::kScaleBytes;
+    // Tile t, the i-th of those looked up.
+    auto load = [&](Raw<D>(&raw)[2], const uint8_t* codes, uint32_t code_page,
+                    const uint8_t* scales, uint32_t scale_page, int t, int i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int page = __builtin_amdgcn_readlane(pages, 2 * i + h);
-        x.there[h] = page >= 0;
-        x.page[h] = max(page, 0);
-        x.row[h] = uint32_t(tile_index * kTokens + 16 * h) & page_mask;
-      }
-      return x;
-    };
-    auto load = [&](Raw<D>(&raw)[2], const Fp4Rows& rows, const Place2& x) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t row = (int64_t(kv_head) << p.cache.page_shift) + x.row[h];
-        load_rows<D>(raw[h], rows.codes + x.page[h] * rows.code_stride + row * (D / 2),
-                     rows.scales + x.page[h] * rows.scale_stride + row * L::kScaleBytes, code_at,
-                     scale_at);
+        const uint32_t row = uint32_t(t * kTokens + 16 * h) & page_mask;
+        const uint32_t code = __builtin_amdgcn_readlane(int(code_page), 2 * i + h);
+        const uint32_t scale = __builtin_amdgcn_readlane(int(scale_page), 2 * i + h);
+        load_rows<D>(raw[h], codes + (uint64_t(code) << 4), scales + (uint64_t(scale) << 3),
+                     code_at + row * (D / 2), scale_at + row * L::kScaleBytes);
       }
     };
 
     // Keys and values of a tile each take the registers of the last as soon as those are used.
+    // After the wave's last tile the loads go on with that one again: were they skipped, the waits
+    // for those before would have to be for all.
     Raw<D> k[2], v[2];
-    Place2 now = {}, next = {};
-    int t = t_begin + wave, i = 0;
+    int t = t_begin + wave, i = 0, there = 3;
     if (t < t_end) {
       load_pages(t);
-      now = place_of(t, 0);
-      load(k, p.cache.k, now);
-      load(v, p.cache.v, now);
+      load(k, k_codes, at_page.k_codes, k_scales, at_page.k_scales, t, 0);
+      load(v, v_codes, at_page.v_codes, v_scales, at_page.v_scales, t, 0);
+      there = int(in_cache & 3);
     }
     while (t < t_end) {
-      const int t_next = t + kWaves;
-      const bool more = t_next < t_end;
-      if (++i == 32) {
+      const bool more = t + kWaves < t_end;
+      const int t_next = more ? t + kWaves : t;
+      if (more && ++i == 32) {
         load_pages(t_next);
         i = 0;
       }
-      next = place_of(t_next, i);
 
       // Tiles that some row sees in part, or that are not whole.
       const bool edge = (t + 1) * kTokens > s.first_high || t * kTokens < s.last_low ||
-                        !now.there[0] || !now.there[1];
+                        there != 3;
       // Scores, lane: row `column`, tokens 4 * group4 + i of each half.
       f32x4 score[kTiles][2];
 #pragma unroll
@@ -315,7 +341,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
 #pragma unroll
           for (int j = 0; j < L::kSteps; ++j) {
             const bf16x8 a = __builtin_bit_cast(
-                bf16x8, fp4_to_bf16x8(k[h].codes[u][j], fp4_scale(k[h].scales[u])));
+                bf16x8, fp4_to_bf16x8(k[h].codes[u][j], fp4_scale_in(k[h].scales[u], scale_turn)));
 #pragma unroll
             for (int n = 0; n < kTiles; ++n)
               score[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -327,7 +353,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
                   score[n][h], 0, 0, 0);
           }
       }
-      if (more) load(k, p.cache.k, next);
+      load(k, k_codes, at_page.k_codes, k_scales, at_page.k_scales, t_next, i);
 
       uint32_t poisoned[2] = {0, 0};
       if (edge) {
@@ -336,10 +362,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int token = t * kTokens + 16 * h + column;
-          const bool real = now.there[h] && token < s.context;
+          const bool real = (there >> h & 1) && token < s.context;
 #pragma unroll
           for (int u = 0; u < L::kChunks; ++u) {
-            if (!real || v[h].scales[u] >= 253) {
+            if (!real || (v[h].scales[u] >> scale_byte % 4 * 8 & 0xFF) >= 253) {
               if (real) poisoned[h] |= 1u << ((4 * u + group4) * L::kChunk / kFp4Block);
 #pragma unroll
               for (int j = 0; j < L::kSteps; ++j) v[h].codes[u][j] = 0;
@@ -358,9 +384,9 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
 #pragma unroll
           for (int j = 0; j < L::kSteps; ++j)
             *reinterpret_cast<u32x4*>(to + 16 * h * L::kPitch + (4 * u * L::kChunk + 8 * j) * 2) =
-                fp4_to_bf16x8(v[h].codes[u][j], fp4_scale(v[h].scales[u]));
+                fp4_to_bf16x8(v[h].codes[u][j], fp4_scale_in(v[h].scales[u], scale_turn));
       wave_order();
-      if (more) load(v, p.cache.v, next);
+      load(v, v_codes, at_page.v_codes, v_scales, at_page.v_scales, t_next, i);
 
       u32x4 weights[kTiles];
 #pragma unroll
@@ -372,8 +398,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int token = t * kTokens + 16 * h + 4 * group4 + j;
-              if (!(now.there[h] && token >= low[n] && token < high[n]))
-                score[n][h][j] = -__builtin_inff();
+              const bool seen = (there >> h & 1) & (token >= low[n]) & (token < high[n]);
+              score[n][h][j] = seen ? score[n][h][j] : -__builtin_inff();
             }
         }
 #pragma unroll
@@ -425,12 +451,14 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
             }
         }
       }
-      now = next;
-      t = t_next;
+      there = int(in_cache >> (2 * i) & 3);
+      t += kWaves;
     }
 
     // Joins the waves: one tile of rows at a time through LDS. Lane numbers are taken anew, so
     // that nothing of this is computed ahead and held through the loop above.
+    {
+    const AttentionArgs& p = arguments();
     int thread = threadIdx.x;
     asm volatile("" : "+v"(thread));
     const int lane = thread & 63, column = lane % 16, group4 = lane / 16;
@@ -494,59 +522,94 @@ __global__ void __launch_bounds__(64 * kWaves, 2 * groups_per_cu(D, kTiles))
       if (place.head + 1 < p.cache.heads) {
         ++place.head;
       } else {
-        place = find_tile(p, kRows, lane, at, place.seq + 1, at);
+        // More tiles are left, so a later sequence has some.
+        place.head = 0;
+        do {
+          ++place.seq;
+          place.tiles = uniform(split_tiles(sequence(p, place.seq), kRows));
+        } while (place.tiles == 0 && place.seq + 1 < p.seqs);
       }
+    }
     }
   }
 }
 
-// Joins the parts of the context that workgroup blockIdx.x of the split kernel began. Slices of
-// the channels go to blockIdx.y; groups of threads take every so many parts.
+// Joins the parts of the context that workgroup blockIdx.x of the split kernel began: 32 channels
+// a workgroup, 8 lanes a row; groups of rows * 8 lanes take every so many parts. Bound by the
+// latency of its dependent reads: the sums of the first parts are on their way while the
+// statistics are read, by a row's own lanes where parts are few and by whole waves where many.
+constexpr int kJoinThreads = 256, kJoinChannels = 32;
 template <int D, int kTiles>
-__global__ void __launch_bounds__(512) attention_join_kernel(const AttentionArgs p) {
-  constexpr int kSlices = D / 64, kRows = 16 * kTiles, kLanes = 16;  // lanes of a row's slice
-  const Joint joint = joints<D>(p)[blockIdx.x];
-  if (joint.parts == 0) return;
-  static_assert(kSlices * 64 == D);
-  __shared__ f32x4 sums[512];
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionArgs p) {
+  constexpr int kRows = 16 * kTiles, kLanes = kJoinChannels / 4, kEarly = 4, kFew = 8;
+  static_assert(kRows * kLanes <= kJoinThreads);
+  Joint joint = joints<D>(p)[blockIdx.x];
+  if (joint.parts <= 0) return;
+  // Whatever stands there (a workspace that another stream writes), accesses stay in bounds.
+  joint.parts = min(joint.parts, int(gridDim.x - blockIdx.x));
+  joint.rows = min(max(joint.rows, 1), min(kRows, p.tokens * p.group));
+  joint.q_begin = min(max(joint.q_begin, 0), p.tokens - (joint.rows + p.group - 1) / p.group);
+  joint.head = min(max(joint.head, 0), p.cache.heads - 1);
+  __shared__ f32x4 sums[kJoinThreads];
   __shared__ float tops[kRows], totals[kRows];
   auto part = [&](int i) { return i == 0 ? 2 * int(blockIdx.x) + 1 : 2 * (int(blockIdx.x) + i); };
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int row = wave; row < joint.rows; row += 8) {
-    float top = kLowest, total = 0;
-    for (int i = lane; i < joint.parts; i += 64)
-      top = fmaxf(top, part_stats<D, kTiles>(p, part(i))[2 * row]);
+  const int width = joint.rows * kLanes, groups = kJoinThreads / width;
+  const int group = threadIdx.x / width, row = threadIdx.x % width / kLanes;
+  const int channel = blockIdx.y * kJoinChannels + threadIdx.x % kLanes * 4;
+  auto sum_at = [&](int i) {
+    return reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel);
+  };
+  auto stats_at = [&](int i, int r) { return part_stats<D, kTiles>(p, part(i)) + 2 * r; };
+  f32x4 early[kEarly];
 #pragma unroll
-    for (int step = 32; step >= 1; step /= 2) top = fmaxf(top, __shfl_xor(top, step, 64));
-    for (int i = lane; i < joint.parts; i += 64) {
-      const float* stats = part_stats<D, kTiles>(p, part(i)) + 2 * row;
-      total += stats[1] * __builtin_amdgcn_exp2f(stats[0] - top);
-    }
-#pragma unroll
-    for (int step = 32; step >= 1; step /= 2) total += __shfl_xor(total, step, 64);
-    if (lane == 0) {
-      tops[row] = top;
-      totals[row] = total;
-    }
+  for (int e = 0; e < kEarly; ++e) {
+    early[e] = f32x4{0, 0, 0, 0};
+    const int i = group + e * groups;
+    if (group < groups && i < joint.parts) early[e] = *sum_at(i);
   }
-  __syncthreads();
-  // rows * 16 lanes are one group; as many groups as fit.
-  const int width = joint.rows * kLanes, groups = 512 / width, group = threadIdx.x / width;
-  const int row = threadIdx.x % width / kLanes;
-  const int channel = blockIdx.y * 64 + threadIdx.x % kLanes * 4;
+  float top = kLowest, total = 0;
+  if (joint.parts <= kFew) {
+#pragma unroll 4
+    for (int i = 0; i < joint.parts; ++i) top = fmaxf(top, stats_at(i, row)[0]);
+#pragma unroll 4
+    for (int i = 0; i < joint.parts; ++i)
+      total += stats_at(i, row)[1] * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
+  } else {
+    const int lane = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < joint.rows; r += kJoinThreads / 64) {
+      float m = kLowest, l = 0;
+      for (int i = lane; i < joint.parts; i += 64) m = fmaxf(m, stats_at(i, r)[0]);
+#pragma unroll
+      for (int step = 32; step >= 1; step /= 2) m = fmaxf(m, __shfl_xor(m, step, 64));
+      for (int i = lane; i < joint.parts; i += 64)
+        l += stats_at(i, r)[1] * __builtin_amdgcn_exp2f(stats_at(i, r)[0] - m);
+#pragma unroll
+      for (int step = 32; step >= 1; step /= 2) l += __shfl_xor(l, step, 64);
+      if (lane == 0) {
+        tops[r] = m;
+        totals[r] = l;
+      }
+    }
+    __syncthreads();
+    top = tops[row];
+    total = totals[row];
+  }
   f32x4 x = {0, 0, 0, 0};
   if (group < groups) {
-    const float top = tops[row];
+#pragma unroll
+    for (int e = 0; e < kEarly; ++e) {
+      const int i = group + e * groups;
+      if (i < joint.parts) x += early[e] * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
+    }
 #pragma unroll 4
-    for (int i = group; i < joint.parts; i += groups)
-      x += *reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel) *
-           __builtin_amdgcn_exp2f(part_stats<D, kTiles>(p, part(i))[2 * row] - top);
+    for (int i = group + kEarly * groups; i < joint.parts; i += groups)
+      x += *sum_at(i) * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
   }
   sums[threadIdx.x] = x;
   __syncthreads();
   if (group == 0) {
     for (int g = 1; g < groups; ++g) x += sums[g * width + threadIdx.x];
-    write_row4(p, D, joint.q_begin, row, joint.head, channel, x, tops[row], totals[row]);
+    write_row4(p, D, joint.q_begin, row, joint.head, channel, x, top, total);
   }
 }
 
@@ -557,19 +620,29 @@ template <int D, int kTiles>
 hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
   const int64_t longest = (int64_t(args.table_width) << args.cache.page_shift) / kTokens;
   const int64_t span = args.window ? (args.window + args.max_q) / kTokens + 2 : longest;
+  const int64_t contexts = int64_t(args.seqs) * args.cache.heads;
   if ((longest < span ? longest : span) <= kWholeTiles) {
-    attention_split_kernel<D, kTiles, false>
-        <<<uint32_t(args.seqs) * args.cache.heads, 64 * kWaves, 0, stream>>>(args, 0);
+    // Eight waves where their registers allow: 517 tokens of 8 key heads of 128 7.6 us, four 8.3.
+    constexpr int kWaves = D == 256 && kTiles == 2 ? 4 : 8;
+    attention_split_kernel<D, kTiles, kWaves, false>
+        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, 0);
     return hipGetLastError();
   }
+  // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
+  // 59; 64 up to 32768 264 and 278. At D = 256 contexts that are few get fewer workgroups and so
+  // fewer parts to join: one of 131071 tokens of 4 heads 40 us, with two a CU 48; 32 up to 9000 53
+  // and 50.
+  constexpr int kWaves = 4;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
-  const int groups = cus * groups_per_cu(D, kTiles);
+  const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
                     kAttentionWorkspaceRows * 2 - 4096 * 4,
                 "parts, statistics and descriptions fit the workspace");
-  attention_split_kernel<D, kTiles, true><<<groups, 64 * kWaves, 0, stream>>>(args, kWaves);
+  attention_split_kernel<D, kTiles, kWaves, true>
+      <<<groups, 64 * kWaves, 0, stream>>>(args, 2 * kWaves);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  attention_join_kernel<D, kTiles><<<dim3(groups, D / 64), 512, 0, stream>>>(args);
+  attention_join_kernel<D, kTiles>
+      <<<dim3(groups, D / kJoinChannels), kJoinThreads, 0, stream>>>(args);
   return hipGetLastError();
 }
 

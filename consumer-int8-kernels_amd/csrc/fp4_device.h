@@ -10,6 +10,14 @@ constexpr int kFp4Block = 32;  // channels that share a scale
 // Scale operand of the conversions: the E8M0 byte as an FP32 exponent. 255 converts to NaN.
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+// The same for byte i of a word of scales: the word turned so that the byte is the exponent, one
+// instruction. The conversion to BF16 reads nothing else of it (65536 random words gave what their
+// exponents alone do).
+__device__ __forceinline__ uint32_t fp4_scale_turn(uint32_t i) { return (8 * i + 9) & 31; }
+__device__ __forceinline__ float fp4_scale_in(uint32_t word, uint32_t turn) {
+  return __uint_as_float(__builtin_amdgcn_alignbit(word, word, turn));
+}
+
 // Eight codes (channel 0 in the lowest bits) times the scale, in BF16: exact, since a code has
 // two significant bits.
 __device__ __forceinline__ u32x4 fp4_to_bf16x8(uint32_t codes, float scale) {

@@ -68,7 +68,8 @@ typedef struct ci8_rotation {
   int64_t interleaved;
 } ci8_rotation;
 
-/* The cache above. Codes start on 16 bytes and scales on 8, and so do all their pages. */
+/* The cache above. Codes start on 16 bytes and scales on 8, and so do all their pages; each of
+ * the four spans at most 32 GiB. */
 typedef struct ci8_fp4_cache {
   uint8_t* k_codes;
   uint8_t* k_scales;
@@ -120,7 +121,8 @@ int ci8_unpack_fp4(const ci8_fp4_cache* cache, const int64_t* slots, void* k, vo
  * rows of q in no sequence are not written. Products are BF16 x BF16 with FP32 sums, the
  * statistics FP32, the weights rounded to BF16 before they meet the values.
  * workspace: FP32 [65536, dim + 2], 16-byte aligned, any content, one a stream.
- * q heads a multiple of the cache's heads; scale finite; max_q >= 1; window >= 0. */
+ * q heads a multiple of the cache's heads; scale finite; max_q >= 1; window >= 0;
+ * table_width * page_size under 2^30. */
 int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
                       const int32_t* page_table, int64_t table_width,
                       const int32_t* context_lens, const int32_t* q_starts, int64_t seqs,

@@ -306,3 +306,22 @@ def test_rope_table():
         attention.rope_table(7, 24)
     with pytest.raises(ValueError):
         attention.new_cache(1, 1, 16, 96, device="cpu")
+
+
+def test_extent_refusals(lib):
+    """What the kernels hold in 32 bits: places of pages, and sums of the tiles of 64 sequences."""
+    *_, large = codes()
+    ref = ctypes.byref
+
+    def call(c, width):
+        return lib.ci8_attention_fp4(ref(heads(n=8)), ref(c), FAKE << 10, width, FAKE << 11, None, 0, 0, 128,
+                                     FAKE << 12, FAKE + (1 << 26), None, 0.1, 1, 0, None)
+
+    size = cache().page_size
+    refused(lib, call(cache(), (1 << 30) // size), large, "Page table too large")
+    assert call(cache(), (1 << 30) // size - 1) == 0
+    far = dict(k_codes=1 << 40, k_scales=1 << 41, v_codes=1 << 42, v_scales=1 << 43)
+    for name in far:
+        stride = {name[:-1] + "_page_stride": 1 << 33}
+        refused(lib, call(cache(pages=5, **far, **stride), 4), large, "Cache too large")
+        assert call(cache(pages=4, **far, **stride), 4) == 0
