@@ -9,8 +9,11 @@
 //
 // About two operations a byte: bound by HBM, and by latency for a few tokens. A lane holds 8
 // channels (16 bytes) of a head, so a head is 8, 16 or 32 lanes and a wave covers 8, 4 or 2
-// heads at once; sums and maxima are exchanges inside those lanes and nothing needs LDS
-// memory. A wave keeps one token's angles for all its heads.
+// heads at once; sums, maxima and the rotation's partners are DPP exchanges inside those lanes
+// (through LDS they took as long as the memory) and nothing needs LDS memory. A wave keeps one
+// token's angles for all its heads. Measured, with bytes read and written: 4096 tokens of 24 + 4
+// heads of 256 at 4.3 TB/s, 9261 of 16 + 16 of 64 with three axes at 3.6 TB/s, where a large copy
+// reaches 5.0; one token of 32 + 8 heads of 128 3 us in the kernel.
 #include "attention_launch.h"
 #include "fp4_device.h"
 
@@ -32,13 +35,41 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
                pack_bf16x2(x[6], x[7])};
 }
 
+// A value from another lane by a DPP control: 0xB1 and 0x4E are lane ^ 1 and lane ^ 2, 0x141 and
+// 0x140 reverse 8 and 16 lanes, which is lane ^ 4 and lane ^ 8 of values that 4 and 8 share.
+template <int kControl>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), kControl, 0xF, 0xF, true));
+}
+template <int kControl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kControl, 0xF, 0xF, true));
+}
+
+// Sums of neighbours, of pairs of those and so on, over kLanes lanes (8, 16 or 32).
+template <int kLanes>
+__device__ __forceinline__ float tree_sum(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  if constexpr (kLanes > 8) v += dpp<0x140>(v);
+  if constexpr (kLanes > 16) {
+    // Both rows of 16 lanes of each 32, in either operand.
+    const auto rows =
+        __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = __int_as_float(rows[0]) + __int_as_float(rows[1]);
+  }
+  return v;
+}
+
 // Largest |x| of a block of 32 channels (4 lanes), as FP32 bits: a NaN is larger than all.
 __device__ __forceinline__ uint32_t block_amax(const float (&x)[8]) {
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-  m = max(m, uint32_t(__shfl_xor(int(m), 1, 64)));
-  return max(m, uint32_t(__shfl_xor(int(m), 2, 64)));
+  m = max(m, dpp<0xB1>(m));
+  return max(m, dpp<0x4E>(m));
 }
 
 // Cosine and signed sine of this lane's 8 channels: y = x cos + partner sin.
@@ -47,14 +78,13 @@ struct Angles {
 };
 
 template <int D>
-__device__ __forceinline__ Angles load_angles(const RotationView& r, int64_t tokens, int token,
-                                              int channel) {
+__device__ __forceinline__ Angles load_angles(const RotationView& r, int64_t at, int64_t tokens,
+                                              int token, int channel) {
   Angles a;
   const int half = r.rot / 2;
   const bool second = !r.interleaved && channel >= half;
   const int first = r.interleaved ? channel / 2 : second ? channel - half : channel;
   if (r.axes == 1) {
-    const int64_t at = r.positions[token];
     const bool inside = at >= 0 && at < r.rows;
     const float* row = r.table + (inside ? at : 0) * r.rot + first;
     if (r.interleaved) {
@@ -83,16 +113,29 @@ __device__ __forceinline__ Angles load_angles(const RotationView& r, int64_t tok
     }
     return a;
   }
+  // Rows of the table for up to four axes, the same in all lanes; -1 outside it.
+  constexpr int kAxes = 4;
+  int64_t rows[kAxes];
+#pragma unroll
+  for (int i = 0; i < kAxes; ++i) {
+    rows[i] = i < r.axes ? r.positions[i * tokens + token] : -1;
+    if (rows[i] >= r.rows) rows[i] = -1;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int pair = first + (r.interleaved ? j / 2 : j);
     const int axis = r.axis_of[pair];
-    const bool known = axis >= 0 && axis < r.axes;
-    const int64_t at = r.positions[(known ? axis : 0) * tokens + token];
-    const bool inside = known && at >= 0 && at < r.rows;
-    const float* row = r.table + (inside ? at : 0) * r.rot + pair;
-    const float s = row[half];
-    a.cos[j] = inside ? row[0] : __builtin_nanf("");
+    int64_t row = -1;
+    if (r.axes <= kAxes) {
+#pragma unroll
+      for (int i = 0; i < kAxes; ++i) row = axis == i ? rows[i] : row;
+    } else if (axis >= 0 && axis < r.axes) {
+      row = r.positions[axis * tokens + token];
+      if (row >= r.rows) row = -1;
+    }
+    const float* values = r.table + (row < 0 ? 0 : row) * r.rot + pair;
+    const float s = values[half];
+    a.cos[j] = row < 0 ? __builtin_nanf("") : values[0];
     a.sin[j] = (r.interleaved ? j % 2 : int(second)) ? s : -s;
   }
   return a;
@@ -104,15 +147,47 @@ __device__ __forceinline__ void norm8(float (&x)[8], const float* weight, float 
   float s[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) s[j] = x[2 * j] * x[2 * j] + x[2 * j + 1] * x[2 * j + 1];
-  float sum = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-  for (int step = 1; step < D / 8; step *= 2) sum += __shfl_xor(sum, step, 64);
+  const float sum = tree_sum<D / 8>((s[0] + s[1]) + (s[2] + s[3]));
   const float inv = 1.f / __builtin_sqrtf(sum * (1.f / D) + eps);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const f32x4 w = *reinterpret_cast<const f32x4*>(weight + 4 * h);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[4 * h + j] = x[4 * h + j] * inv * w[j];
+  }
+}
+
+// The values of lane ^ step, for a step that is a power of two: without LDS. Others by lane number.
+__device__ __forceinline__ void exchange8(const float (&x)[8], float (&other)[8], int step, int lane,
+                                          int from) {
+  switch (step) {
+    case 1:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = dpp<0xB1>(x[j]);
+      break;
+    case 2:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = dpp<0x4E>(x[j]);
+      break;
+    case 4:  // 8 lanes reversed (lane ^ 7), then 4 (lane ^ 3)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = dpp<0x1B>(dpp<0x141>(x[j]));
+      break;
+    case 8:  // a row of 16 turned by 8
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = dpp<0x128>(x[j]);
+      break;
+    case 16:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_int(x[j]),
+                                                           __float_as_int(x[j]), false, false);
+        other[j] = __int_as_float(lane & 16 ? rows[0] : rows[1]);
+      }
+      break;
+    default:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = __shfl(x[j], from, 64);
   }
 }
 
@@ -124,11 +199,10 @@ __device__ __forceinline__ void rotate8(float (&x)[8], const Angles& a, const Ro
 #pragma unroll
     for (int j = 0; j < 8; ++j) other[j] = x[j ^ 1];
   } else {
-    // The pair's other half: rot / 16 lanes on or back. Lanes past rot keep what they hold.
+    // The pair's other half: rot / 16 lanes on or back. Lanes past rot get anything.
     const int step = r.rot / 16;
     const int from = channel < r.rot / 2 ? lane + step : channel < r.rot ? lane - step : lane;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) other[j] = __shfl(x[j], from, 64);
+    exchange8(x, other, step, lane, from);
   }
   if (channel < r.rot) {
 #pragma unroll
@@ -157,9 +231,13 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs p, in
                                                         int k_groups, int groups, int chunks) {
   constexpr int kLanes = D / 8, kHeads = 64 / kLanes;
   const int lane = threadIdx.x & 63, channel = lane % kLanes * 8;
-  const int wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int token = wave / chunks, first = wave % chunks * kGroups;
   if (token >= p.tokens) return;
+  // The token's position and slot come first: its angles' and rows' places wait for them.
+  const int64_t position = p.rotation.rot ? p.rotation.positions[token] : 0;
+  int64_t slot = -1;
+  if constexpr (kAppend) slot = p.slots[token];
 
   u32x4 raw[kGroups];
   int head[kGroups];
@@ -179,11 +257,10 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs p, in
   }
   Angles angles = {};
   if (p.rotation.rot && channel < p.rotation.rot)
-    angles = load_angles<D>(p.rotation, p.tokens, token, channel);
+    angles = load_angles<D>(p.rotation, position, p.tokens, token, channel);
   int64_t page = -1;
   int row = 0;
   if constexpr (kAppend) {
-    const int64_t slot = p.slots[token];
     if (slot >= 0 && slot < int64_t(p.cache.pages) << p.cache.page_shift) {
       page = slot >> p.cache.page_shift;
       row = int(slot & ((1 << p.cache.page_shift) - 1));
@@ -226,10 +303,19 @@ hipError_t launch_dim(const NormRopeArgs& args, bool append, hipStream_t stream)
     kernel<<<uint32_t((waves + 3) / 4), 256, 0, stream>>>(args, q_groups, k_groups, groups,
                                                           chunks);
   };
-  if (append)
+  // Four groups a wave, which share its angles, once waves are many. Microseconds with four and
+  // with one: 4096 tokens of 24 + 4 heads of 256 28.2 and 31.8, 9261 of 16 + 16 of 64 with three
+  // axes 23.4 and 51.2; but 1024 of 32 + 8 of 128 8.6 and 8.3, 64 of them 5.3 and 3.0.
+  if (int64_t(args.tokens) * groups >= 32768) {
+    if (append)
+      launch(norm_rope_kernel<D, true, 4>, 4);
+    else
+      launch(norm_rope_kernel<D, false, 4>, 4);
+  } else if (append) {
     launch(norm_rope_kernel<D, true, 1>, 1);
-  else
+  } else {
     launch(norm_rope_kernel<D, false, 1>, 1);
+  }
   return hipGetLastError();
 }
 
