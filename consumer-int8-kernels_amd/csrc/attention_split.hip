@@ -138,10 +138,13 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
 }
 
 // Parts in the workspace: of workgroup w, part 2w continues a context, part 2w + 1 begins one.
-// Sums of rows [part][row][D] first, then their [reference, sum], then what each workgroup that
-// begins a context says of it.
+// Sums of rows [part][row][D] first, then their [reference, sum], then what the workgroup that
+// begins a context says of it: one for each context (0 parts: its output is written), or, where
+// contexts are more than workgroups, for each workgroup, which begins one at most that another
+// continues.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct Joint {
-  int parts, q_begin, rows, head;
+  int parts, first, q_begin, rows, head, unused[3];
 };
 template <int D, int kTiles>
 __device__ __forceinline__ float* part_sums(const AttentionArgs& p, int part) {
@@ -154,7 +157,7 @@ __device__ __forceinline__ float* part_stats(const AttentionArgs& p, int part) {
 template <int D>
 __device__ __forceinline__ Joint* joints(const AttentionArgs& p) {
   // the last 64 KiB of the [rows, 2] region
-  return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 4096;
+  return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 2048;
 }
 
 // The kernel's first argument, read anew: what one part of a long kernel needs of it is not held
@@ -174,7 +177,7 @@ constexpr int groups_per_cu(int dim, int tiles) {
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
 template <int D, int kTiles, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) : kWaves / 4)
-    attention_split_kernel(const AttentionArgs, int min_quota) {
+    attention_split_kernel(const AttentionArgs, int min_quota, bool by_context) {
   using L = Layout<D>;
   constexpr int kRows = 16 * kTiles;
   constexpr int kTileBytes = kTokens * L::kPitch;
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     run.quota = uniform(max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota)));
     run.begin = blockIdx.x * run.quota;
     run.end = min(run.begin + run.quota, total);
-    if (threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
+    if (!by_context && threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
     if (run.begin >= total) return;
     place = find_tile(p, kRows, lane, run.begin, counted);
   } else {
@@ -510,10 +513,11 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       }
       __syncthreads();
     }
-    if (kSplit && !whole && place.tile == 0 && threadIdx.x == 0) {
+    if (kSplit && place.tile == 0 && (by_context || !whole) && threadIdx.x == 0) {
       const int64_t last = at + place.tiles - 1;
-      joints<D>(p)[blockIdx.x] = {int(last / run.quota) - int(blockIdx.x) + 1, s.q_begin, s.rows,
-                                  kv_head};
+      joints<D>(p)[by_context ? seq * p.cache.heads + kv_head : int(blockIdx.x)] = {
+          whole ? 0 : int(last / run.quota) - int(blockIdx.x) + 1, int(blockIdx.x), s.q_begin,
+          s.rows, kv_head};
     }
     // On to the next key head or sequence.
     at += take;
@@ -534,59 +538,80 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   }
 }
 
-// Joins the parts of the context that workgroup blockIdx.x of the split kernel began: 32 channels
-// a workgroup, 8 lanes a row; groups of rows * 8 lanes take every so many parts. Bound by the
-// latency of its dependent reads: the sums of the first parts are on their way while the
-// statistics are read, by a row's own lanes where parts are few and by whole waves where many.
-constexpr int kJoinThreads = 256, kJoinChannels = 32;
-template <int D, int kTiles>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttentionArgs p) {
+// Joins the parts of a context (by_context: the blockIdx.x-th, else what workgroup blockIdx.x of the
+// split kernel began): 32 channels a workgroup, 8 lanes a row; groups of rows * 8 lanes take every so
+// many parts. Bound by the latency of its dependent reads, 1 to 2 us each: the sums of the first
+// parts are on their way while the statistics are read, by a row's own lanes where parts are few and
+// by whole waves where many.
+constexpr int kJoinChannels = 32;
+template <int D, int kTiles, int kThreads>
+__global__ void __launch_bounds__(kThreads)
+    attention_join_kernel(const AttentionArgs p, int workgroups, bool by_context) {
   constexpr int kRows = 16 * kTiles, kLanes = kJoinChannels / 4, kEarly = 4, kFew = 8;
-  static_assert(kRows * kLanes <= kJoinThreads);
+  static_assert(kRows * kLanes <= kThreads);
   Joint joint = joints<D>(p)[blockIdx.x];
+  // Contexts that the split kernel does not have say nothing.
+  if (by_context && split_tiles(sequence(p, blockIdx.x / p.cache.heads), kRows) == 0) return;
   if (joint.parts <= 0) return;
   // Whatever stands there (a workspace that another stream writes), accesses stay in bounds.
-  joint.parts = min(joint.parts, int(gridDim.x - blockIdx.x));
+  joint.first = min(max(joint.first, 0), workgroups - 1);
+  joint.parts = min(joint.parts, workgroups - joint.first);
   joint.rows = min(max(joint.rows, 1), min(kRows, p.tokens * p.group));
   joint.q_begin = min(max(joint.q_begin, 0), p.tokens - (joint.rows + p.group - 1) / p.group);
   joint.head = min(max(joint.head, 0), p.cache.heads - 1);
-  __shared__ f32x4 sums[kJoinThreads];
+  __shared__ f32x4 sums[kThreads];
   __shared__ float tops[kRows], totals[kRows];
-  auto part = [&](int i) { return i == 0 ? 2 * int(blockIdx.x) + 1 : 2 * (int(blockIdx.x) + i); };
-  const int width = joint.rows * kLanes, groups = kJoinThreads / width;
+  auto part = [&](int i) { return 2 * (joint.first + i) + (i == 0); };
+  const int width = joint.rows * kLanes, groups = kThreads / width;
   const int group = threadIdx.x / width, row = threadIdx.x % width / kLanes;
   const int channel = blockIdx.y * kJoinChannels + threadIdx.x % kLanes * 4;
   auto sum_at = [&](int i) {
-    return reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel);
+    return *reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel);
   };
-  auto stats_at = [&](int i, int r) { return part_stats<D, kTiles>(p, part(i)) + 2 * r; };
+  auto stats_at = [&](int i, int r) {
+    return *reinterpret_cast<const f32x2*>(part_stats<D, kTiles>(p, part(i)) + 2 * r);
+  };
   f32x4 early[kEarly];
+  f32x2 early_stats[kEarly];
 #pragma unroll
   for (int e = 0; e < kEarly; ++e) {
     early[e] = f32x4{0, 0, 0, 0};
+    early_stats[e] = f32x2{kLowest, 0};
     const int i = group + e * groups;
-    if (group < groups && i < joint.parts) early[e] = *sum_at(i);
+    if (group < groups && i < joint.parts) {
+      early[e] = sum_at(i);
+      early_stats[e] = stats_at(i, row);
+    }
   }
   float top = kLowest, total = 0;
   if (joint.parts <= kFew) {
-#pragma unroll 4
-    for (int i = 0; i < joint.parts; ++i) top = fmaxf(top, stats_at(i, row)[0]);
-#pragma unroll 4
-    for (int i = 0; i < joint.parts; ++i)
-      total += stats_at(i, row)[1] * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
+    f32x2 stats[kFew];
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) stats[i] = stats_at(min(i, joint.parts - 1), row);
+#pragma unroll
+    for (int i = 0; i < kFew; ++i) top = fmaxf(top, stats[i][0]);
+#pragma unroll
+    for (int i = 0; i < kFew; ++i)
+      total += i < joint.parts ? stats[i][1] * __builtin_amdgcn_exp2f(stats[i][0] - top) : 0.f;
   } else {
     const int lane = threadIdx.x & 63;
-    for (int r = threadIdx.x >> 6; r < joint.rows; r += kJoinThreads / 64) {
+    for (int r = threadIdx.x >> 6; r < joint.rows; r += kThreads / 64) {
       float m = kLowest, l = 0;
-      for (int i = lane; i < joint.parts; i += 64) m = fmaxf(m, stats_at(i, r)[0]);
+      for (int i = lane; i < joint.parts; i += 64) {
+        const f32x2 stats = stats_at(i, r);
+        const float most = fmaxf(m, stats[0]);
+        l = l * __builtin_amdgcn_exp2f(m - most) +
+            stats[1] * __builtin_amdgcn_exp2f(stats[0] - most);
+        m = most;
+      }
+      float most = m;
 #pragma unroll
-      for (int step = 32; step >= 1; step /= 2) m = fmaxf(m, __shfl_xor(m, step, 64));
-      for (int i = lane; i < joint.parts; i += 64)
-        l += stats_at(i, r)[1] * __builtin_amdgcn_exp2f(stats_at(i, r)[0] - m);
+      for (int step = 32; step >= 1; step /= 2) most = fmaxf(most, __shfl_xor(most, step, 64));
+      l *= __builtin_amdgcn_exp2f(m - most);
 #pragma unroll
       for (int step = 32; step >= 1; step /= 2) l += __shfl_xor(l, step, 64);
       if (lane == 0) {
-        tops[r] = m;
+        tops[r] = most;
         totals[r] = l;
       }
     }
@@ -597,18 +622,16 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Atte
   f32x4 x = {0, 0, 0, 0};
   if (group < groups) {
 #pragma unroll
-    for (int e = 0; e < kEarly; ++e) {
-      const int i = group + e * groups;
-      if (i < joint.parts) x += early[e] * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
-    }
+    for (int e = 0; e < kEarly; ++e)
+      x += early[e] * __builtin_amdgcn_exp2f(early_stats[e][0] - top);
 #pragma unroll 4
     for (int i = group + kEarly * groups; i < joint.parts; i += groups)
-      x += *sum_at(i) * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
+      x += sum_at(i) * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
   }
   sums[threadIdx.x] = x;
   __syncthreads();
   if (group == 0) {
-    for (int g = 1; g < groups; ++g) x += sums[g * width + threadIdx.x];
+    for (int g = 1; g < min(groups, joint.parts); ++g) x += sums[g * width + threadIdx.x];
     write_row4(p, D, joint.q_begin, row, joint.head, channel, x, top, total);
   }
 }
@@ -625,24 +648,30 @@ hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
     // Eight waves where their registers allow: 517 tokens of 8 key heads of 128 7.6 us, four 8.3.
     constexpr int kWaves = D == 256 && kTiles == 2 ? 4 : 8;
     attention_split_kernel<D, kTiles, kWaves, false>
-        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, 0);
+        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, 0, false);
     return hipGetLastError();
   }
   // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
   // 59; 64 up to 32768 264 and 278. At D = 256 contexts that are few get fewer workgroups and so
-  // fewer parts to join: one of 131071 tokens of 4 heads 40 us, with two a CU 48; 32 up to 9000 53
+  // fewer parts to join: one of 131071 tokens of 4 heads 37 us, with two a CU 39; 32 up to 9000 53
   // and 50.
   constexpr int kWaves = 4;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
-  static_assert(2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
-                    kAttentionWorkspaceRows * 2 - 4096 * 4,
+  static_assert(groups_per_cu(D, kTiles) <= 8 &&
+                    2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
+                        kAttentionWorkspaceRows * 2 - 2048 * 8,
                 "parts, statistics and descriptions fit the workspace");
+  const bool by_context = contexts <= groups;
   attention_split_kernel<D, kTiles, kWaves, true>
-      <<<groups, 64 * kWaves, 0, stream>>>(args, 2 * kWaves);
+      <<<groups, 64 * kWaves, 0, stream>>>(args, 2 * kWaves, by_context);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  attention_join_kernel<D, kTiles>
-      <<<dim3(groups, D / kJoinChannels), kJoinThreads, 0, stream>>>(args);
+  // More threads where a context has many parts: one of 131071 tokens of 4 heads, 64 parts each,
+  // is joined in 5.0 us, by 256 threads in 7.2; 32 contexts up to 8000, 4 parts, in 8.8 and 4.9.
+  const bool many = groups > 16 * contexts;
+  const auto join = many ? attention_join_kernel<D, kTiles, 1024> : attention_join_kernel<D, kTiles, 256>;
+  join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : 256, 0,
+         stream>>>(args, groups, by_context);
   return hipGetLastError();
 }
 
