@@ -176,7 +176,7 @@ constexpr int groups_per_cu(int dim, int tiles) {
 
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
 template <int D, int kTiles, int kWaves, bool kSplit>
-__global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) : kWaves / 4)
+__global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) * kWaves / 4 : kWaves / 4)
     attention_split_kernel(const AttentionArgs, int min_quota, bool by_context) {
   using L = Layout<D>;
   constexpr int kRows = 16 * kTiles;
@@ -336,25 +336,28 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       // Scores, lane: row `column`, tokens 4 * group4 + i of each half.
       f32x4 score[kTiles][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) score[n][h] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < L::kChunks; ++u)
+      for (int u = 0; u < L::kChunks; ++u) {
 #pragma unroll
-          for (int j = 0; j < L::kSteps; ++j) {
+        for (int j = 0; j < L::kSteps; ++j) {
+          bf16x8 query[kTiles];
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+            query[n] = __builtin_bit_cast(
+                bf16x8, kQueriesInLds ? queries[((n * L::kChunks + u) * L::kSteps + j) * 64 + lane]
+                                      : q[n][u][j]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
             const bf16x8 a = __builtin_bit_cast(
                 bf16x8, fp4_to_bf16x8(k[h].codes[u][j], fp4_scale_in(k[h].scales[u], scale_turn)));
 #pragma unroll
             for (int n = 0; n < kTiles; ++n)
-              score[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  a,
-                  __builtin_bit_cast(
-                      bf16x8, kQueriesInLds
-                                  ? queries[((n * L::kChunks + u) * L::kSteps + j) * 64 + lane]
-                                  : q[n][u][j]),
-                  score[n][h], 0, 0, 0);
+              score[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, query[n], score[n][h], 0, 0, 0);
           }
+        }
       }
       load(k, k_codes, at_page.k_codes, k_scales, at_page.k_scales, t_next, i);
 
@@ -645,17 +648,19 @@ hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
   const int64_t span = args.window ? (args.window + args.max_q) / kTokens + 2 : longest;
   const int64_t contexts = int64_t(args.seqs) * args.cache.heads;
   if ((longest < span ? longest : span) <= kWholeTiles) {
-    // Eight waves where their registers allow: 517 tokens of 8 key heads of 128 7.6 us, four 8.3.
-    constexpr int kWaves = D == 256 && kTiles == 2 ? 4 : 8;
+    // Eight waves: 517 tokens of 8 key heads of 128 7.6 us, with four 8.3; 4 rows a sequence of 6
+    // heads of 256, 64 contexts up to 1500, 25.5 and 32.4.
+    constexpr int kWaves = 8;
     attention_split_kernel<D, kTiles, kWaves, false>
         <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, 0, false);
     return hipGetLastError();
   }
   // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
-  // 59; 64 up to 32768 264 and 278. At D = 256 contexts that are few get fewer workgroups and so
-  // fewer parts to join: one of 131071 tokens of 4 heads 37 us, with two a CU 39; 32 up to 9000 53
-  // and 50.
-  constexpr int kWaves = 4;
+  // 59; 64 up to 32768 257 and 278. Where the queries are in LDS eight share them: 16 x 4 rows up to
+  // 16000 of 4 heads of 256 58 us, with four 67. At D = 256 contexts that are few get fewer
+  // workgroups and so fewer parts to join: one of 131071 tokens of 4 heads 37 us, with two a CU 39;
+  // 32 up to 9000 53 and 50.
+  constexpr int kWaves = D == 256 && kTiles == 2 ? 8 : 4;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(groups_per_cu(D, kTiles) <= 8 &&

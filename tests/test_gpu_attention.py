@@ -472,6 +472,21 @@ def test_long_context_and_many_sequences(attention):
     check_attention(q, cache, table, lens, None, 0.09, 1, 0, out, lse)
 
 
+@pytest.mark.parametrize("dim,hq,hk,seqs,count", [(256, 16, 4, 80, 5), (64, 8, 4, 300, 1), (128, 30, 2, 130, 3)])
+def test_more_contexts_than_workgroups(attention, dim, hq, hk, seqs, count):
+    rng = np.random.default_rng(seqs)
+    page = 32
+    lens = [int(x) for x in rng.integers(0, 130, seqs)]
+    lens[seqs // 2], lens[-1] = 3001, 2500
+    pages = sum(-(-n // page) for n in lens) + 1
+    cache = random_cache(attention, rng, pages, hk, page, dim)
+    table = tables(rng, lens, pages, page)
+    q = bf16_randn(rng, seqs * count, hq, dim).cuda()
+    starts = [i * count for i in range(seqs + 1)]
+    out, lse = run_attention(attention, q, cache, table, lens, starts, 0.09, count, 0)
+    check_attention(q, cache, table, lens, starts, 0.09, count, 0, out, lse)
+
+
 def test_long_chunk_behind_a_long_context(attention):
     rng = np.random.default_rng(13)
     page, dim, hk = 64, 128, 1
