@@ -67,8 +67,8 @@ struct AttentionArgs {
   uint32_t q_sign;
   int table_width, seqs, tokens, group, max_q, window;
 };
-// Sequences of at most `rows` (16 or 32) rows, and those of more than `few`.
-hipError_t launch_attention_split(const AttentionArgs& args, int dim, int rows,
+// Sequences of at most `most` rows, and those of more than `few`.
+hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream);
 hipError_t launch_attention_prompt(const AttentionArgs& args, int dim, int few,
                                    hipStream_t stream);

@@ -4,7 +4,7 @@
 //   o = sum_t p_t v_t / sum_t p_t,   p_t = exp2(s_t - m),   s_t = q.k_t * scale * log2(e)
 //
 // in one pass with a running reference m. Rows are (token, query head of one key head) pairs,
-// 16 or 32, so that the cache is read once for all heads that share it: bound by HBM, whose
+// 16 or 32 at a time, so that the cache is read once for all heads that share it: bound by HBM, whose
 // stream the conversions (half an instruction a value) and MFMAs have to stay under. A wave
 // works alone on 32 tokens at a time, the next 32 on their way:
 //
@@ -21,13 +21,14 @@
 // 2^8 in weight, so most tiles exchange nothing between lanes and rescale nothing.
 //
 // Contexts differ and only the device knows them, so the work is cut there: all tiles of all
-// sequences and key heads are laid end to end and each workgroup takes an equal run of them.
+// sequences, key heads and blocks of rows are laid end to end and each workgroup takes an equal run
+// of them.
 // A run that covers a whole context writes its output; parts of one go to the workspace, two
 // at most a workgroup, and a second kernel joins them in a fixed order.
 //
-// Measured, of the cache's bytes: 64 contexts up to 32768 tokens, 64 query heads on 8 of 128, 265
-// us, 5.4 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 44 us, 3.3 TB/s with
-// the join (6 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
+// Measured, of the cache's bytes: 64 contexts up to 32768 tokens, 64 query heads on 8 of 128, 257
+// us, 5.5 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 43 us, 3.4 TB/s with
+// the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
 // the launch.
 #include "attention_device.h"
 #include "launch.h"
@@ -78,44 +79,51 @@ __device__ __forceinline__ void load_rows(Raw<D>& r, const uint8_t* codes, const
   }
 }
 
-// Tiles of a sequence that the split kernel has, at least one (it writes the rows that attend
-// to nothing): 0 without rows, or with more than `most`, which are the prompt kernel's.
-__device__ __forceinline__ int split_tiles(const Sequence& s, int most) {
-  return s.rows == 0 || s.rows > most ? 0 : max(s.tiles(kTokens), 1);
+// What the split kernel has of a sequence: blocks of rows, none if those are more than `most`, which
+// are the prompt kernel's, and the tiles of each, at least one (it writes the rows that attend to
+// nothing). Each block of a key head has its own context.
+__device__ __forceinline__ int row_blocks(const Sequence& s, int most, int block_rows) {
+  return s.rows > most ? 0 : (s.rows + block_rows - 1) / block_rows;
 }
+__device__ __forceinline__ int block_tiles(const Sequence& s) { return max(s.tiles(kTokens), 1); }
 
 // A run of tiles: [begin, end) of the row of all sequences' tiles, one after the other for each
-// key head.
+// key head and block of rows.
 struct Run {
   int64_t begin, end, quota;
 };
 struct Place {
-  int seq, head, tile, tiles;  // tile: from the sequence's first
+  int seq, head, block, blocks, tile, tiles;  // tile: from the sequence's first
 };
 
-// Tiles of 64 sequences from `base` on, one a lane, and their sums up to each lane's.
+// Of 64 sequences from `base` on, one a lane: blocks of a key head, tiles of a block, and sums of
+// both's products up to each lane's.
 struct Counted {
-  int base, tiles, sum;
+  int base, blocks, tiles, sum;
 };
-__device__ __forceinline__ Counted count_tiles(const AttentionArgs& p, int most, int lane,
-                                               int base) {
-  Counted c = {base, 0, 0};
-  if (base + lane < p.seqs) c.tiles = split_tiles(sequence(p, base + lane), most);
-  c.sum = wave_scan(c.tiles, lane);
+__device__ __forceinline__ Counted count_tiles(const AttentionArgs& p, int most, int block_rows,
+                                               int lane, int base) {
+  Counted c = {base, 0, 1, 0};
+  if (base + lane < p.seqs) {
+    const Sequence s = sequence(p, base + lane);
+    c.blocks = row_blocks(s, most, block_rows);
+    c.tiles = block_tiles(s);
+  }
+  c.sum = wave_scan(c.blocks * c.tiles, lane);
   return c;
 }
 // Tiles of all; `first` are those of the first 64 sequences.
-__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int lane,
-                                             const Counted& first) {
+__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int block_rows,
+                                             int lane, const Counted& first) {
   int64_t total = uniform(__shfl(first.sum, 63, 64));
   for (int base = 64; base < p.seqs; base += 64)
-    total += uniform(__shfl(count_tiles(p, most, lane, base).sum, 63, 64));
+    total += uniform(__shfl(count_tiles(p, most, block_rows, lane, base).sum, 63, 64));
   return total * p.cache.heads;
 }
 
 // Where tile `at` of all lies; at is less than their number. `first`: of the first 64 sequences.
-__device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int lane, int64_t at,
-                                           const Counted& first) {
+__device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int block_rows,
+                                           int lane, int64_t at, const Counted& first) {
   const int heads = p.cache.heads;
   Counted c = first;
   int64_t before = 0;
@@ -125,15 +133,18 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
       const int which = hit ? __builtin_ctzll(hit) : 0;
       Place place;
       place.seq = uniform(c.base + which);
-      place.tiles = max(uniform(__shfl(c.tiles, which, 64)), 1);
-      const int in_front = uniform(__shfl(c.sum, which, 64)) - place.tiles;
+      place.tiles = uniform(__shfl(c.tiles, which, 64));
+      place.blocks = max(uniform(__shfl(c.blocks, which, 64)), 1);
+      const int in_front = uniform(__shfl(c.sum, which, 64)) - place.tiles * place.blocks;
       const int64_t inside = at - before - int64_t(in_front) * heads;
-      place.head = uniform(int(inside / place.tiles));
+      const int context = uniform(int(inside / place.tiles));
       place.tile = uniform(int(inside % place.tiles));
+      place.head = uniform(context / place.blocks);
+      place.block = uniform(context % place.blocks);
       return place;
     }
     before += int64_t(uniform(__shfl(c.sum, 63, 64))) * heads;
-    c = count_tiles(p, most, lane, c.base + 64);
+    c = count_tiles(p, most, block_rows, lane, c.base + 64);
   }
 }
 
@@ -144,7 +155,7 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
 // continues.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct Joint {
-  int parts, first, q_begin, rows, head, unused[3];
+  int parts, first, q_begin, row0, rows, head, unused[2];
 };
 template <int D, int kTiles>
 __device__ __forceinline__ float* part_sums(const AttentionArgs& p, int part) {
@@ -177,7 +188,8 @@ constexpr int groups_per_cu(int dim, int tiles) {
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
 template <int D, int kTiles, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) * kWaves / 4 : kWaves / 4)
-    attention_split_kernel(const AttentionArgs, int min_quota, bool by_context) {
+    attention_split_kernel(const AttentionArgs, int most, int most_blocks, int min_quota,
+                           bool by_context) {
   using L = Layout<D>;
   constexpr int kRows = 16 * kTiles;
   constexpr int kTileBytes = kTokens * L::kPitch;
@@ -199,21 +211,24 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   Place place;
   if constexpr (kSplit) {
     const AttentionArgs& p = arguments();
-    const Counted counted = count_tiles(p, kRows, lane, 0);
-    const int64_t total = all_tiles(p, kRows, lane, counted);
+    const Counted counted = count_tiles(p, most, kRows, lane, 0);
+    const int64_t total = all_tiles(p, most, kRows, lane, counted);
     run.quota = uniform(max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota)));
     run.begin = blockIdx.x * run.quota;
     run.end = min(run.begin + run.quota, total);
     if (!by_context && threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
     if (run.begin >= total) return;
-    place = find_tile(p, kRows, lane, run.begin, counted);
+    place = find_tile(p, most, kRows, lane, run.begin, counted);
   } else {
     const AttentionArgs& p = arguments();
-    place.seq = blockIdx.x / p.cache.heads;
-    place.head = blockIdx.x % p.cache.heads;
+    place.block = blockIdx.x % most_blocks;
+    place.head = blockIdx.x / most_blocks % p.cache.heads;
+    place.seq = blockIdx.x / most_blocks / p.cache.heads;
+    const Sequence s = sequence(p, place.seq);
+    place.blocks = uniform(row_blocks(s, most, kRows));
+    if (place.block >= place.blocks) return;
     place.tile = 0;
-    place.tiles = uniform(split_tiles(sequence(p, place.seq), kRows));
-    if (place.tiles == 0) return;
+    place.tiles = uniform(block_tiles(s));
     run = {0, place.tiles, place.tiles};
   }
   // Where this lane's rows of 16 tokens start, and its place in the LDS tile.
@@ -229,6 +244,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     const AttentionArgs& p = arguments();
     const int page_mask = (1 << p.cache.page_shift) - 1;
     const Sequence s = sequence(p, seq);
+    const int row0 = place.block * kRows, rows = min(s.rows - row0, kRows);
     const int take = int(min(int64_t(place.tiles - place.tile), run.end - at));
     const int t_begin = s.first_tile(kTokens) + place.tile, t_end = t_begin + take;
 
@@ -238,7 +254,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     if (kQueriesInLds) __syncthreads();  // the last ones are read
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      const int row = 16 * n + column;
+      const int row = row0 + 16 * n + column;
       const bool live = row < s.rows;
       const int query = live ? row / p.group : 0;
       high[n] = live ? s.shift + query + 1 : 0;
@@ -492,7 +508,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       __syncthreads();
       for (int i = thread; i < 16 * D / 4; i += 64 * kWaves) {
         const int r = i / (D / 4), row = 16 * n + r, channel = i % (D / 4) * 4;
-        if (row >= s.rows) continue;
+        if (row >= rows) continue;
         float all = kLowest, l = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) all = fmaxf(all, tops[w][row]);
@@ -504,7 +520,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
                                                (r * kJoinPitch + channel) * 4);
         }
         if (!kSplit || whole) {
-          write_row4(p, D, s.q_begin, row, kv_head, channel, x, all, l);
+          write_row4(p, D, s.q_begin, row0 + row, kv_head, channel, x, all, l);
         } else {
           *reinterpret_cast<f32x4*>(part_sums<D, kTiles>(p, part) + row * D + channel) = x;
           if (channel == 0) {
@@ -518,23 +534,28 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     }
     if (kSplit && place.tile == 0 && (by_context || !whole) && threadIdx.x == 0) {
       const int64_t last = at + place.tiles - 1;
-      joints<D>(p)[by_context ? seq * p.cache.heads + kv_head : int(blockIdx.x)] = {
+      const int context = (seq * p.cache.heads + kv_head) * most_blocks + place.block;
+      joints<D>(p)[by_context ? context : int(blockIdx.x)] = {
           whole ? 0 : int(last / run.quota) - int(blockIdx.x) + 1, int(blockIdx.x), s.q_begin,
-          s.rows, kv_head};
+          row0, rows, kv_head};
     }
-    // On to the next key head or sequence.
+    // On to the next block, key head or sequence.
     at += take;
     if (at < run.end) {
       place.tile = 0;
-      if (place.head + 1 < p.cache.heads) {
+      if (place.block + 1 < place.blocks) {
+        ++place.block;
+      } else if (place.block = 0; place.head + 1 < p.cache.heads) {
         ++place.head;
       } else {
         // More tiles are left, so a later sequence has some.
         place.head = 0;
         do {
           ++place.seq;
-          place.tiles = uniform(split_tiles(sequence(p, place.seq), kRows));
-        } while (place.tiles == 0 && place.seq + 1 < p.seqs);
+          const Sequence next = sequence(p, place.seq);
+          place.blocks = uniform(row_blocks(next, most, kRows));
+          place.tiles = uniform(block_tiles(next));
+        } while (place.blocks == 0 && place.seq + 1 < p.seqs);
       }
     }
     }
@@ -549,18 +570,24 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
 constexpr int kJoinChannels = 32;
 template <int D, int kTiles, int kThreads>
 __global__ void __launch_bounds__(kThreads)
-    attention_join_kernel(const AttentionArgs p, int workgroups, bool by_context) {
+    attention_join_kernel(const AttentionArgs p, int most, int most_blocks, int workgroups,
+                          bool by_context) {
   constexpr int kRows = 16 * kTiles, kLanes = kJoinChannels / 4, kEarly = 4, kFew = 8;
   static_assert(kRows * kLanes <= kThreads);
   Joint joint = joints<D>(p)[blockIdx.x];
   // Contexts that the split kernel does not have say nothing.
-  if (by_context && split_tiles(sequence(p, blockIdx.x / p.cache.heads), kRows) == 0) return;
+  if (by_context) {
+    const int seq = int(blockIdx.x) / most_blocks / p.cache.heads;
+    if (int(blockIdx.x) % most_blocks >= row_blocks(sequence(p, seq), most, kRows)) return;
+  }
   if (joint.parts <= 0) return;
   // Whatever stands there (a workspace that another stream writes), accesses stay in bounds.
   joint.first = min(max(joint.first, 0), workgroups - 1);
   joint.parts = min(joint.parts, workgroups - joint.first);
   joint.rows = min(max(joint.rows, 1), min(kRows, p.tokens * p.group));
-  joint.q_begin = min(max(joint.q_begin, 0), p.tokens - (joint.rows + p.group - 1) / p.group);
+  joint.row0 = min(max(joint.row0, 0), min(most, p.tokens * p.group - joint.rows));
+  joint.q_begin = min(max(joint.q_begin, 0),
+                      p.tokens - (joint.row0 + joint.rows + p.group - 1) / p.group);
   joint.head = min(max(joint.head, 0), p.cache.heads - 1);
   __shared__ f32x4 sums[kThreads];
   __shared__ float tops[kRows], totals[kRows];
@@ -635,7 +662,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   if (group == 0) {
     for (int g = 1; g < min(groups, joint.parts); ++g) x += sums[g * width + threadIdx.x];
-    write_row4(p, D, joint.q_begin, row, joint.head, channel, x, top, total);
+    write_row4(p, D, joint.q_begin, joint.row0 + row, joint.head, channel, x, top, total);
   }
 }
 
@@ -643,16 +670,18 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kWholeTiles = 64;
 
 template <int D, int kTiles>
-hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
+hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream) {
   const int64_t longest = (int64_t(args.table_width) << args.cache.page_shift) / kTokens;
   const int64_t span = args.window ? (args.window + args.max_q) / kTokens + 2 : longest;
-  const int64_t contexts = int64_t(args.seqs) * args.cache.heads;
+  const int64_t rows = int64_t(args.max_q) * args.group;
+  const int blocks = int(((rows < most ? rows : most) + 16 * kTiles - 1) / (16 * kTiles));
+  const int64_t contexts = int64_t(args.seqs) * args.cache.heads * blocks;
   if ((longest < span ? longest : span) <= kWholeTiles) {
     // Eight waves: 517 tokens of 8 key heads of 128 7.6 us, with four 8.3; 4 rows a sequence of 6
     // heads of 256, 64 contexts up to 1500, 25.5 and 32.4.
     constexpr int kWaves = 8;
     attention_split_kernel<D, kTiles, kWaves, false>
-        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, 0, false);
+        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, most, blocks, 0, false);
     return hipGetLastError();
   }
   // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
@@ -669,41 +698,48 @@ hipError_t launch_split(const AttentionArgs& args, hipStream_t stream) {
                 "parts, statistics and descriptions fit the workspace");
   const bool by_context = contexts <= groups;
   attention_split_kernel<D, kTiles, kWaves, true>
-      <<<groups, 64 * kWaves, 0, stream>>>(args, 2 * kWaves, by_context);
+      <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   // More threads where a context has many parts: one of 131071 tokens of 4 heads, 64 parts each,
   // is joined in 5.0 us, by 256 threads in 7.2; 32 contexts up to 8000, 4 parts, in 8.8 and 4.9.
   const bool many = groups > 16 * contexts;
   const auto join = many ? attention_join_kernel<D, kTiles, 1024> : attention_join_kernel<D, kTiles, 256>;
   join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : 256, 0,
-         stream>>>(args, groups, by_context);
+         stream>>>(args, most, blocks, groups, by_context);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_attention_split(const AttentionArgs& args, int dim, int rows,
+// Up to this many rows a sequence are few: above 32 in blocks that each read the cache, which the
+// caches between them and HBM mostly hold. With the prompt kernel's 256 rows a workgroup instead,
+// us: 16 x 5 tokens behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 220, 16
+// tokens each 151 and 224, 32 tokens (256 rows) behind 30000 132 and 125; 4 x 32 tokens of 24 and 4
+// of 256 65 and 135; 16 x 100 rows of 16 heads of 64 203 and 280.
+constexpr int kMostRows = 128;
+
+hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream) {
-  if (rows <= 16) {
+  if (most <= 16) {
     switch (dim) {
-      case 64: return launch_split<64, 1>(args, stream);
-      case 128: return launch_split<128, 1>(args, stream);
-      default: return launch_split<256, 1>(args, stream);
+      case 64: return launch_split<64, 1>(args, most, stream);
+      case 128: return launch_split<128, 1>(args, most, stream);
+      default: return launch_split<256, 1>(args, most, stream);
     }
   }
   switch (dim) {
-    case 64: return launch_split<64, 2>(args, stream);
-    case 128: return launch_split<128, 2>(args, stream);
-    default: return launch_split<256, 2>(args, stream);
+    case 64: return launch_split<64, 2>(args, most, stream);
+    case 128: return launch_split<128, 2>(args, most, stream);
+    default: return launch_split<256, 2>(args, most, stream);
   }
 }
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  // Sequences of at most `few` rows go to the split kernel, the others to the prompt kernel;
-  // 16 or 32 so that the usual decode fits.
+  // Sequences of at most `few` rows go to the split kernel, the others to the prompt kernel. Beside
+  // prompts `few` is 16 or 32, so that the usual decode fits.
   const int64_t most = int64_t(args.max_q) * args.group;
-  int few = most <= 16 || (most > 32 && args.group <= 16) ? 16 : 32;
+  int few = most <= kMostRows ? int(most) : args.group <= 16 ? 16 : 32;
   // No sequence can be that short where all others at their longest leave more than that: then
   // the prompt kernel has them all.
   if (most > few && (args.tokens - int64_t(args.seqs - 1) * args.max_q) * args.group > few) few = 0;

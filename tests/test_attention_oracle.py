@@ -318,8 +318,9 @@ def test_extent_refusals(lib):
                                      FAKE << 12, FAKE + (1 << 26), None, 0.1, 1, 0, None)
 
     size = cache().page_size
-    refused(lib, call(cache(), (1 << 30) // size), large, "Page table too large")
-    assert call(cache(), (1 << 30) // size - 1) == 0
+    most = ((1 << 28) - 4096) // size
+    refused(lib, call(cache(), most + 1), large, "Page table too large")
+    assert call(cache(), most) == 0
     far = dict(k_codes=1 << 40, k_scales=1 << 41, v_codes=1 << 42, v_scales=1 << 43)
     for name in far:
         stride = {name[:-1] + "_page_stride": 1 << 33}

@@ -487,6 +487,33 @@ def test_more_contexts_than_workgroups(attention, dim, hq, hk, seqs, count):
     check_attention(q, cache, table, lens, starts, 0.09, count, 0, out, lse)
 
 
+@pytest.mark.parametrize("dim,hq,hk,lens,counts,window", [
+    (128, 16, 2, [3000, 10, 2500, 7], [5, 0, 16, 1], 0),
+    (128, 16, 2, [700, 10, 1000, 7], [5, 0, 16, 1], 0),
+    (256, 24, 4, [2600, 21], [9, 21], 0),
+    (64, 14, 2, [5000, 3, 18], [18, 3, 18], 300),
+    (64, 2, 2, [2200, 33, 60], [128, 33, 65], 0),
+    (128, 66, 2, [4200, 1], [3, 1], 0),              # blocks of rows end inside a token
+    (128, 66, 2, [400, 30], [3, 1], 50),
+    (256, 2, 1, [2100] + [66] * 69, [64] * 70, 0),   # more contexts than workgroups
+    (128, 5, 1, [3000, 2100], [26, 25], 0),          # 130 and 125 rows
+    (64, 4, 4, [20, 3000, 2], [30, 100, 40], 0),     # rows that see nothing
+])
+def test_blocks_of_rows(attention, dim, hq, hk, lens, counts, window):
+    rng = np.random.default_rng(sum(lens) + dim)
+    page = 16
+    pages = sum(-(-n // page) for n in lens) + 1
+    cache = random_cache(attention, rng, pages, hk, page, dim)
+    table = tables(rng, lens, pages, page)
+    starts = [0] + list(np.cumsum(counts))
+    q = bf16_randn(rng, starts[-1], hq, dim).cuda()
+    out, lse = run_attention(attention, q, cache, table, lens, starts, 0.09, max(counts), window)
+    check_attention(q, cache, table, lens, starts, 0.09, max(counts), window, out, lse)
+    # as many as max_q shows, whatever the blocks
+    out, lse = run_attention(attention, q, cache, table, lens, starts, 0.09, 2, window)
+    check_attention(q, cache, table, lens, starts, 0.09, 2, window, out, lse)
+
+
 def test_long_chunk_behind_a_long_context(attention):
     rng = np.random.default_rng(13)
     page, dim, hk = 64, 128, 1
