@@ -59,14 +59,30 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return int64_t(uint64_t(uint32_t(uniform(int(v)))) | uint64_t(uint32_t(uniform(int(v >> 32)))) << 32);
 }
 
-// Inclusive sums over the lanes.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    const int below = __shfl_up(v, step, 64);
-    if (lane >= step) v += below;
-  }
-  return v;
+// v of a lane whose number is the same in all.
+__device__ __forceinline__ int at_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// Inclusive scans of the wave's 64 lanes by DPP (0 beyond the first): rows of 16 by shifts of 1, 2,
+// 4 and 8, then the last lane of rows 0 and 2 into rows 1 and 3, of row 1 into rows 2 and 3.
+template <int kControl, int kRows>
+__device__ __forceinline__ int dpp_or_0(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kControl, kRows, 0xF, false);
+}
+template <typename Op>
+__device__ __forceinline__ int wave_scan(int v, Op op) {
+  v = op(v, dpp_or_0<0x111, 0xF>(v));
+  v = op(v, dpp_or_0<0x112, 0xF>(v));
+  v = op(v, dpp_or_0<0x114, 0xF>(v));
+  v = op(v, dpp_or_0<0x118, 0xF>(v));
+  v = op(v, dpp_or_0<0x142, 0xA>(v));
+  return op(v, dpp_or_0<0x143, 0xC>(v));
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  return wave_scan(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_sum(int v) { return at_lane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_max(int v) {  // of values that are not negative
+  return at_lane(wave_scan(v, [](int a, int b) { return max(a, b); }), 63);
 }
 
 __device__ __forceinline__ void write_row4(const AttentionArgs& p, int dim, int q_begin, int row,

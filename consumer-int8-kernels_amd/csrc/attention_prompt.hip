@@ -6,10 +6,9 @@
 // weighted and become the operand of O^T += V^T P^T without an exchange. Rows are (token, query
 // head of one key head) pairs, 256 a workgroup, so that heads that share a key head share its
 // tiles. Four operations a score and channel: bound by the MFMA rate, then by the softmax's
-// vector instructions (about five a score) and by LDS reads (each wave reads every tile). So a
-// wave takes 64 rows at D <= 128 (half the LDS reads of 32), one wave a SIMD with its 512
-// registers, and the scores of the next tile are on the matrix unit while the vector unit
-// weighs those of this one.
+// vector instructions (about five a score) and by LDS reads (each wave reads every tile). Two waves a
+// SIMD of 32 rows each (one at D = 256, whose sums take its registers), in alternate phases: the
+// scores of the next tile are on the matrix unit while the vector unit weighs those of this one.
 //
 // Tiles of keys and values are converted to BF16 once a workgroup, on their way into LDS: global
 // loads run two tiles ahead, one barrier a tile.
@@ -64,25 +63,23 @@ __device__ __forceinline__ int all_row_tiles(const AttentionArgs& p, int few, in
   for (int base = 0; base < p.seqs; base += 64) {
     int n = 0;
     if (base + lane < p.seqs) n = row_tiles(sequence(p, base + lane), few, rows);
-#pragma unroll
-    for (int step = 32; step >= 1; step /= 2) n += __shfl_xor(n, step, 64);
-    total += n;
+    total += wave_sum(n);
   }
-  return uniform(total);
+  return total;
 }
 __device__ __forceinline__ RowTile find_row_tile(const AttentionArgs& p, int few, int rows,
                                                  int index, int lane) {
   for (int base = 0; base < p.seqs; base += 64) {
     int n = 0;
     if (base + lane < p.seqs) n = row_tiles(sequence(p, base + lane), few, rows);
-    const int sum = wave_scan(n, lane);
+    const int sum = wave_scan(n);
     const uint64_t hit = __ballot(sum > index);
     if (hit) {
       const int which = __builtin_ctzll(hit);
-      const int tiles = uniform(__shfl(n, which, 64));
-      return {base + which, index - (uniform(__shfl(sum, which, 64)) - tiles), tiles};
+      const int tiles = at_lane(n, which);
+      return {base + which, index - (at_lane(sum, which) - tiles), tiles};
     }
-    index -= uniform(__shfl(sum, 63, 64));
+    index -= at_lane(sum, 63);
   }
   return {-1, 0, 0};
 }
@@ -159,52 +156,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     t_end = min(t_begin + each, end);
   }
 
-  // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
-  // go nowhere.
-  int row_low[kTiles], row_high[kTiles];
-  u32x4 q[kTiles][kSteps];
-  const int wave_row = row0 + wave * 32 * kTiles;
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const int row = min(wave_row + 32 * n + column, s.rows - 1), query = row / p.group;
-    row_high[n] = s.shift + query + 1;
-    row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
-    const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
-                          int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j)
-      q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
-  }
-  // Tokens [all_low, all_high) that all of the wave's rows attend to.
-  const int all_high = s.shift + min(wave_row, s.rows - 1) / p.group + 1;
-  const int any_high = s.shift + min(wave_row + 32 * kTiles - 1, s.rows - 1) / p.group + 1;
-  const int all_low = p.window ? max(any_high - p.window, 0) : 0;
-
-  f32x16 o[kTiles][kChannels];
-  float reference[kTiles], limit[kTiles], sum[kTiles];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-    for (int m = 0; m < kChannels; ++m)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][m][i] = 0;
-    reference[n] = 0;
-    limit[n] = kLowest;
-    sum[n] = 0;
-  }
-
-  // Pages outside the cache are rare: whether there are any is found once.
   const int context_page = max(s.context - 1, 0) >> p.cache.page_shift;
   const int32_t* const table = p.page_table + int64_t(where.seq) * p.table_width;
-  bool missing = false;
-  if (t_begin < t_end) {
-    const int last = min((t_end * kTokens - 1) >> p.cache.page_shift, context_page);
-    for (int i = (t_begin * kTokens >> p.cache.page_shift) + thread; i <= last; i += S::kThreads)
-      missing = missing || uint32_t(table[i]) >= uint32_t(p.cache.pages);
-  }
-  if (thread < 3) poisoned[thread] = -1;
-  const bool any_missing = __syncthreads_or(missing);
-
   // Staging. A thread converts 32 channels of one token a pack; a wave's packs are all of the keys
   // or all of the values, of one page or two. Pages are looked up a tile ahead of the codes, these
   // are loaded a tile ahead of their use. Past the last tile this goes on with tokens that are
@@ -212,9 +165,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   constexpr int kPerTile = kTokens * S::kBlocks, kWaveTokens = 64 / S::kBlocks;
   constexpr bool kTwoPages = kWaveTokens > 16;
   static_assert(kPerTile % 64 == 0 && kWaveTokens <= 32);
-  u32x4 staged_codes[S::kPacks];
-  uint32_t staged_scales[S::kPacks];
-  int pages[S::kPacks];
+  struct Staged {
+    u32x4 codes[S::kPacks];
+    uint32_t scales[S::kPacks];
+  };
+  struct Pages {
+    int at[S::kPacks];
+  };
   const int lane_token = lane / S::kBlocks, block = lane % S::kBlocks;
   const int page_mask = (1 << p.cache.page_shift) - 1;
   // Scales are loaded as the words that hold them: a loop-carried byte would be masked, and so
@@ -252,15 +209,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   int lane_zero = 0;
   asm volatile("" : "+v"(lane_zero));
   // Tiles of the keys and of the values.
-  auto load_pages = [&](int tk, int tv) __attribute__((always_inline)) {
+  auto load_pages = [&](Pages& pages, int tk, int tv) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
       const int token = (packs[c].value ? tv : tk) * kTokens + packs[c].token;
       const int at = (kTwoPages ? token + (lane_token & 16) : token + lane_zero) >> p.cache.page_shift;
-      pages[c] = table[min(at, context_page)];
+      pages.at[c] = table[min(at, context_page)];
     }
   };
-  auto load_codes = [&](int tk, int tv) __attribute__((always_inline)) {
+  auto load_codes = [&](Staged& staged, const Pages& pages, int tk, int tv)
+      __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
       const Pack& x = packs[c];
@@ -274,17 +232,74 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         scale = at * x.scale_stride + row * S::kBlocks;
       };
       int64_t code, scale;
-      offsets(uniform(pages[c]), token, code, scale);
+      offsets(uniform(pages.at[c]), token, code, scale);
       if constexpr (kTwoPages) {
         int64_t code2, scale2;
-        offsets(__builtin_amdgcn_readlane(pages[c], 16 * S::kBlocks), token + 16, code2, scale2);
+        offsets(at_lane(pages.at[c], 16 * S::kBlocks), token + 16, code2, scale2);
         code = lane_token >= 16 ? code2 : code;
         scale = lane_token >= 16 ? scale2 : scale;
       }
-      staged_codes[c] = *reinterpret_cast<const u32x4*>(x.codes + code);
-      staged_scales[c] = *reinterpret_cast<const uint32_t*>(x.scales + scale);
+      staged.codes[c] = *reinterpret_cast<const u32x4*>(x.codes + code);
+      staged.scales[c] = *reinterpret_cast<const uint32_t*>(x.scales + scale);
     }
   };
+
+  // The way in: pages, queries and codes are all on their way before the first wait for HBM but one.
+  Staged staged, ahead;
+  Pages pages, pages_ahead, pages_first;
+  if (t_begin < t_end) {
+    load_pages(pages_first, t_begin, t_begin);
+    load_pages(pages_ahead, t_begin + 1, t_begin);
+    load_pages(pages, t_begin + 2, t_begin + 1);
+  }
+  // Pages outside the cache are rare: whether there are any is found once.
+  bool missing = false;
+  if (t_begin < t_end) {
+    const int last = min((t_end * kTokens - 1) >> p.cache.page_shift, context_page);
+    for (int i = (t_begin * kTokens >> p.cache.page_shift) + thread; i <= last; i += S::kThreads)
+      missing = missing || uint32_t(table[i]) >= uint32_t(p.cache.pages);
+  }
+  // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
+  // go nowhere.
+  int row_low[kTiles], row_high[kTiles];
+  u32x4 q[kTiles][kSteps];
+  const int wave_row = row0 + wave * 32 * kTiles;
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const int row = min(wave_row + 32 * n + column, s.rows - 1), query = row / p.group;
+    row_high[n] = s.shift + query + 1;
+    row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
+    const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
+                          int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+      q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
+  }
+  if (t_begin < t_end) {
+    load_codes(staged, pages_first, t_begin, t_begin);
+    load_codes(ahead, pages_ahead, t_begin + 1, t_begin);
+  }
+  // Tokens [all_low, all_high) that all of the wave's rows attend to.
+  const int all_high = s.shift + min(wave_row, s.rows - 1) / p.group + 1;
+  const int any_high = s.shift + min(wave_row + 32 * kTiles - 1, s.rows - 1) / p.group + 1;
+  const int all_low = p.window ? max(any_high - p.window, 0) : 0;
+
+  f32x16 o[kTiles][kChannels];
+  float reference[kTiles], limit[kTiles], sum[kTiles];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+    for (int m = 0; m < kChannels; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][m][i] = 0;
+    reference[n] = 0;
+    limit[n] = kLowest;
+    sum[n] = 0;
+  }
+
+  if (thread < 3) poisoned[thread] = -1;
+  const bool any_missing = __syncthreads_or(missing);
+
   auto there = [&](int token) __attribute__((always_inline)) {
     return uint32_t(table[min(token >> p.cache.page_shift, context_page)]) < uint32_t(p.cache.pages);
   };
@@ -292,12 +307,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     return (t + 1) * kTokens > first_high || t * kTokens < last_low;
   };
   // key_buffer: where tile tk goes, t % 3 of some count.
-  auto store_tiles = [&](int key_buffer, int tv) __attribute__((always_inline)) {
+  auto store_tiles = [&](const Staged& staged, int key_buffer, int tv) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
       const Pack& x = packs[c];
-      u32x4 codes = staged_codes[c];
-      uint32_t scales = staged_scales[c];
+      u32x4 codes = staged.codes[c];
+      uint32_t scales = staged.scales[c];
       if (x.value && (edge_tile(tv) || any_missing)) {
         // Values of no page or past the context are zeros, and so are an edge tile's NaN blocks.
         const int token = tv * kTokens + x.token + lane_token;
@@ -452,15 +467,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   f32x16 scores[kTiles];
   if (t_begin < t_end) {
     // In a tile's step the keys of the next tile but one are staged, and the values of the next.
-    load_pages(t_begin, t_begin);
-    load_codes(t_begin, t_begin);
-    load_pages(t_begin + 1, t_begin);
-    store_tiles(0, t_begin);
-    load_codes(t_begin + 1, t_begin);
-    load_pages(t_begin + 2, t_begin + 1);
-    store_tiles(1, t_begin);
-    load_codes(t_begin + 2, t_begin + 1);
-    load_pages(t_begin + 3, t_begin + 2);
+    store_tiles(staged, 0, t_begin);
+    load_codes(staged, pages, t_begin + 2, t_begin + 1);
+    load_pages(pages, t_begin + 3, t_begin + 2);
+    store_tiles(ahead, 1, t_begin);
     __syncthreads();
     read_keys(0, 0);
     multiply(scores);
@@ -478,7 +488,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       if (!kAhead) read_keys(buffer[1], 0);
       settle(t * kTokens + 32 * b, scores);
       weigh(scores);
-      if (b == 0) store_tiles(buffer[2], t + 1);
+      if (b == 0) store_tiles(staged, buffer[2], t + 1);
       // This half's values, the next half's scores (past the last tile those of old keys, which
       // nothing reads), and the operands after those.
       __builtin_amdgcn_s_setprio(1);
@@ -489,8 +499,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       if (kAhead) read_values(t + (b + 1) / kHalves, (b + 1) % kHalves);
       scale(scores);
       if (b == 0) {
-        load_codes(t + 3, t + 2);
-        load_pages(t + 4, t + 3);
+        load_codes(staged, pages, t + 3, t + 2);
+        load_pages(pages, t + 4, t + 3);
       }
       // LDS reads and vector instructions go between the MFMAs.
       if (kAhead) {

@@ -109,15 +109,15 @@ __device__ __forceinline__ Counted count_tiles(const AttentionArgs& p, int most,
     c.blocks = row_blocks(s, most, block_rows);
     c.tiles = block_tiles(s);
   }
-  c.sum = wave_scan(c.blocks * c.tiles, lane);
+  c.sum = wave_scan(c.blocks * c.tiles);
   return c;
 }
 // Tiles of all; `first` are those of the first 64 sequences.
 __device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int block_rows,
                                              int lane, const Counted& first) {
-  int64_t total = uniform(__shfl(first.sum, 63, 64));
+  int64_t total = at_lane(first.sum, 63);
   for (int base = 64; base < p.seqs; base += 64)
-    total += uniform(__shfl(count_tiles(p, most, block_rows, lane, base).sum, 63, 64));
+    total += at_lane(count_tiles(p, most, block_rows, lane, base).sum, 63);
   return total * p.cache.heads;
 }
 
@@ -133,9 +133,9 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
       const int which = hit ? __builtin_ctzll(hit) : 0;
       Place place;
       place.seq = uniform(c.base + which);
-      place.tiles = uniform(__shfl(c.tiles, which, 64));
-      place.blocks = max(uniform(__shfl(c.blocks, which, 64)), 1);
-      const int in_front = uniform(__shfl(c.sum, which, 64)) - place.tiles * place.blocks;
+      place.tiles = at_lane(c.tiles, which);
+      place.blocks = max(at_lane(c.blocks, which), 1);
+      const int in_front = at_lane(c.sum, which) - place.tiles * place.blocks;
       const int64_t inside = at - before - int64_t(in_front) * heads;
       const int context = uniform(int(inside / place.tiles));
       place.tile = uniform(int(inside % place.tiles));
@@ -143,7 +143,7 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
       place.block = uniform(context % place.blocks);
       return place;
     }
-    before += int64_t(uniform(__shfl(c.sum, 63, 64))) * heads;
+    before += int64_t(at_lane(c.sum, 63)) * heads;
     c = count_tiles(p, most, block_rows, lane, c.base + 64);
   }
 }
