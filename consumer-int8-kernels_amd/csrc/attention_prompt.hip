@@ -7,8 +7,10 @@
 // head of one key head) pairs, 256 a workgroup, so that heads that share a key head share its
 // tiles. Four operations a score and channel: bound by the MFMA rate, then by the softmax's
 // vector instructions (about five a score) and by LDS reads (each wave reads every tile). Two waves a
-// SIMD of 32 rows each (one at D = 256, whose sums take its registers), in alternate phases: the
-// scores of the next tile are on the matrix unit while the vector unit weighs those of this one.
+// SIMD of 32 rows each, in alternate phases: the scores of the next tile are on the matrix unit while
+// the vector unit weighs those of this one. Measured: 4096 tokens of 40 query and 8 key heads of 128
+// 192 us, 890 TFLOP/s of what the mask leaves (a large product reaches 1157 to 1265); 24 and 4 of
+// 256 245 us, 840 (415 us with one wave a SIMD that holds all its queries).
 //
 // Tiles of keys and values are converted to BF16 once a workgroup, on their way into LDS: global
 // loads run two tiles ahead, one barrier a tile.
@@ -24,7 +26,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <int D>
 struct Shape {
   static constexpr int kTiles = 1;  // of a wave
-  static constexpr int kWaves = D <= 128 ? 8 : 4;
+  static constexpr int kWaves = 8;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 32 * kTiles * kWaves;
   static constexpr int kTokens = D == 64 ? 128 : D == 128 ? 64 : 32;
@@ -117,6 +119,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   using S = Shape<D>;
   constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = kTokens / 32;
   constexpr int kSteps = D / 16, kChannels = D / 32;
+  // The waves' queries stay in registers; where the sums leave room for half of them, the others are
+  // in LDS.
+  constexpr int kHeld = D == 256 ? kSteps / 2 : kSteps;
+  __shared__ u32x4 late_q[D == 256 ? (kSteps - kHeld) * S::kThreads : 1];
   // Three buffers of keys, then two of values.
   __shared__ __align__(256) char lds[S::kLdsBytes];
   constexpr int kValues = S::kKeyBuffers * S::kKeyBytes;
@@ -178,12 +184,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   // waited for, at the loop's end.
   const uint32_t scale_byte = lane_token % 16 * S::kBlocks + block;
   const uint32_t scale_turn = fp4_scale_turn(scale_byte % 4);
+  // The lane's bytes from its row of 16 tokens on.
+  const uint32_t code_at = lane_token % 16 * (D / 2) + 16 * block, scale_at = scale_byte & ~3u;
   struct Pack {
     bool value;
     int token;                // the wave's first in a tile
-    const uint8_t *codes, *scales;  // of this head's rows in page 0, at the lane's place
+    const uint8_t *codes, *scales;  // of this head's rows in page 0
     int64_t code_stride, scale_stride;
-    int to[4];                // LDS bytes of the lane's four pieces in the first buffer
+    int to;                   // LDS byte of the lane's first piece in the first buffer
   };
   auto pack = [&](int c) __attribute__((always_inline)) {
     Pack x;
@@ -191,15 +199,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     x.token = (c * S::kThreads + 64 * wave) % kPerTile / S::kBlocks;
     const Fp4Rows& rows = x.value ? p.cache.v : p.cache.k;
     const int64_t row = int64_t(kv_head) << p.cache.page_shift;
-    x.codes = rows.codes + row * (D / 2) + lane_token % 16 * (D / 2) + 16 * block;
-    x.scales = rows.scales + row * S::kBlocks + (scale_byte & ~3u);
+    x.codes = rows.codes + row * (D / 2);
+    x.scales = rows.scales + row * S::kBlocks;
     x.code_stride = rows.code_stride;
     x.scale_stride = rows.scale_stride;
     const int token = x.token + lane_token;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x.to[j] = x.value ? kValues + S::value_at(token, block, j)
-                        : token * S::kKeyPitch + 64 * block + 16 * j;
+    x.to = x.value ? kValues + S::value_at(token, block, 0) : token * S::kKeyPitch + 64 * block;
     return x;
   };
   Pack packs[S::kPacks];
@@ -239,8 +244,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         code = lane_token >= 16 ? code2 : code;
         scale = lane_token >= 16 ? scale2 : scale;
       }
-      staged.codes[c] = *reinterpret_cast<const u32x4*>(x.codes + code);
-      staged.scales[c] = *reinterpret_cast<const uint32_t*>(x.scales + scale);
+      staged.codes[c] = *reinterpret_cast<const u32x4*>(x.codes + code + code_at);
+      staged.scales[c] = *reinterpret_cast<const uint32_t*>(x.scales + scale + scale_at);
     }
   };
 
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
   // go nowhere.
   int row_low[kTiles], row_high[kTiles];
-  u32x4 q[kTiles][kSteps];
+  u32x4 q[kTiles][kHeld];
   const int wave_row = row0 + wave * 32 * kTiles;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
@@ -272,8 +277,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
                           int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
-      q[n][j] = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
+    for (int j = 0; j < kSteps; ++j) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(src + 16 * j + 8 * half) ^ p.q_sign;
+      if (j < kHeld)
+        q[n][j] = x;
+      else
+        late_q[(j - kHeld) * S::kThreads + thread] = x;
+    }
   }
   if (t_begin < t_end) {
     load_codes(staged, pages_first, t_begin, t_begin);
@@ -326,7 +336,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       const int buffer = x.value ? (tv & 1) * S::kValueBytes : key_buffer * S::kKeyBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<u32x4*>(lds + (x.to[j] + buffer)) =
+        *reinterpret_cast<u32x4*>(
+            lds + (((x.to + buffer) ^ (x.value ? 16 * j : 0)) + (x.value ? 0 : 16 * j))) =
             fp4_to_bf16x8(codes[j], fp4_scale_in(scales, scale_turn));
     }
   };
@@ -346,7 +357,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 #pragma unroll
       for (int i = 0; i < 16; ++i) score[n][i] = 0;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
+    for (int j = 0; j < kHeld; ++j)
 #pragma unroll
       for (int n = 0; n < kTiles; ++n)
         score[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -424,21 +435,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     }
   };
   u32x4 value[2][kChannels];
-  auto read_values = [&](int t, int b) __attribute__((always_inline)) {
+  auto read_value = [&](int t, int b, int c, int m) __attribute__((always_inline)) {
     // The lane's row of four and its 8 bytes of the 64 that two groups of 16 lanes read: piece
     // 2 * (lane / 16 % 2) + lane % 4 / 2. Tokens of other fours keep its place in the row.
     const int row = 4 * half + lane % 16 / 4, piece = 2 * (lane / 16 % 2) + lane % 4 / 2;
-    const char* from = lds + (kValues + (t & 1) * S::kValueBytes + 32 * b * S::kValuePitch) +
-                       lane % 2 * 8;
+    const char* at = lds + (kValues + (t & 1) * S::kValueBytes + 32 * b * S::kValuePitch) +
+                     lane % 2 * 8 + S::value_at(row, m, piece) + 16 * c * S::kValuePitch;
+    const u32x2 x = lds_read_transposed(at);
+    const u32x2 y = lds_read_transposed(at + 8 * S::kValuePitch);
+    return u32x4{x[0], x[1], y[0], y[1]};
+  };
+  auto read_values = [&](int t, int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int m = 0; m < kChannels; ++m) {
-        const char* at = from + S::value_at(row, m, piece) + 16 * c * S::kValuePitch;
-        const u32x2 x = lds_read_transposed(at);
-        const u32x2 y = lds_read_transposed(at + 8 * S::kValuePitch);
-        value[c][m] = u32x4{x[0], x[1], y[0], y[1]};
-      }
+      for (int m = 0; m < kChannels; ++m) value[c][m] = read_value(t, b, c, m);
   };
   auto add_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -465,6 +476,33 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   };
 
   f32x16 scores[kTiles];
+  static_assert(kAhead ? kHeld == kSteps : kTiles == 1);
+  // At D = 256 operands are read where they are used, a few at a time: all of a tile's would not fit
+  // beside the sums.
+  auto stream_scores = [&](int buffer) __attribute__((always_inline)) {
+    const char* from = lds + buffer * S::kKeyBytes + column * S::kKeyPitch + 16 * half;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scores[0][i] = 0;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const u32x4 query = j < kHeld ? q[0][j] : late_q[(j - kHeld) * S::kThreads + thread];
+      scores[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(from + 32 * j)),
+          __builtin_bit_cast(bf16x8, query), scores[0], 0, 0, 0);
+      if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto stream_values = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < kChannels; ++m) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        o[0][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, read_value(t, 0, c, m)),
+            __builtin_bit_cast(bf16x8, weights[0][c]), o[0][m], 0, 0, 0);
+      if (m % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
   if (t_begin < t_end) {
     // In a tile's step the keys of the next tile but one are staged, and the values of the next.
     store_tiles(staged, 0, t_begin);
@@ -472,8 +510,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     load_pages(pages, t_begin + 3, t_begin + 2);
     store_tiles(ahead, 1, t_begin);
     __syncthreads();
-    read_keys(0, 0);
-    multiply(scores);
+    if (kAhead) {
+      read_keys(0, 0);
+      multiply(scores);
+    } else {
+      stream_scores(0);
+    }
     scale(scores);
     if (kAhead) {
       read_keys(1 / kHalves, 1 % kHalves);
@@ -485,17 +527,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 #pragma unroll
     for (int b = 0; b < kHalves; ++b) {
       // Weighs this half's scores, and stages what the next halves read.
-      if (!kAhead) read_keys(buffer[1], 0);
       settle(t * kTokens + 32 * b, scores);
       weigh(scores);
       if (b == 0) store_tiles(staged, buffer[2], t + 1);
       // This half's values, the next half's scores (past the last tile those of old keys, which
       // nothing reads), and the operands after those.
       __builtin_amdgcn_s_setprio(1);
-      if (!kAhead) read_values(t, b);
-      multiply(scores);
+      if (kAhead)
+        multiply(scores);
+      else
+        stream_scores(buffer[1]);
       if (kAhead) read_keys(buffer[(b + 2) / kHalves], (b + 2) % kHalves);
-      add_values();
+      if (kAhead)
+        add_values();
+      else
+        stream_values(t);
       if (kAhead) read_values(t + (b + 1) / kHalves, (b + 1) % kHalves);
       scale(scores);
       if (b == 0) {
