@@ -11,6 +11,7 @@ constexpr float kLowest = -3.402823466e38f;
 // weights stay in FP32, and BF16 weights are as exact at any size.
 constexpr float kSlack = 8.f;
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 

@@ -14,6 +14,8 @@
 //
 // Tiles of keys and values are converted to BF16 once a workgroup, on their way into LDS: global
 // loads run two tiles ahead, one barrier a tile.
+#include <type_traits>
+
 #include "attention_device.h"
 #include "launch.h"
 
@@ -627,15 +629,35 @@ __global__ void __launch_bounds__(kJoinThreads)
   if (row >= s.rows) return;
   const int64_t first = int64_t(cut) * c.splits * kRows + r;
   float top = kLowest, total = 0;
-  for (int i = 0; i < c.splits; ++i)
-    top = fmaxf(top, part_stats(p, first + int64_t(i) * kRows, D)[0]);
   f32x4 x = {0, 0, 0, 0};
-  for (int i = 0; i < c.splits; ++i) {
-    const int64_t at = first + int64_t(i) * kRows;
-    const float factor = __builtin_amdgcn_exp2f(part_stats(p, at, D)[0] - top);
-    total += part_stats(p, at, D)[1] * factor;
-    x += *reinterpret_cast<const f32x4*>(part_sums(p, at, D) + channel) * factor;
-  }
+  // Parts i .. i + n - 1, on their way together; past the last they are that one again, and count 0.
+  auto add = [&](int i, auto n) {
+    f32x2 stats[n];
+    f32x4 sums[n];
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const int64_t at = first + int64_t(min(i + j, c.splits - 1)) * kRows;
+      stats[j] = *reinterpret_cast<const f32x2*>(part_stats(p, at, D));
+      sums[j] = *reinterpret_cast<const f32x4*>(part_sums(p, at, D) + channel);
+    }
+    float most = top;
+#pragma unroll
+    for (int j = 0; j < n; ++j) most = fmaxf(most, stats[j][0]);
+    const float old = __builtin_amdgcn_exp2f(top - most);
+    top = most;
+    total *= old;
+    x *= old;
+#pragma unroll
+    for (int j = 0; j < n; ++j)
+      if (i + j < c.splits) {
+        const float factor = __builtin_amdgcn_exp2f(stats[j][0] - most);
+        total += stats[j][1] * factor;
+        x += sums[j] * factor;
+      }
+  };
+  int i = 0;
+  for (; i + 8 <= c.splits; i += 8) add(i, std::integral_constant<int, 8>());
+  for (; i < c.splits; i += 2) add(i, std::integral_constant<int, 2>());
   write_row4(p, D, s.q_begin, row, unit % p.cache.heads, channel, x, top, total);
 }
 

@@ -153,7 +153,6 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
 // begins a context says of it: one for each context (0 parts: its output is written), or, where
 // contexts are more than workgroups, for each workgroup, which begins one at most that another
 // continues.
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct Joint {
   int parts, first, q_begin, row0, rows, head, unused[2];
 };
