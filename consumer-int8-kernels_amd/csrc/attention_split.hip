@@ -21,13 +21,13 @@
 // 2^8 in weight, so most tiles exchange nothing between lanes and rescale nothing.
 //
 // Contexts differ and only the device knows them, so the work is cut there: all tiles of all
-// sequences, key heads and blocks of rows are laid end to end and each workgroup takes an equal run
-// of them.
+// sequences, key heads and blocks of rows are laid end to end, each context with what it costs to
+// begin it, and each workgroup takes an equal run of them.
 // A run that covers a whole context writes its output; parts of one go to the workspace, two
 // at most a workgroup, and a second kernel joins them in a fixed order.
 //
 // Measured, of the cache's bytes: 64 contexts up to 32768 tokens, 64 query heads on 8 of 128, 257
-// us, 5.5 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 43 us, 3.4 TB/s with
+// us, 5.5 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 38 us, 3.9 TB/s with
 // the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
 // the launch.
 #include "attention_device.h"
@@ -86,44 +86,49 @@ __device__ __forceinline__ int row_blocks(const Sequence& s, int most, int block
   return s.rows > most ? 0 : (s.rows + block_rows - 1) / block_rows;
 }
 __device__ __forceinline__ int block_tiles(const Sequence& s) { return max(s.tiles(kTokens), 1); }
+// What it costs to begin a context, in tiles: queries and pages on their way in and sums out take a
+// workgroup 9000 clocks, a tile 800 with three workgroups a CU. Not counted, workgroups that had four
+// short contexts ran 73000 clocks where others ran 47000: 32 contexts up to 8000 41 us, counted 37.7,
+// 64 from 100 to 4000 58 and 39.
+constexpr int kBegin = 10;
 
-// A run of tiles: [begin, end) of the row of all sequences' tiles, one after the other for each
-// key head and block of rows.
+// A run: [begin, end) of the row of all sequences' costs, one after the other for each key head and
+// block of rows.
 struct Run {
   int64_t begin, end, quota;
 };
 struct Place {
-  int seq, head, block, blocks, tile, tiles;  // tile: from the sequence's first
+  int seq, head, block, blocks, at, cost;  // at: of its cost
 };
 
-// Of 64 sequences from `base` on, one a lane: blocks of a key head, tiles of a block, and sums of
+// Of 64 sequences from `base` on, one a lane: blocks of a key head, cost of a block, and sums of
 // both's products up to each lane's.
 struct Counted {
-  int base, blocks, tiles, sum;
+  int base, blocks, cost, sum;
 };
-__device__ __forceinline__ Counted count_tiles(const AttentionArgs& p, int most, int block_rows,
-                                               int lane, int base) {
+__device__ __forceinline__ Counted count_costs(const AttentionArgs& p, int most, int block_rows,
+                                               int begin, int lane, int base) {
   Counted c = {base, 0, 1, 0};
   if (base + lane < p.seqs) {
     const Sequence s = sequence(p, base + lane);
     c.blocks = row_blocks(s, most, block_rows);
-    c.tiles = block_tiles(s);
+    c.cost = block_tiles(s) + begin;
   }
-  c.sum = wave_scan(c.blocks * c.tiles);
+  c.sum = wave_scan(c.blocks * c.cost);
   return c;
 }
-// Tiles of all; `first` are those of the first 64 sequences.
-__device__ __forceinline__ int64_t all_tiles(const AttentionArgs& p, int most, int block_rows,
-                                             int lane, const Counted& first) {
+// Costs of all; `first` are those of the first 64 sequences.
+__device__ __forceinline__ int64_t all_costs(const AttentionArgs& p, int most, int block_rows,
+                                             int begin, int lane, const Counted& first) {
   int64_t total = at_lane(first.sum, 63);
   for (int base = 64; base < p.seqs; base += 64)
-    total += at_lane(count_tiles(p, most, block_rows, lane, base).sum, 63);
+    total += at_lane(count_costs(p, most, block_rows, begin, lane, base).sum, 63);
   return total * p.cache.heads;
 }
 
-// Where tile `at` of all lies; at is less than their number. `first`: of the first 64 sequences.
-__device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int block_rows,
-                                           int lane, int64_t at, const Counted& first) {
+// Where `at` of all costs lies; it is less than their sum. `first`: of the first 64 sequences.
+__device__ __forceinline__ Place find_place(const AttentionArgs& p, int most, int block_rows,
+                                            int begin, int lane, int64_t at, const Counted& first) {
   const int heads = p.cache.heads;
   Counted c = first;
   int64_t before = 0;
@@ -133,18 +138,18 @@ __device__ __forceinline__ Place find_tile(const AttentionArgs& p, int most, int
       const int which = hit ? __builtin_ctzll(hit) : 0;
       Place place;
       place.seq = uniform(c.base + which);
-      place.tiles = at_lane(c.tiles, which);
+      place.cost = at_lane(c.cost, which);
       place.blocks = max(at_lane(c.blocks, which), 1);
-      const int in_front = at_lane(c.sum, which) - place.tiles * place.blocks;
+      const int in_front = at_lane(c.sum, which) - place.cost * place.blocks;
       const int64_t inside = at - before - int64_t(in_front) * heads;
-      const int context = uniform(int(inside / place.tiles));
-      place.tile = uniform(int(inside % place.tiles));
+      const int context = uniform(int(inside / place.cost));
+      place.at = uniform(int(inside % place.cost));
       place.head = uniform(context / place.blocks);
       place.block = uniform(context % place.blocks);
       return place;
     }
     before += int64_t(at_lane(c.sum, 63)) * heads;
-    c = count_tiles(p, most, block_rows, lane, c.base + 64);
+    c = count_costs(p, most, block_rows, begin, lane, c.base + 64);
   }
 }
 
@@ -188,7 +193,7 @@ constexpr int groups_per_cu(int dim, int tiles) {
 template <int D, int kTiles, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) * kWaves / 4 : kWaves / 4)
     attention_split_kernel(const AttentionArgs, int most, int most_blocks, int min_quota,
-                           bool by_context) {
+                           bool by_context, bool apart) {
   using L = Layout<D>;
   constexpr int kRows = 16 * kTiles;
   constexpr int kTileBytes = kTokens * L::kPitch;
@@ -206,18 +211,32 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane % 16, group4 = lane / 16;
 
+  // Contexts that are few against the workgroups lie apart: each takes a whole number of equal runs,
+  // so that no workgroup has two. Counted are at most 64 sequences then.
+  const int begin = apart ? 0 : kBegin;
   Run run;
   Place place;
   if constexpr (kSplit) {
     const AttentionArgs& p = arguments();
-    const Counted counted = count_tiles(p, most, kRows, lane, 0);
-    const int64_t total = all_tiles(p, most, kRows, lane, counted);
+    Counted counted = count_costs(p, most, kRows, begin, lane, 0);
+    int64_t total = all_costs(p, most, kRows, begin, lane, counted);
     run.quota = uniform(max((total + gridDim.x - 1) / gridDim.x, int64_t(min_quota)));
+    if (apart) {
+      int quota = int(run.quota), parts;
+      for (;; quota += quota / 64 + 1) {
+        parts = (counted.cost + quota - 1) / quota;
+        if (wave_sum(counted.blocks * parts) * p.cache.heads <= int(gridDim.x)) break;
+      }
+      counted.cost = parts * quota;
+      counted.sum = wave_scan(counted.blocks * counted.cost);
+      total = int64_t(at_lane(counted.sum, 63)) * p.cache.heads;
+      run.quota = quota;
+    }
     run.begin = blockIdx.x * run.quota;
     run.end = min(run.begin + run.quota, total);
     if (!by_context && threadIdx.x == 0) joints<D>(p)[blockIdx.x].parts = 0;
     if (run.begin >= total) return;
-    place = find_tile(p, most, kRows, lane, run.begin, counted);
+    place = find_place(p, most, kRows, begin, lane, run.begin, counted);
   } else {
     const AttentionArgs& p = arguments();
     place.block = blockIdx.x % most_blocks;
@@ -226,9 +245,9 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     const Sequence s = sequence(p, place.seq);
     place.blocks = uniform(row_blocks(s, most, kRows));
     if (place.block >= place.blocks) return;
-    place.tile = 0;
-    place.tiles = uniform(block_tiles(s));
-    run = {0, place.tiles, place.tiles};
+    place.at = 0;
+    place.cost = uniform(block_tiles(s));
+    run = {0, place.cost, place.cost};
   }
   // Where this lane's rows of 16 tokens start, and its place in the LDS tile.
   const uint32_t code_at = column * (D / 2) + group4 * (L::kChunk / 2);
@@ -244,8 +263,15 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     const int page_mask = (1 << p.cache.page_shift) - 1;
     const Sequence s = sequence(p, seq);
     const int row0 = place.block * kRows, rows = min(s.rows - row0, kRows);
-    const int take = int(min(int64_t(place.tiles - place.tile), run.end - at));
-    const int t_begin = s.first_tile(kTokens) + place.tile, t_end = t_begin + take;
+    const int take = int(min(int64_t(place.cost - place.at), run.end - at));
+    // The run's share of the context's cost is its share of the tiles.
+    const int tiles = block_tiles(s);
+    const float share = float(tiles) / float(place.cost);
+    auto tile_at = [&](int cost) {
+      return s.first_tile(kTokens) +
+             uniform(cost == place.cost ? tiles : min(int(float(cost) * share), tiles));
+    };
+    const int t_begin = tile_at(place.at), t_end = tile_at(place.at + take);
 
     // The lane's rows: their queries, and the tokens [low, high) that each attends to.
     int low[kTiles], high[kTiles];
@@ -493,8 +519,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       }
     }
     __syncthreads();
-    const bool whole = place.tile == 0 && take == place.tiles;
-    const int part = 2 * blockIdx.x + (place.tile == 0 ? 1 : 0);
+    const bool whole = place.at == 0 && take == place.cost;
+    const int part = 2 * blockIdx.x + (place.at == 0 ? 1 : 0);
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       float top = kLowest;
@@ -531,8 +557,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       }
       __syncthreads();
     }
-    if (kSplit && place.tile == 0 && (by_context || !whole) && threadIdx.x == 0) {
-      const int64_t last = at + place.tiles - 1;
+    if (kSplit && place.at == 0 && (by_context || !whole) && threadIdx.x == 0) {
+      const int64_t last = at + place.cost - 1;
       const int context = (seq * p.cache.heads + kv_head) * most_blocks + place.block;
       joints<D>(p)[by_context ? context : int(blockIdx.x)] = {
           whole ? 0 : int(last / run.quota) - int(blockIdx.x) + 1, int(blockIdx.x), s.q_begin,
@@ -541,19 +567,19 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     // On to the next block, key head or sequence.
     at += take;
     if (at < run.end) {
-      place.tile = 0;
+      place.at = 0;
       if (place.block + 1 < place.blocks) {
         ++place.block;
       } else if (place.block = 0; place.head + 1 < p.cache.heads) {
         ++place.head;
       } else {
-        // More tiles are left, so a later sequence has some.
+        // More is left, so a later sequence has some.
         place.head = 0;
         do {
           ++place.seq;
           const Sequence next = sequence(p, place.seq);
           place.blocks = uniform(row_blocks(next, most, kRows));
-          place.tiles = uniform(block_tiles(next));
+          place.cost = uniform(block_tiles(next)) + begin;
         } while (place.blocks == 0 && place.seq + 1 < p.seqs);
       }
     }
@@ -680,7 +706,7 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
     // heads of 256, 64 contexts up to 1500, 25.5 and 32.4.
     constexpr int kWaves = 8;
     attention_split_kernel<D, kTiles, kWaves, false>
-        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, most, blocks, 0, false);
+        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, most, blocks, 0, false, false);
     return hipGetLastError();
   }
   // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
@@ -696,8 +722,12 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
                         kAttentionWorkspaceRows * 2 - 2048 * 8,
                 "parts, statistics and descriptions fit the workspace");
   const bool by_context = contexts <= groups;
+  // With two workgroups a context or more, us, and with runs of all: one of 100000 tokens of 4 heads
+  // of 256 28.1 and 31.5, 9 up to 90857 of 8 of 128 113 and 116, 4 up to 5000 14 and 17; but 32 up to
+  // 8000 (three a context) 38.1 and 37.7.
+  const bool apart = 2 * contexts <= groups && args.seqs <= 64;
   attention_split_kernel<D, kTiles, kWaves, true>
-      <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context);
+      <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context, apart);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   // More threads where a context has many parts: one of 131071 tokens of 4 heads, 64 parts each,
   // is joined in 5.0 us, by 256 threads in 7.2; 32 contexts up to 8000, 4 parts, in 8.8 and 4.9.
