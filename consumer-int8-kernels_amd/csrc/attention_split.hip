@@ -691,8 +691,10 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Up to this many tiles of the longest context a workgroup takes a whole context.
-constexpr int kWholeTiles = 64;
+// Up to this many tiles of the longest context a workgroup takes a whole context: fewer where contexts
+// leave most of the GPU idle. Whole and split, us: 16 contexts up to 2000 tokens of 8 heads of 128 14.4
+// and 15.8, 4 of them 13.5 and 11.5, one of 1100 9.6 and 11.3; 16 of 4 heads of 256 23.9 and 17.6.
+constexpr int whole_tiles(int dim, bool few) { return !few ? 64 : dim == 256 ? 32 : 48; }
 
 template <int D, int kTiles>
 hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream) {
@@ -701,7 +703,8 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   const int64_t rows = int64_t(args.max_q) * args.group;
   const int blocks = int(((rows < most ? rows : most) + 16 * kTiles - 1) / (16 * kTiles));
   const int64_t contexts = int64_t(args.seqs) * args.cache.heads * blocks;
-  if ((longest < span ? longest : span) <= kWholeTiles) {
+  const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
+  if ((longest < span ? longest : span) <= whole_tiles(D, 4 * contexts <= cus)) {
     // Eight waves: 517 tokens of 8 key heads of 128 7.6 us, with four 8.3; 4 rows a sequence of 6
     // heads of 256, 64 contexts up to 1500, 25.5 and 32.4.
     constexpr int kWaves = 8;
@@ -709,13 +712,12 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
         <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, most, blocks, 0, false, false);
     return hipGetLastError();
   }
-  // Four waves a workgroup: 32 contexts up to 8000 tokens of 8 heads of 128 take 42 us, with eight
-  // 59; 64 up to 32768 257 and 278. Where the queries are in LDS eight share them: 16 x 4 rows up to
-  // 16000 of 4 heads of 256 58 us, with four 67. At D = 256 contexts that are few get fewer
-  // workgroups and so fewer parts to join: one of 131071 tokens of 4 heads 37 us, with two a CU 39;
-  // 32 up to 9000 53 and 50.
+  // Four waves a workgroup; each pair of times was taken in turn, before runs counted beginnings: 32
+  // contexts up to 8000 tokens of 8 heads of 128 42 us, with eight waves 59; 64 up to 32768 257 and
+  // 278. Where the queries are in LDS eight waves share them: 16 x 4 rows up to 16000 of 4 heads of 256
+  // 58 us, with four 67. At D = 256 contexts that are few get one workgroup a CU and so fewer parts to
+  // join: one of 131071 tokens of 4 heads 32.6 us, with two 34.9; 12 up to 9000 23.2 and 25.7.
   constexpr int kWaves = D == 256 && kTiles == 2 ? 8 : 4;
-  const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(groups_per_cu(D, kTiles) <= 8 &&
                     2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
