@@ -29,7 +29,7 @@ attention_fp4(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens,
     how many tokens a query sees, itself included (0: all). out BF16 like q, contiguous;
     lse FP32 [T,Hq] or None. Queries that see nothing give zeros and -inf. workspace FP32
     [65536, D + 2], of any content, used by one stream at a time. Cache tensors span at most
-    32 GiB each, page tables width * page_size <= 2^28 - 4096 tokens.
+    32 GiB each, page tables width * page_size <= 2^26 - 4096 tokens.
 """
 
 from typing import NamedTuple

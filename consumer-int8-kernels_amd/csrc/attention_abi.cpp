@@ -322,8 +322,9 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
     return abi_fail(CI8_ERR_GEOMETRY,
                     "Invalid attention: expected at most 65535 sequences, max_q >= 1, window >= "
                     "0, a finite scale, and q_starts unless each sequence has one query");
-  // Tiles of 32 tokens, of 4 row blocks each of 64 sequences, are summed in 32 bits.
-  if (i128(table_width) * cache->page_size > (1 << 28) - 4096 ||
+  // Tiles of 32 tokens, of 4 row blocks each of 64 sequences, are summed in 32 bits, and up to twice
+  // as many where each context takes a whole number of runs.
+  if (i128(table_width) * cache->page_size > (1 << 26) - 4096 ||
       i128(seqs) * table_width * 4 > kMaxExtent)
     return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large");
   if (!aligned(page_table, 4) || !aligned(context_lens, 4) || !aligned(q_starts, 4) ||

@@ -27,8 +27,8 @@
 // at most a workgroup, and a second kernel joins them in a fixed order.
 //
 // Measured, of the cache's bytes: 64 contexts up to 32768 tokens, 64 query heads on 8 of 128, 257
-// us, 5.5 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 38 us, 3.9 TB/s with
-// the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
+// to 266 us, 5.4 to 5.6 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 40 us, 3.7
+// TB/s with the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
 // the launch.
 #include "attention_device.h"
 #include "launch.h"

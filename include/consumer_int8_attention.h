@@ -122,7 +122,7 @@ int ci8_unpack_fp4(const ci8_fp4_cache* cache, const int64_t* slots, void* k, vo
  * statistics FP32, the weights rounded to BF16 before they meet the values.
  * workspace: FP32 [65536, dim + 2], 16-byte aligned, any content, one a stream.
  * q heads a multiple of the cache's heads; scale finite; max_q >= 1; window >= 0;
- * table_width * page_size at most 2^28 - 4096. */
+ * table_width * page_size at most 2^26 - 4096. */
 int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
                       const int32_t* page_table, int64_t table_width,
                       const int32_t* context_lens, const int32_t* q_starts, int64_t seqs,

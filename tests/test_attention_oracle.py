@@ -318,7 +318,7 @@ def test_extent_refusals(lib):
                                      FAKE << 12, FAKE + (1 << 26), None, 0.1, 1, 0, None)
 
     size = cache().page_size
-    most = ((1 << 28) - 4096) // size
+    most = ((1 << 26) - 4096) // size
     refused(lib, call(cache(), most + 1), large, "Page table too large")
     assert call(cache(), most) == 0
     far = dict(k_codes=1 << 40, k_scales=1 << 41, v_codes=1 << 42, v_scales=1 << 43)
