@@ -10,7 +10,7 @@
 // SIMD of 32 rows each, in alternate phases: the scores of the next tile are on the matrix unit while
 // the vector unit weighs those of this one. Measured: 4096 tokens of 40 query and 8 key heads of 128
 // 192 us, 890 TFLOP/s of what the mask leaves (a large product reaches 1157 to 1265); 24 and 4 of
-// 256 245 us, 840 (415 us with one wave a SIMD that holds all its queries).
+// 256 241 us, 855 (415 us with one wave a SIMD that holds all its queries).
 //
 // Tiles of keys and values are converted to BF16 once a workgroup, on their way into LDS: global
 // loads run two tiles ahead, one barrier a tile.

@@ -724,10 +724,11 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
                         kAttentionWorkspaceRows * 2 - 2048 * 8,
                 "parts, statistics and descriptions fit the workspace");
   const bool by_context = contexts <= groups;
-  // With two workgroups a context or more, us, and with runs of all: one of 100000 tokens of 4 heads
-  // of 256 28.1 and 31.5, 9 up to 90857 of 8 of 128 113 and 116, 4 up to 5000 14 and 17; but 32 up to
-  // 8000 (three a context) 38.1 and 37.7.
-  const bool apart = 2 * contexts <= groups && args.seqs <= 64;
+  // With more than three workgroups a context, us, and with runs of all: one of 100000 tokens of 4
+  // heads of 256 28.1 and 31.5, 9 up to 90857 of 8 of 128 113 and 116, 4 up to 5000 14 and 17, 51 up
+  // to 3006 of 4 (3.8 a context) 21.8 and 23.5; but 32 up to 8000 of 8 (3) 38.1 and 37.7, 16 x 5 rows
+  // of 64 heads up to 16000 (2) 91 and 81.
+  const bool apart = 3 * contexts < groups && args.seqs <= 64;
   attention_split_kernel<D, kTiles, kWaves, true>
       <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context, apart);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -744,9 +745,9 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
 
 // Up to this many rows a sequence are few: above 32 in blocks that each read the cache, which the
 // caches between them and HBM mostly hold. With the prompt kernel's 256 rows a workgroup instead,
-// us: 16 x 5 tokens behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 220, 16
-// tokens each 151 and 224, 32 tokens (256 rows) behind 30000 132 and 125; 4 x 32 tokens of 24 and 4
-// of 256 65 and 135; 16 x 100 rows of 16 heads of 64 203 and 280.
+// us: 16 x 5 tokens behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 216, 16
+// tokens each 147 and 223, 32 tokens (256 rows) behind 30000 142 and 123; 4 x 32 tokens (192 rows) of
+// 24 and 4 of 256 67 and 85; 16 x 100 rows of 16 heads of 64 200 and 269, 2 x 200 66 and 49.
 constexpr int kMostRows = 128;
 
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
