@@ -18,6 +18,7 @@
 
 #include "attention_device.h"
 #include "launch.h"
+#include "prompt_schedule.h"
 
 namespace ci8 {
 namespace {
@@ -40,8 +41,9 @@ struct Shape {
   static constexpr int kKeyBytes = kTokens * kKeyPitch, kValueBytes = kTokens * kValuePitch;
   static constexpr int kPacks = 2 * kTokens * kBlocks / kThreads;  // 16 bytes of codes a thread
   static_assert(2 * kTokens * kBlocks % kThreads == 0);
-  static constexpr int kKeyBuffers = 3;
-  static constexpr int kLdsBytes = kKeyBuffers * kKeyBytes + 2 * kValueBytes;
+  static constexpr int kHalves = kTokens / 32;
+  static_assert(schedule_holds(kHalves, barrier_half(kHalves)), "LDS buffers are not raced for");
+  static constexpr int kLdsBytes = kKeyBuffers * kKeyBytes + kValueBuffers * kValueBytes;
   static_assert(kKeyBuffers * kKeyBytes % 256 == 0);
   // Byte of piece j (8 channels) of a token's block in a buffer of values: among the 256 bytes
   // that hold it, blocks are XORed by the token, and in a block the pieces are.
@@ -119,17 +121,17 @@ template <int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads)
     attention_prompt_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
   using S = Shape<D>;
-  constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = kTokens / 32;
+  constexpr int kTokens = S::kTokens, kTiles = S::kTiles, kHalves = S::kHalves;
   constexpr int kSteps = D / 16, kChannels = D / 32;
   // The waves' queries stay in registers; where the sums leave room for half of them, the others are
   // in LDS.
   constexpr int kHeld = D == 256 ? kSteps / 2 : kSteps;
   __shared__ u32x4 late_q[D == 256 ? (kSteps - kHeld) * S::kThreads : 1];
-  // Three buffers of keys, then two of values.
+  // The buffers of keys, then those of values.
   __shared__ __align__(256) char lds[S::kLdsBytes];
-  constexpr int kValues = S::kKeyBuffers * S::kKeyBytes;
-  __shared__ uint8_t poison[3][kTokens][S::kBlocks];      // NaN blocks of edge tiles
-  __shared__ int poisoned[3];                             // the last such tile that has any
+  constexpr int kValues = kKeyBuffers * S::kKeyBytes;
+  __shared__ uint8_t poison[kPoisonBuffers][kTokens][S::kBlocks];  // NaN blocks of edge tiles
+  __shared__ int poisoned[kPoisonBuffers];  // the last such tile that has any
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6);
   const int column = lane & 31, half = lane >> 5;
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     sum[n] = 0;
   }
 
-  if (thread < 3) poisoned[thread] = -1;
+  if (thread < kPoisonBuffers) poisoned[thread] = -1;
   const bool any_missing = __syncthreads_or(missing);
 
   auto there = [&](int token) __attribute__((always_inline)) {
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   auto edge_tile = [&](int t) __attribute__((always_inline)) {
     return (t + 1) * kTokens > first_high || t * kTokens < last_low;
   };
-  // key_buffer: where tile tk goes, t % 3 of some count.
+  // key_buffer: where tile tk goes, one of the three in turn.
   auto store_tiles = [&](const Staged& staged, int key_buffer, int tv) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < S::kPacks; ++c) {
@@ -330,12 +332,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         const int token = tv * kTokens + x.token + lane_token;
         const bool real = token < s.context && (!any_missing || there(token));
         const bool nan = real && (scales >> scale_byte % 4 * 8 & 0xFF) >= 253 && edge_tile(tv);
-        poison[tv % 3][x.token + lane_token][block] = nan;
-        if (nan) poisoned[tv % 3] = tv;
+        poison[tv % kPoisonBuffers][x.token + lane_token][block] = nan;
+        if (nan) poisoned[tv % kPoisonBuffers] = tv;
         codes = nan || !real ? u32x4{0, 0, 0, 0} : codes;
         scales = nan || !real ? 0 : scales;
       }
-      const int buffer = x.value ? (tv & 1) * S::kValueBytes : key_buffer * S::kKeyBytes;
+      const int buffer = x.value ? int(uint32_t(tv) % kValueBuffers) * S::kValueBytes : key_buffer * S::kKeyBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<u32x4*>(
@@ -347,6 +349,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   // Half b of tile t is 32 tokens. Where registers allow, operands are read from LDS half a step
   // before their products.
   constexpr bool kAhead = kHalves > 1;
+  constexpr int kKeysAhead = keys_ahead(kHalves), kValuesAhead = values_ahead(kHalves);
   u32x4 key[kSteps];
   auto read_keys = [&](int buffer, int b) __attribute__((always_inline)) {
     const char* from = lds + buffer * S::kKeyBytes + (32 * b + column) * S::kKeyPitch + 16 * half;
@@ -441,7 +444,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     // The lane's row of four and its 8 bytes of the 64 that two groups of 16 lanes read: piece
     // 2 * (lane / 16 % 2) + lane % 4 / 2. Tokens of other fours keep its place in the row.
     const int row = 4 * half + lane % 16 / 4, piece = 2 * (lane / 16 % 2) + lane % 4 / 2;
-    const char* at = lds + (kValues + (t & 1) * S::kValueBytes + 32 * b * S::kValuePitch) +
+    const char* at = lds + (kValues + int(uint32_t(t) % kValueBuffers) * S::kValueBytes + 32 * b * S::kValuePitch) +
                      lane % 2 * 8 + S::value_at(row, m, piece) + 16 * c * S::kValuePitch;
     const u32x2 x = lds_read_transposed(at);
     const u32x2 y = lds_read_transposed(at + 8 * S::kValuePitch);
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     for (int token = 0; token < kTokens; ++token)
 #pragma unroll
       for (int m = 0; m < kChannels; ++m)
-        if (poison[t % 3][token][m]) {
+        if (poison[t % kPoisonBuffers][token][m]) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
             if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n])
@@ -507,6 +510,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   };
   if (t_begin < t_end) {
     // In a tile's step the keys of the next tile but one are staged, and the values of the next.
+    static_assert(kKeysStaged == 2 && kValuesStaged == 1);
     store_tiles(staged, 0, t_begin);
     load_codes(staged, pages, t_begin + 2, t_begin + 1);
     load_pages(pages, t_begin + 3, t_begin + 2);
@@ -539,12 +543,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         multiply(scores);
       else
         stream_scores(buffer[1]);
-      if (kAhead) read_keys(buffer[(b + 2) / kHalves], (b + 2) % kHalves);
+      if (kAhead) read_keys(buffer[(b + kKeysAhead) / kHalves], (b + kKeysAhead) % kHalves);
       if (kAhead)
         add_values();
       else
         stream_values(t);
-      if (kAhead) read_values(t + (b + 1) / kHalves, (b + 1) % kHalves);
+      if (kAhead) read_values(t + (b + kValuesAhead) / kHalves, (b + kValuesAhead) % kHalves);
       scale(scores);
       if (b == 0) {
         load_codes(staged, pages, t + 3, t + 2);
@@ -564,11 +568,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (b + 1 == kHalves && edge_tile(t) && poisoned[t % 3] == t) add_poison(t);
-      // One barrier a tile. Before it, what the first half of step t stores was last read in step
-      // t - 1's first half or before; it is read from step t's second half on (with one half, from
-      // step t + 1 on).
-      if (b == 0) {
+      if (b + 1 == kHalves && edge_tile(t) && poisoned[t % kPoisonBuffers] == t) add_poison(t);
+      // One barrier a tile, where it parts what is stored from what is read (prompt_schedule.h): with
+      // one or two halves at the end of the first, with four of the third.
+      if (b == barrier_half(kHalves)) {
         __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
