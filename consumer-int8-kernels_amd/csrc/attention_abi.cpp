@@ -368,7 +368,8 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
   args.tokens = int(tokens);
   args.group = int(q->heads / cache->heads);
   args.max_q = int(max_q < tokens ? max_q : tokens);
-  args.window = int(window < INT_MAX ? window : 0);
+  // As many tokens as a page table holds are all; differences and sums with fewer stay in 32 bits.
+  args.window = int(window < table_width * cache->page_size ? window : 0);
   return abi_launched(ci8::launch_attention_fp4(args, int(dim), as_stream(stream)));
 }
 

@@ -65,7 +65,8 @@ struct AttentionArgs {
   // ones become 0), and the sign bits of a BF16 pair where scale is negative.
   float scale_log2;
   uint32_t q_sign;
-  int table_width, seqs, tokens, group, max_q, window;
+  int table_width, seqs, tokens, group, max_q;
+  int window;  // 0, or less than the tokens of a page table
 };
 // Sequences of at most `most` rows, and those of more than `few`.
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,

@@ -699,7 +699,7 @@ constexpr int whole_tiles(int dim, bool few) { return !few ? 64 : dim == 256 ? 3
 template <int D, int kTiles>
 hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream) {
   const int64_t longest = (int64_t(args.table_width) << args.cache.page_shift) / kTokens;
-  const int64_t span = args.window ? (args.window + args.max_q) / kTokens + 2 : longest;
+  const int64_t span = args.window ? (int64_t(args.window) + args.max_q) / kTokens + 2 : longest;
   const int64_t rows = int64_t(args.max_q) * args.group;
   const int blocks = int(((rows < most ? rows : most) + 16 * kTiles - 1) / (16 * kTiles));
   const int64_t contexts = int64_t(args.seqs) * args.cache.heads * blocks;
