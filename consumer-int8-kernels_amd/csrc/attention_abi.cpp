@@ -8,6 +8,7 @@
 
 #include "abi_checks.h"
 #include "attention_launch.h"
+#include "attention_plan.h"
 
 namespace {
 
@@ -199,11 +200,12 @@ int check_tokens(int64_t tokens, int64_t dim) {
   return CI8_OK;
 }
 
-// Workgroups of the norm kernels stay within a launch's 2^31 - 1.
-int check_work(int64_t tokens, int64_t heads, int64_t dim) {
-  if (i128(tokens) * (heads + 16) * dim > (i128(1) << 40))
-    return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
-  return CI8_OK;
+// Whether the norm kernels' work-items are few enough for one launch.
+int check_norm_launch(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim, bool append) {
+  const ci8::NormRopeGrid grid =
+      ci8::norm_rope_grid(tokens, int(q_heads), int(k_heads), int(dim), append);
+  if (ci8::launch_fits(grid.workgroups, ci8::kNormThreads)) return CI8_OK;
+  return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
 }
 
 }  // namespace
@@ -220,7 +222,7 @@ int ci8_qk_norm_rope(const ci8_heads* q, const ci8_heads* k, const ci8_heads* q_
   if (int s = check_rotation(rotation, tokens, dim)) return s;
   if (int s = check_output(q_out, *q, *norm, *rotation, tokens, dim)) return s;
   if (int s = check_output(k_out, *k, *norm, *rotation, tokens, dim)) return s;
-  if (int s = check_work(tokens, q->heads + k->heads, dim)) return s;
+  if (int s = check_norm_launch(tokens, q->heads, k->heads, dim, false)) return s;
   if (share(*q_out, *k, tokens, dim) || share(*k_out, *q, tokens, dim) ||
       share(*q_out, *k_out, tokens, dim))
     return abi_fail(CI8_ERR_OVERLAP, "An output must be its input or overlap no input");
@@ -275,7 +277,7 @@ int ci8_append_fp4(const ci8_heads* q, const ci8_heads* k, const ci8_heads* v,
     args.q = view(*q);
     args.q_out = view(*q_out);
   }
-  if (int s = check_work(tokens, (q ? q->heads : 0) + 2 * k->heads, dim)) return s;
+  if (int s = check_norm_launch(tokens, q ? q->heads : 0, k->heads, dim, true)) return s;
   args.k = view(*k);
   args.v = view(*v);
   args.q_weight = norm->q_weight;
@@ -295,7 +297,9 @@ int ci8_unpack_fp4(const ci8_fp4_cache* cache, const int64_t* slots, void* k, vo
   if (int s = check_cache(cache, dim, e)) return s;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8))
     return abi_fail(CI8_ERR_ALIGNMENT, "unpack_fp4 requires aligned buffers");
-  if (int s = check_work(count, cache->heads, dim)) return s;
+  if (!ci8::launch_fits(ci8::unpack_workgroups(count, int(cache->heads), int(dim)),
+                        ci8::kUnpackThreads))
+    return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
   const int64_t bytes = count * cache->heads * dim * 2;
   if (overlap(k, bytes, v, bytes) || overlap(k, bytes, slots, count * 8) ||
       overlap(v, bytes, slots, count * 8) || shares_cache(*cache, e, k, bytes) ||

@@ -15,6 +15,7 @@
 // heads of 256 at 4.3 TB/s, 9261 of 16 + 16 of 64 with three axes at 3.6 TB/s, where a large copy
 // reaches 5.0; one token of 32 + 8 heads of 128 3 us in the kernel.
 #include "attention_launch.h"
+#include "attention_plan.h"
 #include "fp4_device.h"
 
 #pragma clang fp contract(off)
@@ -227,8 +228,8 @@ __device__ __forceinline__ void store_fp4(const float (&x)[8], const Fp4Rows& ro
 // A wave takes kGroups groups of 512 / D heads of one token; a group is of queries, of keys or
 // of values alone. All loads of the wave come first.
 template <int D, bool kAppend, int kGroups>
-__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs p, int q_groups,
-                                                        int k_groups, int groups, int chunks) {
+__global__ void __launch_bounds__(kNormThreads)
+    norm_rope_kernel(const NormRopeArgs p, int q_groups, int k_groups, int groups, int chunks) {
   constexpr int kLanes = D / 8, kHeads = 64 / kLanes;
   const int lane = threadIdx.x & 63, channel = lane % kLanes * 8;
   const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -293,39 +294,24 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs p, in
 
 template <int D>
 hipError_t launch_dim(const NormRopeArgs& args, bool append, hipStream_t stream) {
-  constexpr int kHeads = 512 / D;
-  const int q_groups = (args.q.heads + kHeads - 1) / kHeads;
-  const int k_groups = (args.k.heads + kHeads - 1) / kHeads;
-  const int groups = q_groups + k_groups * (append ? 2 : 1);
-  auto launch = [&](auto kernel, int per_wave) {
-    const int chunks = (groups + per_wave - 1) / per_wave;
-    const int64_t waves = int64_t(args.tokens) * chunks;
-    kernel<<<uint32_t((waves + 3) / 4), 256, 0, stream>>>(args, q_groups, k_groups, groups,
-                                                          chunks);
+  const NormRopeGrid grid = norm_rope_grid(args.tokens, args.q.heads, args.k.heads, D, append);
+  auto launch = [&](auto kernel) {
+    kernel<<<uint32_t(grid.workgroups), kNormThreads, 0, stream>>>(args, grid.q_groups, grid.k_groups,
+                                                                   grid.groups, grid.chunks);
   };
-  // Four groups a wave, which share its angles, once waves are many. Microseconds with four and
-  // with one: 4096 tokens of 24 + 4 heads of 256 28.2 and 31.8, 9261 of 16 + 16 of 64 with three
-  // axes 23.4 and 51.2; but 1024 of 32 + 8 of 128 8.6 and 8.3, 64 of them 5.3 and 3.0.
-  if (int64_t(args.tokens) * groups >= 32768) {
-    if (append)
-      launch(norm_rope_kernel<D, true, 4>, 4);
-    else
-      launch(norm_rope_kernel<D, false, 4>, 4);
-  } else if (append) {
-    launch(norm_rope_kernel<D, true, 1>, 1);
-  } else {
-    launch(norm_rope_kernel<D, false, 1>, 1);
-  }
+  if (grid.per_wave == 4)
+    launch(append ? norm_rope_kernel<D, true, 4> : norm_rope_kernel<D, false, 4>);
+  else
+    launch(append ? norm_rope_kernel<D, true, 1> : norm_rope_kernel<D, false, 1>);
   return hipGetLastError();
 }
 
 // One lane for 8 channels of a row, keys and values both.
 template <int D>
-__global__ void __launch_bounds__(256) unpack_fp4_kernel(const Fp4CacheView cache,
-                                                         const int64_t* __restrict__ slots,
-                                                         uint16_t* __restrict__ k,
-                                                         uint16_t* __restrict__ v, int64_t packs) {
-  const int64_t index = int64_t(blockIdx.x) * 256 + threadIdx.x;
+__global__ void __launch_bounds__(kUnpackThreads)
+    unpack_fp4_kernel(const Fp4CacheView cache, const int64_t* __restrict__ slots,
+                      uint16_t* __restrict__ k, uint16_t* __restrict__ v, int64_t packs) {
+  const int64_t index = int64_t(blockIdx.x) * kUnpackThreads + threadIdx.x;
   if (index >= packs) return;
   const int channel = int(index % (D / 8)) * 8;
   const int64_t rows = index / (D / 8);
@@ -368,7 +354,8 @@ hipError_t launch_unpack_fp4(const Fp4CacheView& cache, const int64_t* slots, ui
   const auto kernel = dim == 64    ? unpack_fp4_kernel<64>
                       : dim == 128 ? unpack_fp4_kernel<128>
                                    : unpack_fp4_kernel<256>;
-  kernel<<<uint32_t((packs + 255) / 256), 256, 0, stream>>>(cache, slots, k, v, packs);
+  kernel<<<uint32_t(unpack_workgroups(count, cache.heads, dim)), kUnpackThreads, 0, stream>>>(
+      cache, slots, k, v, packs);
   return hipGetLastError();
 }
 
