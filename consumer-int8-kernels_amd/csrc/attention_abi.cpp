@@ -372,6 +372,12 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
   args.tokens = int(tokens);
   args.group = int(q->heads / cache->heads);
   args.max_q = int(max_q < tokens ? max_q : tokens);
+  // A workgroup a unit, and one more for each of up to 256 CUs.
+  if (ci8::row_split(tokens, seqs, args.group, args.max_q).prompt &&
+      !ci8::launch_fits(
+          ci8::prompt_units(tokens, seqs, args.group, args.max_q, args.cache.heads) + 256,
+          ci8::kPromptThreads))
+    return abi_fail(CI8_ERR_TOO_LARGE, "Too many sequences");
   // As many tokens as a page table holds are all; differences and sums with fewer stay in 32 bits.
   args.window = int(window < table_width * cache->page_size ? window : 0);
   return abi_launched(ci8::launch_attention_fp4(args, int(dim), as_stream(stream)));

@@ -38,4 +38,36 @@ inline int64_t unpack_workgroups(int64_t count, int heads, int dim) {
   return (count * heads * (dim / 8) + kUnpackThreads - 1) / kUnpackThreads;
 }
 
+// attention_fp4: rows are (token, query head of one key head) pairs. Sequences of at most `few` rows go
+// to the split kernel, the others to the prompt kernel.
+//
+// Up to kMostRows they are few: above 32 in blocks that each read the cache, which the caches between
+// them and HBM mostly hold. With the prompt kernel's 256 rows a workgroup instead, us: 16 x 5 tokens
+// behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 216, 16 tokens each 147 and
+// 223, 32 tokens (256 rows) behind 30000 142 and 123; 4 x 32 tokens (192 rows) of 24 and 4 of 256 67
+// and 85; 16 x 100 rows of 16 heads of 64 200 and 269, 2 x 200 66 and 49.
+constexpr int kMostRows = 128;
+struct RowSplit {
+  int few;
+  bool split, prompt;  // which kernels may have sequences
+};
+inline RowSplit row_split(int64_t tokens, int64_t seqs, int group, int64_t max_q) {
+  // Beside prompts `few` is 16 or 32, so that the usual decode fits.
+  const int64_t most = max_q * group;
+  int few = most <= kMostRows ? int(most) : group <= 16 ? 16 : 32;
+  // No sequence can be that short where all others at their longest leave more than that: then
+  // the prompt kernel has them all.
+  if (most > few && (tokens - (seqs - 1) * max_q) * group > few) few = 0;
+  return {few, group <= few, most > few};
+}
+
+// Units of the prompt kernel's work at most: its row tiles (each but a sequence's last is full) for
+// each key head. The kernel has as many workgroups, and one more a CU where contexts may be cut.
+constexpr int kPromptRows = 256, kPromptThreads = 512;
+inline int64_t prompt_units(int64_t tokens, int64_t seqs, int group, int64_t max_q, int heads) {
+  const int64_t each = (max_q * group + kPromptRows - 1) / kPromptRows;
+  const int64_t bound = tokens * group / kPromptRows + seqs;
+  return (bound < each * seqs ? bound : each * seqs) * heads;
+}
+
 }  // namespace ci8

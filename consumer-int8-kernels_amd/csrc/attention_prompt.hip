@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "attention_device.h"
+#include "attention_plan.h"
 #include "launch.h"
 #include "prompt_schedule.h"
 
@@ -32,6 +33,7 @@ struct Shape {
   static constexpr int kWaves = 8;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kRows = 32 * kTiles * kWaves;
+  static_assert(kRows == kPromptRows && kThreads == kPromptThreads);
   static constexpr int kTokens = D == 64 ? 128 : D == 128 ? 64 : 32;
   static constexpr int kBlocks = D / kFp4Block;
   // Byte pitch of LDS rows of keys: 16 of them, 16 bytes each, fall on different banks. Rows of
@@ -669,10 +671,8 @@ hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream)
   using S = Shape<D>;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
   static_assert(256 * S::kRows <= kAttentionWorkspaceRows, "one part a CU");
-  // Row tiles of all sequences, at most: each but its last is full.
-  const int64_t each = (int64_t(args.max_q) * args.group + S::kRows - 1) / S::kRows;
-  const int64_t bound = int64_t(args.tokens) * args.group / S::kRows + args.seqs;
-  const int64_t units = (bound < each * args.seqs ? bound : each * args.seqs) * args.cache.heads;
+  const int64_t units =
+      prompt_units(args.tokens, args.seqs, args.group, args.max_q, args.cache.heads);
   // Cut into parts of four tiles or more. After many rounds the last one counts for little, and
   // the last units of prompts without a context before them are short by themselves.
   const int64_t longest = int64_t(args.table_width) << args.cache.page_shift;

@@ -31,6 +31,7 @@
 // TB/s with the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
 // the launch.
 #include "attention_device.h"
+#include "attention_plan.h"
 #include "launch.h"
 
 namespace ci8 {
@@ -559,8 +560,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     }
     if (kSplit && place.at == 0 && (by_context || !whole) && threadIdx.x == 0) {
       const int64_t last = at + place.cost - 1;
-      const int context = (seq * p.cache.heads + kv_head) * most_blocks + place.block;
-      joints<D>(p)[by_context ? context : int(blockIdx.x)] = {
+      joints<D>(p)[by_context ? (seq * p.cache.heads + kv_head) * most_blocks + place.block
+                              : int(blockIdx.x)] = {
           whole ? 0 : int(last / run.quota) - int(blockIdx.x) + 1, int(blockIdx.x), s.q_begin,
           row0, rows, kv_head};
     }
@@ -704,12 +705,14 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   const int blocks = int(((rows < most ? rows : most) + 16 * kTiles - 1) / (16 * kTiles));
   const int64_t contexts = int64_t(args.seqs) * args.cache.heads * blocks;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
-  if ((longest < span ? longest : span) <= whole_tiles(D, 4 * contexts <= cus)) {
-    // Eight waves: 517 tokens of 8 key heads of 128 7.6 us, with four 8.3; 4 rows a sequence of 6
-    // heads of 256, 64 contexts up to 1500, 25.5 and 32.4.
-    constexpr int kWaves = 8;
-    attention_split_kernel<D, kTiles, kWaves, false>
-        <<<uint32_t(contexts), 64 * kWaves, 0, stream>>>(args, most, blocks, 0, false, false);
+  // Eight waves: 517 tokens of 8 key heads of 128 7.6 us, with four 8.3; 4 rows a sequence of 6
+  // heads of 256, 64 contexts up to 1500, 25.5 and 32.4. Contexts past a launch's limit are split,
+  // which takes any number.
+  constexpr int kWholeWaves = 8;
+  if ((longest < span ? longest : span) <= whole_tiles(D, 4 * contexts <= cus) &&
+      launch_fits(contexts, 64 * kWholeWaves)) {
+    attention_split_kernel<D, kTiles, kWholeWaves, false>
+        <<<uint32_t(contexts), 64 * kWholeWaves, 0, stream>>>(args, most, blocks, 0, false, false);
     return hipGetLastError();
   }
   // Four waves a workgroup; each pair of times was taken in turn, before runs counted beginnings: 32
@@ -743,13 +746,6 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
 
 }  // namespace
 
-// Up to this many rows a sequence are few: above 32 in blocks that each read the cache, which the
-// caches between them and HBM mostly hold. With the prompt kernel's 256 rows a workgroup instead,
-// us: 16 x 5 tokens behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 216, 16
-// tokens each 147 and 223, 32 tokens (256 rows) behind 30000 142 and 123; 4 x 32 tokens (192 rows) of
-// 24 and 4 of 256 67 and 85; 16 x 100 rows of 16 heads of 64 200 and 269, 2 x 200 66 and 49.
-constexpr int kMostRows = 128;
-
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream) {
   if (most <= 16) {
@@ -768,18 +764,12 @@ hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  // Sequences of at most `few` rows go to the split kernel, the others to the prompt kernel. Beside
-  // prompts `few` is 16 or 32, so that the usual decode fits.
-  const int64_t most = int64_t(args.max_q) * args.group;
-  int few = most <= kMostRows ? int(most) : args.group <= 16 ? 16 : 32;
-  // No sequence can be that short where all others at their longest leave more than that: then
-  // the prompt kernel has them all.
-  if (most > few && (args.tokens - int64_t(args.seqs - 1) * args.max_q) * args.group > few) few = 0;
-  if (args.group <= few) {
-    if (const hipError_t e = launch_attention_split(args, dim, few, stream); e != hipSuccess)
+  const RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
+  if (rows.split) {
+    if (const hipError_t e = launch_attention_split(args, dim, rows.few, stream); e != hipSuccess)
       return e;
   }
-  return most > few ? launch_attention_prompt(args, dim, few, stream) : hipSuccess;
+  return rows.prompt ? launch_attention_prompt(args, dim, rows.few, stream) : hipSuccess;
 }
 
 }  // namespace ci8

@@ -22,9 +22,14 @@ int main(int argc, char** argv) {
   long long v[8] = {};
   for (int i = 1; i < argc;) {
     const char* what = argv[i++];
-    const int n = !std::strcmp(what, "norm") ? 5 : 3;
+    const bool attend = !std::strcmp(what, "attend");
+    const int n = attend || !std::strcmp(what, "norm") ? 5 : 3;
     for (int j = 0; j < n; ++j) v[j] = std::atoll(argv[i++]);
-    if (n == 5) {
+    if (attend) {
+      const RowSplit r = row_split(v[0], v[1], int(v[2]), v[3]);
+      const int64_t units = prompt_units(v[0], v[1], int(v[2]), v[3], int(v[4]));
+      std::printf("%d %d %d %lld\n", r.few, int(r.split), int(r.prompt), (long long)units);
+    } else if (n == 5) {
       const NormRopeGrid g = norm_rope_grid(v[0], int(v[1]), int(v[2]), int(v[3]), v[4] != 0);
       std::printf("%lld %d %d\n", (long long)g.workgroups, g.per_wave, int(launch_fits(g.workgroups, kNormThreads)));
     } else {
@@ -75,6 +80,26 @@ def test_norm_and_unpack_grids(plan):
     assert [g[2] for g in got] == [int(n * 256 <= MOST_ITEMS) for n, _ in want]
 
 
+def test_kernels_and_units_of_attention(plan):
+    """Tokens, sequences, query heads of a key head, longest, key heads."""
+    cases = [
+        ("attend", 64, 64, 4, 1, 8),          # decodes: up to 4 rows, one kernel
+        ("attend", 64, 2, 4, 32, 8),          # 128 rows: still that one
+        ("attend", 4096, 1, 5, 4096, 8),      # a prompt alone: the other, 80 full row tiles
+        ("attend", 4100, 5, 5, 4096, 8),      # beside decodes: both
+        ("attend", 300, 1, 48, 300, 2),       # 57 row tiles, the last of 64 rows
+        ("attend", 301, 2, 48, 300, 2),       # 48 rows at least: too many for the first kernel
+        ("attend", 65535, 65535, 1, 1, 65535),
+        ("attend", 65535 * 33, 65535, 4, 33, 128),   # a row tile a sequence and head: 2^23 - 128 units
+    ]
+    want = [(4, 1, 0, 64 * 8), (128, 1, 0, 2 * 8), (0, 0, 1, 640), (16, 1, 1, 8 * 85), (0, 0, 1, 114), (0, 0, 1, 116),
+            (1, 1, 0, (65535 * 65535 // 256 + 65535) * 65535), (16, 1, 1, 65535 * 128)]
+    got = plan(*cases)
+    assert [g[:3] for g in got] == [w[:3] for w in want]
+    # units: never fewer than a count of the tiles
+    assert [g[3] for g in got[:6]] == [w[3] for w in want[:6]] and got[7][3] == want[7][3]
+
+
 def test_calls_that_no_launch_holds_are_refused(lib):
     """Each is past the limit by a little; nothing is launched."""
     from consumer_int8 import _abi as A
@@ -100,3 +125,20 @@ def test_calls_that_no_launch_holds_are_refused(lib):
         setattr(cache, name + "_scale_page_stride", 16 * 16 * 4)
     refused(lib, lib.ci8_unpack_fp4(ref(cache), 11 << 42, 12 << 42, 13 << 42, tokens, 128, None),
             large, "Too many tokens")
+
+
+def test_attention_that_no_launch_holds_is_refused(lib):
+    """Prompts of 65535 sequences and 128 key heads: 2^23 - 128 workgroups of 512, and one a CU."""
+    from consumer_int8 import _abi as A
+
+    geometry, alignment, overlap, large = codes()
+    ref = ctypes.byref
+    page = 128 * 16 * 64
+    cache = A.Fp4CacheView(3 << 42, 4 << 42, 5 << 42, 6 << 42, page, page // 16, page, page // 16, 8, 128, 16)
+    for seqs, count, group, status, text in [(65535, 33, 4, large, "Too many sequences"),
+                                             (65535, 33, 5, geometry, "a multiple")]:
+        q = A.Heads(1 << 42, 512, 512 * 128, 128)
+        if group == 5:
+            q.heads = 513
+        refused(lib, lib.ci8_attention_fp4(ref(q), ref(cache), 7 << 42, 4, 8 << 42, 9 << 42, seqs, 1 << 21, 128,
+                                           10 << 42, 11 << 42, None, 0.1, count, 0, None), status, text)
