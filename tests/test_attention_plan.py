@@ -93,7 +93,7 @@ def test_kernels_and_units_of_attention(plan):
         ("attend", 65535 * 33, 65535, 4, 33, 128),   # a row tile a sequence and head: 2^23 - 128 units
     ]
     want = [(4, 1, 0, 64 * 8), (128, 1, 0, 2 * 8), (0, 0, 1, 640), (16, 1, 1, 8 * 85), (0, 0, 1, 114), (0, 0, 1, 116),
-            (1, 1, 0, (65535 * 65535 // 256 + 65535) * 65535), (16, 1, 1, 65535 * 128)]
+            (1, 1, 0, (65535 * 65535 // 256 + 65535) * 65535), (0, 0, 1, 65535 * 128)]
     got = plan(*cases)
     assert [g[:3] for g in got] == [w[:3] for w in want]
     # units: never fewer than a count of the tiles
