@@ -108,10 +108,11 @@ __device__ __forceinline__ Angles load_angles(const RotationView& r, int64_t at,
         }
       }
     }
-    if (!inside) {
+    // NaN for a position outside the table, and for pairs that name an axis that there is not.
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.cos[j] = __builtin_nanf("");
-    }
+    for (int j = 0; j < 8; ++j)
+      if (!inside || (r.axis_of && r.axis_of[first + (r.interleaved ? j / 2 : j)] != 0))
+        a.cos[j] = __builtin_nanf("");
     return a;
   }
   // Rows of the table for up to four axes, the same in all lanes; -1 outside it.

@@ -4,8 +4,10 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_attention import (attention, bf16_randn, check_attention, random_cache,  # noqa: F401
-                                      run_attention, say, tables)
+from oracle import attention as OA
+from tests.helpers import host
+from tests.test_gpu_attention import (attention, bf16_randn, check_attention, dev, f64, random_cache,  # noqa: F401
+                                      rope_inputs, run_attention, say, tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +36,35 @@ def test_windows_past_the_page_table_hide_nothing(attention, dim, hq, hk, lens, 
     for window in (holds - 1, max(lens) - 1):
         out, lse = run_attention(attention, q, cache, table, lens, starts, 0.09, max(counts), window)
         check_attention(q, cache, table, lens, starts, 0.09, max(counts), window, out, lse)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens", [3, 9000])
+def test_pairs_of_an_axis_that_there_is_not_are_nan(attention, tokens, interleaved):  # noqa: F811
+    """One axis, whose positions may be [T] or [1, T], and pairs that name axes 0, 1 and -1."""
+    rng = np.random.default_rng(tokens)
+    dim, rot, hq, hk = 64, 48, 2, 2
+    table, at, _ = rope_inputs(rng, 50, rot, tokens, 1)
+    of = np.zeros(rot // 2, dtype=np.int32)
+    q, k = bf16_randn(rng, tokens, hq, dim).cuda(), bf16_randn(rng, tokens, hk, dim).cuda()
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    attention.qk_norm_rope(q, k, None, None, dev(table), dev(at), None, q_out, k_out, 1e-6, interleaved)
+    plain = q_out.clone(), k_out.clone()
+    attention.qk_norm_rope(q, k, None, None, dev(table), dev(at[0]), dev(of), q_out, k_out, 1e-6, interleaved)
+    assert torch.equal(q_out, plain[0]) and torch.equal(k_out, plain[1])
+    of[3], of[10], of[23] = 1, -1, 2**31 - 1
+    attention.qk_norm_rope(q, k, None, None, dev(table), dev(at), dev(of), q_out, k_out, 1e-6, interleaved)
+    for x, got in ((q, q_out), (k, k_out)):
+        y, size = OA.norm_rope64(f64(x), None, 0, table, rot, at, of, interleaved)
+        nan = np.isnan(y)
+        assert nan.sum() == tokens * 2 * 6 and np.array_equal(np.isnan(f64(got)), nan)
+        assert np.all((np.abs(f64(got) - y) <= OA.norm_rope_bound(y, size, dim))[~nan])
+    # appended, such a pair makes its blocks NaN
+    cache = attention.new_cache(tokens // 16 + 1, hk, 16, dim)
+    slots = torch.arange(tokens, device="cuda")
+    attention.append_fp4(None, k, k, None, None, dev(table), dev(at), dev(of), slots, None, *cache, 1e-6, interleaved)
+    with np.errstate(invalid="ignore"):
+        codes, scales = OA.fp4_quantize(OA.norm_rope32(host(k.float()), None, 0, table, rot, at, of, interleaved))
+    k_back, v_back = torch.empty_like(k), torch.empty_like(k)
+    attention.unpack_fp4(*cache, slots, k_back, v_back)
+    assert np.array_equal(f64(k_back), OA.fp4_values(codes, scales), equal_nan=True) and (scales == 255).any()
