@@ -59,9 +59,19 @@ bool same(const ci8_heads& a, const ci8_heads& b) {
          a.head_stride == b.head_stride;
 }
 
-// Whether two views share elements: exact for rows of one buffer, and else by their extents.
+// Whether two views share elements: exact for rows of one buffer, and for heads that take turns in
+// it ([tokens, heads, 3, dim]); else by their extents.
 bool share(const ci8_heads& a, const ci8_heads& b, int64_t tokens, int64_t dim) {
   if (!overlap(a.data, extent(a, tokens, dim), b.data, extent(b, tokens, dim))) return false;
+  if (a.head_stride == b.head_stride && a.head_stride > 0 &&
+      (tokens == 1 ||
+       (a.token_stride % a.head_stride == 0 && b.token_stride % b.head_stride == 0))) {
+    // All heads of one view begin the same number of bytes into a stride.
+    const int64_t turn = a.head_stride * 2;
+    const int64_t apart = reinterpret_cast<intptr_t>(b.data) - reinterpret_cast<intptr_t>(a.data);
+    const int64_t shift = ((apart % turn) + turn) % turn;
+    if (shift >= dim * 2 && shift + dim * 2 <= turn) return false;
+  }
   const int64_t stride = a.token_stride * 2;
   if (a.token_stride != b.token_stride || stride == 0) return true;
   const int64_t row_a = ((a.heads - 1) * a.head_stride + dim) * 2;

@@ -142,3 +142,21 @@ def test_attention_that_no_launch_holds_is_refused(lib):
             q.heads = 513
         refused(lib, lib.ci8_attention_fp4(ref(q), ref(cache), 7 << 42, 4, 8 << 42, 9 << 42, seqs, 1 << 21, 128,
                                            10 << 42, 11 << 42, None, 0.1, count, 0, None), status, text)
+
+
+def test_heads_that_take_turns_and_touch_are_refused(lib):
+    """Heads of [tokens, heads, 3, dim] half a head on, a token and half a head on, or of other strides."""
+    from consumer_int8 import _abi as A
+
+    *_, overlap, _large = codes()
+    ref, base, dim = ctypes.byref, 1 << 40, 128
+
+    def view(at, n=4, step=3 * dim, row=None):
+        return A.Heads(base + 2 * at, n, n * step if row is None else row, step)
+
+    q = view(0)
+    for k in [view(dim // 2), view(3 * dim - 64), view(12 * dim + 64), view(15 * dim), view(dim, 4, 2 * dim, 12 * dim),
+              view(dim, 3, 3 * dim, 12 * dim + 8)]:
+        r = rotation(table=9 << 42, positions=10 << 42)
+        refused(lib, lib.ci8_qk_norm_rope(ref(q), ref(k), ref(q), ref(k), ref(norm()), ref(r), 8, dim, None), overlap,
+                "An output must be its input")

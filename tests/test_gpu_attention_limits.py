@@ -68,3 +68,27 @@ def test_pairs_of_an_axis_that_there_is_not_are_nan(attention, tokens, interleav
     k_back, v_back = torch.empty_like(k), torch.empty_like(k)
     attention.unpack_fp4(*cache, slots, k_back, v_back)
     assert np.array_equal(f64(k_back), OA.fp4_values(codes, scales), equal_nan=True) and (scales == 255).any()
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (5, 6), (600, 4)])
+def test_heads_that_take_turns_in_a_row(attention, tokens, heads):  # noqa: F811
+    """Projections laid out [tokens, heads, 3, dim]: views of one buffer that share no element, in place."""
+    rng = np.random.default_rng(tokens)
+    dim, rot = 64, 64
+    qkv = bf16_randn(rng, tokens, heads, 3, dim).cuda()
+    apart = [qkv[:, :, i].contiguous() for i in range(3)]
+    table, at, _ = rope_inputs(rng, 700, rot, tokens, 1)
+    w = dev(np.exp(0.5 * rng.standard_normal(dim)).astype(np.float32))
+    args = w, w, dev(table), dev(at[0]), None
+    want = [torch.empty_like(t) for t in apart[:2]]
+    attention.qk_norm_rope(*apart[:2], *args, *want)
+    cache, cache2 = (attention.new_cache(tokens // 16 + 1, heads, 16, dim) for _ in range(2))
+    slots = torch.arange(tokens, device="cuda")
+    attention.append_fp4(*apart, *args, slots, torch.empty_like(apart[0]), *cache)
+    q, k, v = qkv.unbind(2)
+    mixed = qkv.clone().unbind(2)
+    attention.append_fp4(*mixed, *args, slots, mixed[0], *cache2)
+    assert torch.equal(mixed[0], want[0]) and torch.equal(mixed[1], apart[1]) and torch.equal(mixed[2], apart[2])
+    assert all(torch.equal(a, b) for a, b in zip(cache, cache2))
+    attention.qk_norm_rope(q, k, *args, q, k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, apart[2])
