@@ -18,7 +18,8 @@ qk_norm_rope(q, k, q_weight, k_weight, rope, positions, axes, q_out, k_out, eps=
 append_fp4(q, k, v, q_weight, k_weight, rope, positions, axes, slots, q_out, k_codes,
            k_scales, v_codes, v_scales, eps=1e-6, interleaved=False)
     In one launch: keys, normed and rotated, and values into the cache rows that INT64 slots
-    [T] names (negative: skipped); queries as qk_norm_rope (q and q_out may both be None).
+    [T] names (negative: skipped; no two alike); queries as qk_norm_rope (q and q_out may both
+    be None).
 unpack_fp4(k_codes, k_scales, v_codes, v_scales, slots, k, v)
     Cache rows back as BF16 k, v [count, heads, D], exactly.
 attention_fp4(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens, q_starts,

@@ -24,8 +24,9 @@ inline NormRopeGrid norm_rope_grid(int64_t tokens, int q_heads, int k_heads, int
   g.k_groups = (k_heads + heads - 1) / heads;
   g.groups = g.q_groups + g.k_groups * (append ? 2 : 1);
   // Four groups a wave, which share its angles, once waves are many. Microseconds with four and
-  // with one: 4096 tokens of 24 + 4 heads of 256 28.2 and 31.8, 9261 of 16 + 16 of 64 with three
-  // axes 23.4 and 51.2; but 1024 of 32 + 8 of 128 8.6 and 8.3, 64 of them 5.3 and 3.0.
+  // with one, in a graph: 9261 tokens of 16 + 16 heads of 64 with three axes 20.3 and 35.2; with one axis
+  // little between them, 4096 of 24 + 4 of 256 24.1 and 23.9, of 32 + 8 of 128 20.4 and 18.7; but 300 of
+  // 40 + 8 of 128 5.7 and 4.1, 64 of 32 + 8 5.2 and 3.1.
   g.per_wave = tokens * g.groups >= 32768 ? 4 : 1;
   g.chunks = (g.groups + g.per_wave - 1) / g.per_wave;
   g.workgroups = (tokens * g.chunks + 3) / 4;
@@ -43,9 +44,10 @@ inline int64_t unpack_workgroups(int64_t count, int heads, int dim) {
 //
 // Up to kMostRows they are few: above 32 in blocks that each read the cache, which the caches between
 // them and HBM mostly hold. With the prompt kernel's 256 rows a workgroup instead, us: 16 x 5 tokens
-// behind contexts up to 16000 of 64 query and 8 key heads of 128 83 and 216, 16 tokens each 147 and
-// 223, 32 tokens (256 rows) behind 30000 142 and 123; 4 x 32 tokens (192 rows) of 24 and 4 of 256 67
-// and 85; 16 x 100 rows of 16 heads of 64 200 and 269, 2 x 200 66 and 49.
+// behind contexts up to 16000 of 64 query and 8 key heads of 128 79 and 214, 16 tokens each 145 and
+// 220; 16 x 100 rows of 16 heads of 64 199 and 268, 48 rows 109 and 267. Above, blocks and the prompt
+// kernel: 4 x 32 tokens (256 rows) behind up to 30000 133 and 122, 16 x 32 277 and 235, 2 x 200 rows at 64
+// channels 61 and 49; but 8 x 150 132 and 145, 4 x 32 tokens (192 rows) of 24 and 4 heads of 256 65 and 85.
 constexpr int kMostRows = 128;
 struct RowSplit {
   int few;

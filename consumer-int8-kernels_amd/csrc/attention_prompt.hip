@@ -6,11 +6,14 @@
 // weighted and become the operand of O^T += V^T P^T without an exchange. Rows are (token, query
 // head of one key head) pairs, 256 a workgroup, so that heads that share a key head share its
 // tiles. Four operations a score and channel: bound by the MFMA rate, then by the softmax's
-// vector instructions (about five a score) and by LDS reads (each wave reads every tile). Two waves a
+// vector instructions (by the counters 7.8 for each MFMA at 128 channels, which is each register of
+// scores; masks, staging and addresses counted) and by LDS reads (each wave reads every tile). Two waves a
 // SIMD of 32 rows each, in alternate phases: the scores of the next tile are on the matrix unit while
 // the vector unit weighs those of this one. Measured: 4096 tokens of 40 query and 8 key heads of 128
-// 192 us, 890 TFLOP/s of what the mask leaves (a large product reaches 1157 to 1265); 24 and 4 of
-// 256 241 us, 855 (415 us with one wave a SIMD that holds all its queries).
+// 192 us (199 on another card), 895 TFLOP/s of what the mask leaves (a large product reaches 1157 to
+// 1265); 24 and 4 of 256 242 us, 853 (415 us with one wave a SIMD that holds all its queries); 16 heads of
+// 64 81 us, 423, and 14 and 2 of 64 behind 8000 more 209 us, 687: half the MFMAs for as many scores.
+// Weights are rounded to BF16 for the second product as in attention_split.hip.
 //
 // Tiles of keys and values are converted to BF16 once a workgroup, on their way into LDS: global
 // loads run two tiles ahead, one barrier a tile.

@@ -17,6 +17,11 @@
 //                    loads it, stored to the wave's own LDS tile and read transposed
 //                    (ds_read_b64_tr_b16) with the tokens in that order.
 //
+// The weights are rounded to BF16 for the second product, since BF16 is what its MFMA takes (FP32 weights
+// would need a second BF16 product for what the first leaves, in a loop that runs close to HBM): 2^-8 of
+// each at most, averaged over the tokens. Their sum is of the FP32 weights. Outputs are 0.0019 to 0.0022
+// from 64 bits where FP32 weights give 0.0016 to 0.0017, most of it the outputs' own rounding.
+//
 // All statistics of a row sit in the lanes of its column. m moves only when a score passes it by
 // 2^8 in weight, so most tiles exchange nothing between lanes and rescale nothing.
 //
@@ -693,8 +698,10 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Up to this many tiles of the longest context a workgroup takes a whole context: fewer where contexts
-// leave most of the GPU idle. Whole and split, us: 16 contexts up to 2000 tokens of 8 heads of 128 14.4
-// and 15.8, 4 of them 13.5 and 11.5, one of 1100 9.6 and 11.3; 16 of 4 heads of 256 23.9 and 17.6.
+// leave most of the GPU idle. Whole and split, us: 16 contexts up to 2000 tokens of 8 heads of 128 14.3
+// and 15.3, 64 of them 22.1 and 29.4, 4 13.5 and 12.1, one of 1100 9.6 and 11.8; 16 of 4 heads of 256
+// 23.9 and 17.7. How long contexts are is known by the width of the page table alone here: a wide one of
+// short contexts is split.
 constexpr int whole_tiles(int dim, bool few) { return !few ? 64 : dim == 256 ? 32 : 48; }
 
 template <int D, int kTiles>
@@ -715,11 +722,12 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
         <<<uint32_t(contexts), 64 * kWholeWaves, 0, stream>>>(args, most, blocks, 0, false, false);
     return hipGetLastError();
   }
-  // Four waves a workgroup; each pair of times was taken in turn, before runs counted beginnings: 32
-  // contexts up to 8000 tokens of 8 heads of 128 42 us, with eight waves 59; 64 up to 32768 257 and
-  // 278. Where the queries are in LDS eight waves share them: 16 x 4 rows up to 16000 of 4 heads of 256
-  // 58 us, with four 67. At D = 256 contexts that are few get one workgroup a CU and so fewer parts to
-  // join: one of 131071 tokens of 4 heads 32.6 us, with two 34.9; 12 up to 9000 23.2 and 25.7.
+  // Four waves a workgroup; with eight, in one workgroup a CU (two at 64 channels), us in turn: 32 contexts
+  // up to 8000 tokens of 8 heads of 128 36.9 and 44.0, of 16 heads of 64 39.0 and 50.6; the longest would
+  // gain, 64 up to 32768 264 and 258. Where the queries are in LDS eight waves share them: 16 x 4 rows up to 16000
+  // of 4 heads of 256 51.4 us, with four 61.7. At D = 256 contexts that are few get one workgroup a CU and
+  // so fewer parts to join: one of 131071 tokens of 4 heads 32.8 us, with two 34.8; 12 up to 9000 24.6 and
+  // 25.6.
   constexpr int kWaves = D == 256 && kTiles == 2 ? 8 : 4;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(groups_per_cu(D, kTiles) <= 8 &&
@@ -735,8 +743,8 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   attention_split_kernel<D, kTiles, kWaves, true>
       <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context, apart);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  // More threads where a context has many parts: one of 131071 tokens of 4 heads, 64 parts each,
-  // is joined in 5.0 us, by 256 threads in 7.2; 32 contexts up to 8000, 4 parts, in 8.8 and 4.9.
+  // More threads where a context has many parts. Whole calls with 1024 and with 256, us: one of 131071
+  // tokens of 4 heads of 256, 64 parts each, 32.6 and 34.8; 32 up to 8000, 3 or 4 parts, 41.4 and 37.6.
   const bool many = groups > 16 * contexts;
   const auto join = many ? attention_join_kernel<D, kTiles, 1024> : attention_join_kernel<D, kTiles, 256>;
   join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : 256, 0,

@@ -93,8 +93,8 @@ int ci8_qk_norm_rope(const ci8_heads* q, const ci8_heads* k, const ci8_heads* q_
 
 /* append_fp4: keys, normed and rotated as above and not rounded on the way, and values are
  * quantized into the cache rows that slots INT64 [tokens] names; a slot outside the cache
- * (negative for a padding token) is skipped. Slots must differ: of tokens that share one,
- * any may be kept. Where q is not NULL the queries are normed and rotated into q_out as
+ * (negative for a padding token) is skipped. Slots must differ: a row that several tokens
+ * share may hold parts of each. Where q is not NULL the queries are normed and rotated into q_out as
  * ci8_qk_norm_rope does, in the same launch. */
 int ci8_append_fp4(const ci8_heads* q, const ci8_heads* k, const ci8_heads* v,
                    const ci8_heads* q_out, const ci8_head_norm* norm,
