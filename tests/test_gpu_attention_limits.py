@@ -92,3 +92,28 @@ def test_heads_that_take_turns_in_a_row(attention, tokens, heads):  # noqa: F811
     assert all(torch.equal(a, b) for a, b in zip(cache, cache2))
     attention.qk_norm_rope(q, k, *args, q, k)
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, apart[2])
+
+
+def test_more_contexts_than_a_launch_holds(attention):  # noqa: F811
+    """65535 sequences of 129 key heads, of no token or of one: 2^23 + 65407 contexts, which 512 threads
+    each would not fit. One token's output is its value, exactly."""
+    rng = np.random.default_rng(1)
+    seqs, heads, dim, page, pages, scale = 65535, 129, 64, 16, 40, 0.125
+    cache = random_cache(attention, rng, pages, heads, page, dim)
+    gen = torch.Generator("cuda").manual_seed(1)
+    q = torch.randn(seqs, heads, dim, device="cuda", generator=gen, dtype=torch.float32).bfloat16()
+    table = torch.randint(0, pages, (seqs, 1), device="cuda", generator=gen, dtype=torch.int32)
+    lens = torch.randint(0, 2, (seqs,), device="cuda", generator=gen, dtype=torch.int32)
+    out, lse = torch.full_like(q, 5.0), torch.full((seqs, heads), 5.0, device="cuda")
+    attention.attention_fp4(q, *cache, table, lens, None, attention.new_workspace(dim), out, lse, scale)
+    torch.cuda.synchronize()
+    k, v = (torch.empty(pages, heads, dim, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    attention.unpack_fp4(*cache, torch.arange(pages, device="cuda") * page, k, v)
+    for first in range(0, seqs, 4096):
+        part = slice(first, min(first + 4096, seqs))
+        at, one = table[part, 0].long(), lens[part].bool()
+        assert torch.equal(out[part], torch.where(one[:, None, None], v[at], 0))
+        assert (lse[part][~one] == -torch.inf).all()
+        terms = q[part].double() * k[at].double() * scale
+        score, off = terms.sum(-1), terms.abs().sum(-1) * (dim + 2) * 2.0**-24
+        assert ((lse[part].double() - score).abs() <= off + 2.0**-15 + score.abs() * 2.0**-21)[one].all()
