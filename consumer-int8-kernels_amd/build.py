@@ -2,7 +2,8 @@
 
 Outputs (next to the Python package, so they travel with the source tree):
   consumer_int8/libci8_amd.so   -- HIP kernels + the C ABI of include/consumer_int8_amd.h
-                                   and include/consumer_int8_attention.h
+                                   (include/consumer_int8_attention.h and
+                                   include/consumer_int8_drafts.h too)
   consumer_int8/_C.so           -- torch.ops.consumer_int8.* registration (stable ABI)
   consumer_int8/libci8_probe.so -- bench.py's MFMA-loop clock probe (not the drop-in)
 
@@ -34,8 +35,9 @@ ARCH = "gfx950"
 HIP_SOURCES = ["quantize.hip", "gemm.hip", "gemm_small.hip", "gemm_ring.hip", "gemm_pp.hip", "gemv.hip", "gemv_stream.hip", "silu.hip",
                "allspark.hip", "q8block.hip", "gguf_q8.hip", "gguf_ring.hip",
                "gemm_grouped.hip", "grouped_ring.hip", "noalloc.hip", "gemm_bytes.hip",
-               "norm_rope.hip", "attention_split.hip", "attention_prompt.hip"]
-HOST_SOURCES = ["abi.cpp", "attention_abi.cpp"]
+               "norm_rope.hip", "attention_split.hip", "attention_prompt.hip",
+               "move_fp4.hip", "sampling.hip"]
+HOST_SOURCES = ["abi.cpp", "attention_abi.cpp", "sampling_abi.cpp"]
 
 # -packed-fp32-ops: keep packed FP32 (v_pk_*_f32) out of the generated code.
 HIP_FLAGS = [
@@ -118,7 +120,8 @@ def build_torch_module() -> Path:
     _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
           "-DTORCH_STABLE_ONLY", "-DUSE_ROCM", "-DTORCH_TARGET_VERSION=0x020A000000000000",
           f"-I{torch_dir / 'include'}", f"-I{py_include}", f"-I{INCLUDE}",
-          str(CSRC / "torch_ops.cpp"), str(CSRC / "attention_ops.cpp"), "-o", str(tmp),
+          str(CSRC / "torch_ops.cpp"), str(CSRC / "attention_ops.cpp"),
+          str(CSRC / "sampling_ops.cpp"), "-o", str(tmp),
           f"-L{OUT_DIR}", "-lci8_amd", "-Wl,-rpath,$ORIGIN",
           f"-L{torch_dir / 'lib'}", "-ltorch_hip", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{torch_dir / 'lib'}"])
     os.replace(tmp, target)

@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in include/consumer_int8_amd.h and
-include/consumer_int8_attention.h (libci8_amd.so).
+"""ctypes binding of the C ABI in include/consumer_int8_amd.h, include/consumer_int8_attention.h
+and include/consumer_int8_drafts.h (libci8_amd.so).
 
 This is the binding an FFI caller would write; the torch ops do not use it (they call
 the same entry points from C++). Tests use it to reach the C ABI directly.
@@ -80,6 +80,16 @@ ATTENTION_SIGNATURES = {
                            ctypes.c_double, _i64, _i64, _p], ctypes.c_int),
 }
 
+# include/consumer_int8_drafts.h
+DRAFTS_SIGNATURES = {
+    "ci8_attention_fp4_tree": ([_heads, _cache, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p,
+                                ctypes.c_double, _i64, _i64, _p], ctypes.c_int),
+    "ci8_move_fp4": ([_cache, _p, _p, _p, _i64, _i64, _i64, _p], ctypes.c_int),
+    "ci8_token_probs": ([_p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p], ctypes.c_int),
+    "ci8_verify_drafts": ([_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
+                          ctypes.c_int),
+}
+
 _lib = None
 
 
@@ -87,7 +97,8 @@ def load(path: Path | str = LIB_PATH) -> ctypes.CDLL:
     global _lib
     if _lib is None:
         lib = ctypes.CDLL(str(path))
-        for name, (args, res) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
+        for name, (args, res) in {**SIGNATURES, **ATTENTION_SIGNATURES,
+                                      **DRAFTS_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.argtypes = args
             fn.restype = res

@@ -31,6 +31,17 @@ attention_fp4(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens,
     lse FP32 [T,Hq] or None. Queries that see nothing give zeros and -inf. workspace FP32
     [65536, D + 2], of any content, used by one stream at a time. Cache tensors span at most
     32 GiB each, page tables width * page_size <= 2^26 - 4096 tokens.
+attention_fp4_tree(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens, q_starts,
+                   parents, workspace, out, lse, scale, max_q, window=0)
+    The same for trees of at most 64 drafted tokens a sequence. Row i of a sequence's n is token
+    context_lens - n + i of the cache; INT32 parents [T] names its parent, a row before it, by its
+    number in the sequence (-1: the context alone is before it). A row attends to the tokens before
+    the tree, its ancestors and itself; its position is context_lens - n + the number of its
+    ancestors, which is what a window goes by (and what rope positions are).
+move_fp4(k_codes, k_scales, v_codes, v_scales, rows, slots, q_starts)
+    Cache rows to earlier ones of their sequence, all heads: slots[rows[i]] to slots[i] for i in
+    order where rows[i] > i; INT32 rows [T] are numbers in the sequence (others: nothing moves),
+    INT64 slots [T]. With verify_drafts' path the accepted rows become the sequence's first.
 """
 
 from typing import NamedTuple
@@ -43,6 +54,8 @@ qk_norm_rope = torch.ops.consumer_int8.qk_norm_rope
 append_fp4 = torch.ops.consumer_int8.append_fp4
 unpack_fp4 = torch.ops.consumer_int8.unpack_fp4
 attention_fp4 = torch.ops.consumer_int8.attention_fp4
+attention_fp4_tree = torch.ops.consumer_int8.attention_fp4_tree
+move_fp4 = torch.ops.consumer_int8.move_fp4
 
 
 @torch.library.register_fake("consumer_int8::qk_norm_rope")
@@ -65,6 +78,17 @@ def _unpack_fp4_fake(k_codes, k_scales, v_codes, v_scales, slots, k, v):
 @torch.library.register_fake("consumer_int8::attention_fp4")
 def _attention_fp4_fake(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens,
                         q_starts, workspace, out, lse, scale, max_q=1, window=0):
+    return None
+
+
+@torch.library.register_fake("consumer_int8::attention_fp4_tree")
+def _attention_fp4_tree_fake(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens,
+                             q_starts, parents, workspace, out, lse, scale, max_q, window=0):
+    return None
+
+
+@torch.library.register_fake("consumer_int8::move_fp4")
+def _move_fp4_fake(k_codes, k_scales, v_codes, v_scales, rows, slots, q_starts):
     return None
 
 

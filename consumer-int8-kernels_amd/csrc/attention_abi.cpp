@@ -1,6 +1,8 @@
-// The C ABI of the attention operators (include/consumer_int8_attention.h): argument
+// The C ABI of the attention operators (include/consumer_int8_attention.h, and of
+// include/consumer_int8_drafts.h what works on the same cache): argument
 // validation, then the launch. Pure host code up to the launch.
 #include "consumer_int8_attention.h"
+#include "consumer_int8_drafts.h"
 
 #include <cfloat>
 #include <climits>
@@ -218,6 +220,81 @@ int check_norm_launch(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t 
   return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
 }
 
+// Attention of chains of queries, and of trees where parents is not null.
+int attend(const ci8_heads* q, const ci8_fp4_cache* cache, const int32_t* page_table,
+           int64_t table_width, const int32_t* context_lens, const int32_t* q_starts,
+           const int32_t* parents, int64_t seqs, int64_t tokens, int64_t dim, void* workspace,
+           void* out, float* lse, double scale, int64_t max_q, int64_t window, void* stream) {
+  if (int s = check_tokens(tokens, dim)) return s;
+  if (int s = check_heads(q, tokens, dim)) return s;
+  Extents e;
+  if (int s = check_cache(cache, dim, e)) return s;
+  if (q->heads % cache->heads)
+    return abi_fail(CI8_ERR_GEOMETRY, "Query heads must be a multiple of the cache's heads");
+  if (!(seqs >= 0 && seqs <= 65535 && table_width >= 0 && max_q >= 1 && window >= 0 &&
+        std::isfinite(float(scale * 1.4426950408889634)) && (q_starts || seqs == tokens)))
+    return abi_fail(CI8_ERR_GEOMETRY,
+                    "Invalid attention: expected at most 65535 sequences, max_q >= 1, window >= "
+                    "0, a finite scale, and q_starts unless each sequence has one query");
+  // Tiles of 32 tokens, of 4 row blocks each of 64 sequences, are summed in 32 bits, and up to twice
+  // as many where each context takes a whole number of runs.
+  if (i128(table_width) * cache->page_size > (1 << 26) - 4096 ||
+      i128(seqs) * table_width * 4 > kMaxExtent)
+    return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large");
+  if (!aligned(page_table, 4) || !aligned(context_lens, 4) || !aligned(q_starts, 4) ||
+      !aligned(parents, 4) || !aligned(workspace, 16) || !aligned(out, 16) || !aligned(lse, 4))
+    return abi_fail(CI8_ERR_ALIGNMENT, "attention_fp4 requires aligned buffers");
+  const int64_t q_bytes = extent(*q, tokens, dim), out_bytes = tokens * q->heads * dim * 2;
+  const struct {
+    const void* p;
+    int64_t bytes;
+  } outputs[3] = {{out, out_bytes},
+                  {lse, lse ? tokens * q->heads * 4 : 0},
+                  {workspace, ci8::kAttentionWorkspaceRows * (dim + 2) * 4}},
+    inputs[5] = {{q->data, q_bytes},
+                 {page_table, seqs * table_width * 4},
+                 {context_lens, seqs * 4},
+                 {q_starts, q_starts ? (seqs + 1) * 4 : 0},
+                 {parents, parents ? tokens * 4 : 0}};
+  for (int i = 0; i < 3; ++i) {
+    bool shared = shares_cache(*cache, e, outputs[i].p, outputs[i].bytes);
+    for (const auto& in : inputs)
+      shared = shared || overlap(outputs[i].p, outputs[i].bytes, in.p, in.bytes);
+    for (int j = 0; j < i; ++j)
+      shared = shared || overlap(outputs[i].p, outputs[i].bytes, outputs[j].p, outputs[j].bytes);
+    if (shared)
+      return abi_fail(CI8_ERR_OVERLAP, "attention_fp4 outputs must not overlap anything else");
+  }
+  if (i128(tokens) * q->heads > (i128(1) << 30))
+    return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
+  ci8::AttentionArgs args = {};
+  args.q = view(*q);
+  args.cache = view(*cache);
+  args.page_table = page_table;
+  args.context_lens = context_lens;
+  args.q_starts = q_starts;
+  args.parents = parents;
+  args.workspace = static_cast<float*>(workspace);
+  args.out = static_cast<uint16_t*>(out);
+  args.lse = lse;
+  args.scale_log2 = std::fmax(std::fabs(float(scale * 1.4426950408889634)), FLT_MIN);
+  args.q_sign = scale < 0 ? 0x80008000u : 0;
+  args.table_width = int(table_width);
+  args.seqs = int(seqs);
+  args.tokens = int(tokens);
+  args.group = int(q->heads / cache->heads);
+  args.max_q = int(max_q < tokens ? max_q : tokens);
+  // A workgroup a unit, and one more for each of up to 256 CUs.
+  if (ci8::row_split(tokens, seqs, args.group, args.max_q).prompt &&
+      !ci8::launch_fits(
+          ci8::prompt_units(tokens, seqs, args.group, args.max_q, args.cache.heads) + 256,
+          ci8::kPromptThreads))
+    return abi_fail(CI8_ERR_TOO_LARGE, "Too many sequences");
+  // As many tokens as a page table holds are all; differences and sums with fewer stay in 32 bits.
+  args.window = int(window < table_width * cache->page_size ? window : 0);
+  return abi_launched(ci8::launch_attention_fp4(args, int(dim), as_stream(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -325,72 +402,41 @@ int ci8_attention_fp4(const ci8_heads* q, const ci8_fp4_cache* cache,
                       const int32_t* context_lens, const int32_t* q_starts, int64_t seqs,
                       int64_t tokens, int64_t dim, void* workspace, void* out, float* lse,
                       double scale, int64_t max_q, int64_t window, void* stream) {
+  return attend(q, cache, page_table, table_width, context_lens, q_starts, nullptr, seqs, tokens, dim,
+                workspace, out, lse, scale, max_q, window, stream);
+}
+
+int ci8_attention_fp4_tree(const ci8_heads* q, const ci8_fp4_cache* cache,
+                           const int32_t* page_table, int64_t table_width,
+                           const int32_t* context_lens, const int32_t* q_starts,
+                           const int32_t* parents, int64_t seqs, int64_t tokens, int64_t dim,
+                           void* workspace, void* out, float* lse, double scale, int64_t max_q,
+                           int64_t window, void* stream) {
+  if (!q_starts || (!parents && tokens > 0))
+    return abi_fail(CI8_ERR_GEOMETRY, "A tree needs q_starts and parents");
+  if (max_q > ci8::kMostTree)
+    return abi_fail(CI8_ERR_TOO_LARGE, "A tree has at most 64 queries");
+  return attend(q, cache, page_table, table_width, context_lens, q_starts, parents, seqs, tokens, dim,
+                workspace, out, lse, scale, max_q, window, stream);
+}
+
+int ci8_move_fp4(const ci8_fp4_cache* cache, const int32_t* rows, const int64_t* slots,
+                 const int32_t* q_starts, int64_t seqs, int64_t tokens, int64_t dim, void* stream) {
   if (int s = check_tokens(tokens, dim)) return s;
-  if (int s = check_heads(q, tokens, dim)) return s;
   Extents e;
   if (int s = check_cache(cache, dim, e)) return s;
-  if (q->heads % cache->heads)
-    return abi_fail(CI8_ERR_GEOMETRY, "Query heads must be a multiple of the cache's heads");
-  if (!(seqs >= 0 && seqs <= 65535 && table_width >= 0 && max_q >= 1 && window >= 0 &&
-        std::isfinite(float(scale * 1.4426950408889634)) && (q_starts || seqs == tokens)))
-    return abi_fail(CI8_ERR_GEOMETRY,
-                    "Invalid attention: expected at most 65535 sequences, max_q >= 1, window >= "
-                    "0, a finite scale, and q_starts unless each sequence has one query");
-  // Tiles of 32 tokens, of 4 row blocks each of 64 sequences, are summed in 32 bits, and up to twice
-  // as many where each context takes a whole number of runs.
-  if (i128(table_width) * cache->page_size > (1 << 26) - 4096 ||
-      i128(seqs) * table_width * 4 > kMaxExtent)
-    return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large");
-  if (!aligned(page_table, 4) || !aligned(context_lens, 4) || !aligned(q_starts, 4) ||
-      !aligned(workspace, 16) || !aligned(out, 16) || !aligned(lse, 4))
-    return abi_fail(CI8_ERR_ALIGNMENT, "attention_fp4 requires aligned buffers");
-  const int64_t q_bytes = extent(*q, tokens, dim), out_bytes = tokens * q->heads * dim * 2;
-  const struct {
-    const void* p;
-    int64_t bytes;
-  } outputs[3] = {{out, out_bytes},
-                  {lse, lse ? tokens * q->heads * 4 : 0},
-                  {workspace, ci8::kAttentionWorkspaceRows * (dim + 2) * 4}},
-    inputs[4] = {{q->data, q_bytes},
-                 {page_table, seqs * table_width * 4},
-                 {context_lens, seqs * 4},
-                 {q_starts, q_starts ? (seqs + 1) * 4 : 0}};
-  for (int i = 0; i < 3; ++i) {
-    bool shared = shares_cache(*cache, e, outputs[i].p, outputs[i].bytes);
-    for (const auto& in : inputs)
-      shared = shared || overlap(outputs[i].p, outputs[i].bytes, in.p, in.bytes);
-    for (int j = 0; j < i; ++j)
-      shared = shared || overlap(outputs[i].p, outputs[i].bytes, outputs[j].p, outputs[j].bytes);
-    if (shared)
-      return abi_fail(CI8_ERR_OVERLAP, "attention_fp4 outputs must not overlap anything else");
-  }
-  if (i128(tokens) * q->heads > (i128(1) << 30))
-    return abi_fail(CI8_ERR_TOO_LARGE, "Too many tokens");
-  ci8::AttentionArgs args = {};
-  args.q = view(*q);
-  args.cache = view(*cache);
-  args.page_table = page_table;
-  args.context_lens = context_lens;
-  args.q_starts = q_starts;
-  args.workspace = static_cast<float*>(workspace);
-  args.out = static_cast<uint16_t*>(out);
-  args.lse = lse;
-  args.scale_log2 = std::fmax(std::fabs(float(scale * 1.4426950408889634)), FLT_MIN);
-  args.q_sign = scale < 0 ? 0x80008000u : 0;
-  args.table_width = int(table_width);
-  args.seqs = int(seqs);
-  args.tokens = int(tokens);
-  args.group = int(q->heads / cache->heads);
-  args.max_q = int(max_q < tokens ? max_q : tokens);
-  // A workgroup a unit, and one more for each of up to 256 CUs.
-  if (ci8::row_split(tokens, seqs, args.group, args.max_q).prompt &&
-      !ci8::launch_fits(
-          ci8::prompt_units(tokens, seqs, args.group, args.max_q, args.cache.heads) + 256,
-          ci8::kPromptThreads))
+  if (!(seqs >= 0 && seqs <= 65535))
+    return abi_fail(CI8_ERR_GEOMETRY, "Invalid move: expected at most 65535 sequences");
+  if (!aligned(rows, 4) || !aligned(slots, 8) || !aligned(q_starts, 4))
+    return abi_fail(CI8_ERR_ALIGNMENT, "move_fp4 requires aligned buffers");
+  if (int s = check_cache_written(*cache, e)) return s;
+  if (shares_cache(*cache, e, rows, tokens * 4) || shares_cache(*cache, e, slots, tokens * 8) ||
+      shares_cache(*cache, e, q_starts, (seqs + 1) * 4))
+    return abi_fail(CI8_ERR_OVERLAP, "The cache must not overlap an input");
+  if (!ci8::launch_fits(seqs * ci8::move_blocks(cache->heads, int(dim)), ci8::kMoveThreads))
     return abi_fail(CI8_ERR_TOO_LARGE, "Too many sequences");
-  // As many tokens as a page table holds are all; differences and sums with fewer stay in 32 bits.
-  args.window = int(window < table_width * cache->page_size ? window : 0);
-  return abi_launched(ci8::launch_attention_fp4(args, int(dim), as_stream(stream)));
+  return abi_launched(ci8::launch_move_fp4(view(*cache), rows, slots, q_starts, int(seqs),
+                                           int(tokens), int(dim), as_stream(stream)));
 }
 
 }  // extern "C"

@@ -26,6 +26,7 @@ __device__ __forceinline__ u32x2 lds_read_transposed(const char* p) {
 // What one sequence asks for.
 struct Sequence {
   int q_begin, rows;        // first query row, and rows of (query, head) computed
+  int shown;                // queries computed
   int context, shift;       // tokens; position of query 0
   int low, high;            // tokens that any row attends to
   int first_high, last_low; // every row attends to [last_low, first_high)
@@ -44,6 +45,7 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int seq) {
     count = min(max(p.q_starts[seq + 1], s.q_begin), p.tokens) - s.q_begin;
   }
   const int shown = min(count, p.max_q);
+  s.shown = shown;
   s.rows = shown * p.group;
   const int64_t capacity = int64_t(p.table_width) << p.cache.page_shift;
   s.context = int(min(int64_t(max(p.context_lens[seq], 0)), capacity));
@@ -53,6 +55,45 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int seq) {
   s.low = p.window ? max(s.first_high - p.window, 0) : 0;
   s.last_low = p.window ? max(s.high - p.window, 0) : 0;
   return s;
+}
+
+// A tree of at most 64 queries. Lane l gets the set of query l and its ancestors, bit a for query a:
+// sets of parents are joined while the way up from each doubles, six rounds at most. A parent is
+// a query before its own; any other number is none.
+__device__ __forceinline__ uint64_t tree_ancestors(const AttentionArgs& p, const Sequence& s,
+                                                   int lane) {
+  int up = -1;
+  if (lane < s.shown) up = p.parents[s.q_begin + lane];
+  if (up >= lane) up = -1;
+  uint64_t set = uint64_t(1) << lane;
+  while (__any(up >= 0)) {
+    const int from = max(up, 0);
+    const uint32_t low = __shfl(int(set), from, 64), high = __shfl(int(set >> 32), from, 64);
+    const int next = __shfl(up, from, 64);
+    if (up >= 0) {
+      set |= uint64_t(high) << 32 | low;
+      up = next < 0 ? -1 : next;
+    }
+  }
+  return set;
+}
+
+// Those that query l attends to: of its own set a window leaves the last, whose depths are largest.
+__device__ __forceinline__ uint64_t tree_seen(const AttentionArgs& p, uint64_t set) {
+  if (p.window)
+    while (__builtin_popcountll(set) > p.window) set &= set - 1;
+  return set;
+}
+// The first token that query `query` attends to; depths are those of the lanes' queries.
+__device__ __forceinline__ int tree_low(const AttentionArgs& p, const Sequence& s, int depth,
+                                        int query) {
+  return p.window ? max(s.shift + __shfl(depth, query, 64) + 1 - p.window, 0) : 0;
+}
+// Whether a row of a tree, which sees tokens up to `high`, sees one of them: those before the tree,
+// and those that its query's set in LDS names.
+__device__ __forceinline__ bool tree_sees(const uint64_t* seen, int high, int token, int shift) {
+  const uint64_t set = seen[max(high - 1 - shift, 0) & 63];
+  return (token < shift) | ((set >> (uint32_t(token - shift) & 63) & 1) != 0);
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

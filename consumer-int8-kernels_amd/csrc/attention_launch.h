@@ -49,6 +49,10 @@ hipError_t launch_norm_rope(const NormRopeArgs& args, int dim, bool append, hipS
 hipError_t launch_unpack_fp4(const Fp4CacheView& cache, const int64_t* slots, uint16_t* k,
                              uint16_t* v, int count, int dim, hipStream_t stream);
 
+hipError_t launch_move_fp4(const Fp4CacheView& cache, const int32_t* rows, const int64_t* slots,
+                           const int32_t* q_starts, int seqs, int tokens, int dim,
+                           hipStream_t stream);
+
 // Rows of partial sums that the workspace holds, FP32 [rows, dim] and then [rows, 2].
 constexpr int kAttentionWorkspaceRows = 65536;
 
@@ -58,6 +62,7 @@ struct AttentionArgs {
   const int32_t* page_table;
   const int32_t* context_lens;
   const int32_t* q_starts;  // null: one query a sequence
+  const int32_t* parents;   // null: each query sees those before it; else a tree of at most 64
   float* workspace;
   uint16_t* out;
   float* lse;  // may be null

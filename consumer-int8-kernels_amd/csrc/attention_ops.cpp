@@ -1,44 +1,13 @@
 // torch.ops.consumer_int8 registration of the attention operators over their C ABI
-// (include/consumer_int8_attention.h). As in torch_ops.cpp: devices, dtypes and shapes are
+// (include/consumer_int8_attention.h; of include/consumer_int8_drafts.h what works on the same
+// cache). As in torch_ops.cpp: devices, dtypes and shapes are
 // checked here, geometry, alignment and overlap by the C ABI; calls run on the current stream
 // of the input's device, allocate nothing and never synchronize.
-#include <torch/csrc/inductor/aoti_torch/c/shim.h>
-#include <torch/csrc/stable/accelerator.h>
-#include <torch/csrc/stable/library.h>
-#include <torch/csrc/stable/tensor.h>
-#include <torch/headeronly/util/Exception.h>
-
-#include <optional>
-#include <string>
-
 #include "consumer_int8_attention.h"
-
-using torch::headeronly::ScalarType;
-using torch::stable::Tensor;
-using MaybeTensor = std::optional<Tensor>;
+#include "consumer_int8_drafts.h"
+#include "torch_checks.h"
 
 namespace {
-
-void check_type(const Tensor& t, ScalarType dtype, int device) {
-  STD_TORCH_CHECK(t.is_cuda() && t.get_device_index() == device,
-                  "All tensors must be on the same CUDA device");
-  STD_TORCH_CHECK(t.scalar_type() == dtype, "Unexpected dtype");
-}
-
-void check_plain(const Tensor& t, ScalarType dtype, int device) {
-  check_type(t, dtype, device);
-  STD_TORCH_CHECK(t.is_contiguous(), "Unexpected noncontiguous tensor");
-}
-
-void* stream_for(int device) {
-  void* stream = nullptr;
-  TORCH_ERROR_CODE_CHECK(aoti_torch_get_current_cuda_stream(device, &stream));
-  return stream;
-}
-
-void raise_on_error(int status) {
-  STD_TORCH_CHECK(status == CI8_OK, std::string(ci8_last_error()));
-}
 
 // BF16 [tokens, heads, dim] with contiguous channels. The stride of an axis of length 1 says
 // nothing and is set.
@@ -197,10 +166,12 @@ void unpack_fp4(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales
                                 k.data_ptr(), v.data_ptr(), count, dim, stream_for(device)));
 }
 
-void attention_fp4(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales,
-                   Tensor page_table, Tensor context_lens, MaybeTensor q_starts,
-                   Tensor workspace, Tensor out, MaybeTensor lse, double scale, int64_t max_q,
-                   int64_t window) {
+// Attention of chains of queries, and of trees where there are parents.
+void attend(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes,
+            const Tensor& v_scales, const Tensor& page_table, const Tensor& context_lens,
+            const MaybeTensor& q_starts, const Tensor* parents, const Tensor& workspace,
+            const Tensor& out, const MaybeTensor& lse, double scale, int64_t max_q,
+            int64_t window) {
   const int device = q.get_device_index();
   const ci8_heads qv = heads_of(q, device);
   const int64_t tokens = q.size(0), dim = q.size(2);
@@ -226,14 +197,60 @@ void attention_fp4(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Te
     STD_TORCH_CHECK(lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == q.size(1),
                     "Expected FP32 lse [tokens, heads]");
   }
+  if (parents) {
+    check_plain(*parents, ScalarType::Int, device);
+    STD_TORCH_CHECK(parents->dim() == 1 && parents->size(0) == tokens,
+                    "Expected INT32 parents [tokens]");
+  }
   torch::stable::accelerator::DeviceGuard guard(device);
-  raise_on_error(ci8_attention_fp4(
-      &qv, &cache, static_cast<const int32_t*>(page_table.data_ptr()), page_table.size(1),
-      static_cast<const int32_t*>(context_lens.data_ptr()),
-      q_starts.has_value() ? static_cast<const int32_t*>(q_starts->data_ptr()) : nullptr, seqs,
-      tokens, dim, workspace.data_ptr(), out.data_ptr(),
-      lse.has_value() ? static_cast<float*>(lse->data_ptr()) : nullptr, scale, max_q, window,
-      stream_for(device)));
+  const auto* table = static_cast<const int32_t*>(page_table.data_ptr());
+  const auto* lens = static_cast<const int32_t*>(context_lens.data_ptr());
+  const auto* starts =
+      q_starts.has_value() ? static_cast<const int32_t*>(q_starts->data_ptr()) : nullptr;
+  float* const sums = lse.has_value() ? static_cast<float*>(lse->data_ptr()) : nullptr;
+  void* const stream = stream_for(device);
+  raise_on_error(
+      parents ? ci8_attention_fp4_tree(&qv, &cache, table, page_table.size(1), lens, starts,
+                                       static_cast<const int32_t*>(parents->data_ptr()), seqs,
+                                       tokens, dim, workspace.data_ptr(), out.data_ptr(), sums,
+                                       scale, max_q, window, stream)
+              : ci8_attention_fp4(&qv, &cache, table, page_table.size(1), lens, starts, seqs, tokens,
+                                  dim, workspace.data_ptr(), out.data_ptr(), sums, scale, max_q,
+                                  window, stream));
+}
+
+void attention_fp4(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales,
+                   Tensor page_table, Tensor context_lens, MaybeTensor q_starts,
+                   Tensor workspace, Tensor out, MaybeTensor lse, double scale, int64_t max_q,
+                   int64_t window) {
+  attend(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens, q_starts, nullptr,
+         workspace, out, lse, scale, max_q, window);
+}
+
+void attention_fp4_tree(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales,
+                        Tensor page_table, Tensor context_lens, Tensor q_starts, Tensor parents,
+                        Tensor workspace, Tensor out, MaybeTensor lse, double scale, int64_t max_q,
+                        int64_t window) {
+  attend(q, k_codes, k_scales, v_codes, v_scales, page_table, context_lens, q_starts, &parents,
+         workspace, out, lse, scale, max_q, window);
+}
+
+void move_fp4(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor rows,
+              Tensor slots, Tensor q_starts) {
+  const int device = rows.get_device_index();
+  check_plain(rows, ScalarType::Int, device);
+  check_plain(slots, ScalarType::Long, device);
+  check_plain(q_starts, ScalarType::Int, device);
+  STD_TORCH_CHECK(rows.dim() == 1 && slots.dim() == 1 && slots.size(0) == rows.size(0) &&
+                      q_starts.dim() == 1 && q_starts.size(0) >= 1 && k_codes.dim() == 4,
+                  "Expected INT32 rows [tokens], INT64 slots [tokens] and INT32 q_starts [seqs + 1]");
+  const int64_t dim = k_codes.size(3) * 2;
+  const ci8_fp4_cache cache = cache_of(k_codes, k_scales, v_codes, v_scales, dim, device);
+  torch::stable::accelerator::DeviceGuard guard(device);
+  raise_on_error(ci8_move_fp4(&cache, static_cast<const int32_t*>(rows.data_ptr()),
+                              static_cast<const int64_t*>(slots.data_ptr()),
+                              static_cast<const int32_t*>(q_starts.data_ptr()),
+                              q_starts.size(0) - 1, rows.size(0), dim, stream_for(device)));
 }
 
 }  // namespace
@@ -243,6 +260,8 @@ STABLE_TORCH_LIBRARY_FRAGMENT(consumer_int8, m) {
   m.def("append_fp4(Tensor? q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor? rope, Tensor? positions, Tensor? axes, Tensor slots, Tensor(a!)? q_out, Tensor(b!) k_codes, Tensor(c!) k_scales, Tensor(d!) v_codes, Tensor(e!) v_scales, float eps=1e-06, bool interleaved=False) -> ()");
   m.def("unpack_fp4(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor slots, Tensor(a!) k, Tensor(b!) v) -> ()");
   m.def("attention_fp4(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor page_table, Tensor context_lens, Tensor? q_starts, Tensor(a!) workspace, Tensor(b!) out, Tensor(c!)? lse, float scale, int max_q=1, int window=0) -> ()");
+  m.def("attention_fp4_tree(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor page_table, Tensor context_lens, Tensor q_starts, Tensor parents, Tensor(a!) workspace, Tensor(b!) out, Tensor(c!)? lse, float scale, int max_q, int window=0) -> ()");
+  m.def("move_fp4(Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!) v_codes, Tensor(d!) v_scales, Tensor rows, Tensor slots, Tensor q_starts) -> ()");
 }
 
 STABLE_TORCH_LIBRARY_IMPL(consumer_int8, CUDA, m) {
@@ -250,4 +269,6 @@ STABLE_TORCH_LIBRARY_IMPL(consumer_int8, CUDA, m) {
   m.impl("append_fp4", TORCH_BOX(&append_fp4));
   m.impl("unpack_fp4", TORCH_BOX(&unpack_fp4));
   m.impl("attention_fp4", TORCH_BOX(&attention_fp4));
+  m.impl("attention_fp4_tree", TORCH_BOX(&attention_fp4_tree));
+  m.impl("move_fp4", TORCH_BOX(&move_fp4));
 }

@@ -39,6 +39,15 @@ inline int64_t unpack_workgroups(int64_t count, int heads, int dim) {
   return (count * heads * (dim / 8) + kUnpackThreads - 1) / kUnpackThreads;
 }
 
+// move_fp4: a thread for 16 bytes of codes or the scales of a head's row, keys or values.
+constexpr int kMoveThreads = 256;
+inline int64_t move_blocks(int64_t heads, int dim) {
+  return (heads * 2 * (dim / 32 + 1) + kMoveThreads - 1) / kMoveThreads;
+}
+
+// attention_fp4_tree: a tree's queries are a wave's lanes.
+constexpr int kMostTree = 64;
+
 // attention_fp4: rows are (token, query head of one key head) pairs. Sequences of at most `few` rows go
 // to the split kernel, the others to the prompt kernel.
 //

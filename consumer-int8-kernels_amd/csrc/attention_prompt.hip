@@ -122,7 +122,8 @@ __device__ __forceinline__ float* part_stats(const AttentionArgs& p, int64_t row
   return p.workspace + int64_t(kAttentionWorkspaceRows) * dim + row * 2;
 }
 
-template <int D>
+// kTree: queries are a tree of drafted tokens.
+template <int D, bool kTree>
 __global__ void __launch_bounds__(Shape<D>::kThreads)
     attention_prompt_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
   using S = Shape<D>;
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   constexpr int kValues = kKeyBuffers * S::kKeyBytes;
   __shared__ uint8_t poison[kPoisonBuffers][kTokens][S::kBlocks];  // NaN blocks of edge tiles
   __shared__ int poisoned[kPoisonBuffers];  // the last such tile that has any
+  __shared__ uint64_t tree[kTree ? 64 : 1];  // what each query sees of the tree, bit a for query a
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6);
   const int column = lane & 31, half = lane >> 5;
@@ -159,9 +161,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   const int row0 = (where.tiles - 1 - where.tile) * S::kRows;
   const int last_row = min(row0 + S::kRows, s.rows) - 1;
 
-  // Tokens that any row of the workgroup attends to, and those that all attend to.
-  const int first_high = s.shift + row0 / p.group + 1, high = max(s.shift + last_row / p.group + 1, 0);
-  const int tile_low = p.window ? max(first_high - p.window, 0) : 0;
+  // Tokens that any row of the workgroup attends to, and those that all attend to: of a tree none,
+  // and its first positions are those right behind the context.
+  const int first_high = kTree ? s.shift : s.shift + row0 / p.group + 1;
+  const int high = max(s.shift + last_row / p.group + 1, 0);
+  const int tile_low = p.window ? max(first_high + (kTree ? 1 : 0) - p.window, 0) : 0;
   const int last_low = p.window ? max(high - p.window, 0) : 0;
   int t_begin = tile_low / kTokens, t_end = (high + kTokens - 1) / kTokens;
   if (splits > 1) {
@@ -276,13 +280,22 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
   // go nowhere.
   int row_low[kTiles], row_high[kTiles];
+  int depth = 0;
+  if (kTree) {
+    const uint64_t set = tree_ancestors(p, s, lane);
+    depth = __builtin_popcountll(set) - 1;
+    tree[kTree ? lane : 0] = tree_seen(p, set);  // every wave the same
+  }
   u32x4 q[kTiles][kHeld];
   const int wave_row = row0 + wave * 32 * kTiles;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
     const int row = min(wave_row + 32 * n + column, s.rows - 1), query = row / p.group;
     row_high[n] = s.shift + query + 1;
-    row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
+    if constexpr (kTree)
+      row_low[n] = tree_low(p, s, depth, query);
+    else
+      row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
     const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
                           int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
 #pragma unroll
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     load_codes(ahead, pages_ahead, t_begin + 1, t_begin);
   }
   // Tokens [all_low, all_high) that all of the wave's rows attend to.
-  const int all_high = s.shift + min(wave_row, s.rows - 1) / p.group + 1;
+  const int all_high = kTree ? s.shift : s.shift + min(wave_row, s.rows - 1) / p.group + 1;
   const int any_high = s.shift + min(wave_row + 32 * kTiles - 1, s.rows - 1) / p.group + 1;
   const int all_low = p.window ? max(any_high - p.window, 0) : 0;
 
@@ -404,7 +417,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         for (int i = 0; i < 16; ++i) {
           const int at = 8 * (i / 4) + i % 4, token = first + at + 4 * half;
           const bool seen = (token >= row_low[n]) & (token < row_high[n]) &
-                            (at < 16 ? low_there : high_there);
+                            (at < 16 ? low_there : high_there) &
+                            (!kTree || tree_sees(tree, row_high[n], token, s.shift));
           x[n][i] = seen ? x[n][i] : -__builtin_inff();
         }
         most[n] = largest(x[n]);
@@ -480,7 +494,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         if (poison[t % kPoisonBuffers][token][m]) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n])
+            if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n] &&
+                (!kTree || tree_sees(tree, row_high[n], t * kTokens + token, s.shift)))
               o[n][m] += __builtin_nanf("");
         }
   };
@@ -669,7 +684,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   write_row4(p, D, s.q_begin, row, unit % p.cache.heads, channel, x, top, total);
 }
 
-template <int D>
+template <int D, bool kTree>
 hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream) {
   using S = Shape<D>;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
@@ -686,7 +701,7 @@ hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream)
   if (splits > cus) splits = cus;
   if (splits < 1) splits = 1;
   const int64_t grid = units + (splits > 1 ? cus : 0);
-  attention_prompt_kernel<D>
+  attention_prompt_kernel<D, kTree>
       <<<uint32_t(grid), S::kThreads, 0, stream>>>(args, few, cus, int(splits));
   if (splits == 1) return hipGetLastError();
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
@@ -701,9 +716,15 @@ hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream)
 
 hipError_t launch_attention_prompt(const AttentionArgs& args, int dim, int few, hipStream_t stream) {
   switch (dim) {
-    case 64: return launch_prompt<64>(args, few, stream);
-    case 128: return launch_prompt<128>(args, few, stream);
-    default: return launch_prompt<256>(args, few, stream);
+    case 64:
+      return args.parents ? launch_prompt<64, true>(args, few, stream)
+                          : launch_prompt<64, false>(args, few, stream);
+    case 128:
+      return args.parents ? launch_prompt<128, true>(args, few, stream)
+                          : launch_prompt<128, false>(args, few, stream);
+    default:
+      return args.parents ? launch_prompt<256, true>(args, few, stream)
+                          : launch_prompt<256, false>(args, few, stream);
   }
 }
 

@@ -195,8 +195,9 @@ constexpr int groups_per_cu(int dim, int tiles) {
   return dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
 }
 
-// kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone.
-template <int D, int kTiles, int kWaves, bool kSplit>
+// kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone. kTree:
+// queries are a tree of drafted tokens.
+template <int D, int kTiles, int kWaves, bool kSplit, bool kTree>
 __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles) * kWaves / 4 : kWaves / 4)
     attention_split_kernel(const AttentionArgs, int most, int most_blocks, int min_quota,
                            bool by_context, bool apart) {
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   constexpr bool kQueriesInLds = D == 256 && kTiles == 2;
   constexpr int kSteps = L::kChunks * L::kSteps;
   __shared__ u32x4 queries[kQueriesInLds ? kTiles * kSteps * 64 : 1];
+  __shared__ uint64_t tree[kTree ? 64 : 1];  // what each query sees of the tree, bit a for query a
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -281,6 +283,15 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
 
     // The lane's rows: their queries, and the tokens [low, high) that each attends to.
     int low[kTiles], high[kTiles];
+    int depth = 0;
+    // Every row attends to [last_low, all_high). Of a tree nothing is known; the sets are for the
+    // tiles that have some of it, and depths for a window.
+    const int all_high = kTree ? s.shift : s.first_high;
+    if (kTree && (p.window || t_end * kTokens > s.shift)) {
+      const uint64_t set = tree_ancestors(p, s, lane);
+      depth = __builtin_popcountll(set) - 1;
+      tree[kTree ? lane : 0] = tree_seen(p, set);  // every wave the same
+    }
     u32x4 q[kTiles][L::kChunks][L::kSteps];
     if (kQueriesInLds) __syncthreads();  // the last ones are read
 #pragma unroll
@@ -289,7 +300,10 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       const bool live = row < s.rows;
       const int query = live ? row / p.group : 0;
       high[n] = live ? s.shift + query + 1 : 0;
-      low[n] = p.window ? max(high[n] - p.window, 0) : 0;
+      if constexpr (kTree)
+        low[n] = tree_low(p, s, depth, query);
+      else
+        low[n] = p.window ? max(high[n] - p.window, 0) : 0;
       const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
                             int64_t(kv_head * p.group + (live ? row % p.group : 0)) *
                                 p.q.head_stride;
@@ -378,7 +392,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       }
 
       // Tiles that some row sees in part, or that are not whole.
-      const bool edge = (t + 1) * kTokens > s.first_high || t * kTokens < s.last_low ||
+      const bool edge = (t + 1) * kTokens > all_high || t * kTokens < s.last_low ||
                         there != 3;
       // Scores, lane: row `column`, tokens 4 * group4 + i of each half.
       f32x4 score[kTiles][2];
@@ -451,7 +465,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int token = t * kTokens + 16 * h + 4 * group4 + j;
-              const bool seen = (there >> h & 1) & (token >= low[n]) & (token < high[n]);
+              const bool seen = (there >> h & 1) & (token >= low[n]) & (token < high[n]) &
+                                (!kTree || tree_sees(tree, high[n], token, s.shift));
               score[n][h][j] = seen ? score[n][h][j] : -__builtin_inff();
             }
         }
@@ -497,7 +512,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
           const uint32_t blocks = uint32_t(__shfl(int(poisoned[token / 16]), token % 16, 64));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            if (t * kTokens + token >= low[n] && t * kTokens + token < high[n]) {
+            if (t * kTokens + token >= low[n] && t * kTokens + token < high[n] &&
+                (!kTree || tree_sees(tree, high[n], t * kTokens + token, s.shift))) {
 #pragma unroll
               for (int m = 0; m < D / 16; ++m)
                 o[n][m] += blocks >> (m / 2) & 1 ? __builtin_nanf("") : 0.f;
@@ -704,7 +720,7 @@ __global__ void __launch_bounds__(kThreads)
 // short contexts is split.
 constexpr int whole_tiles(int dim, bool few) { return !few ? 64 : dim == 256 ? 32 : 48; }
 
-template <int D, int kTiles>
+template <int D, int kTiles, bool kTree>
 hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream) {
   const int64_t longest = (int64_t(args.table_width) << args.cache.page_shift) / kTokens;
   const int64_t span = args.window ? (int64_t(args.window) + args.max_q) / kTokens + 2 : longest;
@@ -718,7 +734,7 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   constexpr int kWholeWaves = 8;
   if ((longest < span ? longest : span) <= whole_tiles(D, 4 * contexts <= cus) &&
       launch_fits(contexts, 64 * kWholeWaves)) {
-    attention_split_kernel<D, kTiles, kWholeWaves, false>
+    attention_split_kernel<D, kTiles, kWholeWaves, false, kTree>
         <<<uint32_t(contexts), 64 * kWholeWaves, 0, stream>>>(args, most, blocks, 0, false, false);
     return hipGetLastError();
   }
@@ -740,7 +756,7 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   // to 3006 of 4 (3.8 a context) 21.8 and 23.5; but 32 up to 8000 of 8 (3) 38.1 and 37.7, 16 x 5 rows
   // of 64 heads up to 16000 (2) 91 and 81.
   const bool apart = 3 * contexts < groups && args.seqs <= 64;
-  attention_split_kernel<D, kTiles, kWaves, true>
+  attention_split_kernel<D, kTiles, kWaves, true, kTree>
       <<<groups, 64 * kWaves, 0, stream>>>(args, most, blocks, 2 * kWaves, by_context, apart);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   // More threads where a context has many parts. Whole calls with 1024 and with 256, us: one of 131071
@@ -754,20 +770,26 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
 
 }  // namespace
 
+template <int kTiles>
+static hipError_t launch_split_rows(const AttentionArgs& args, int dim, int most,
+                                    hipStream_t stream) {
+  switch (dim) {
+    case 64:
+      return args.parents ? launch_split<64, kTiles, true>(args, most, stream)
+                          : launch_split<64, kTiles, false>(args, most, stream);
+    case 128:
+      return args.parents ? launch_split<128, kTiles, true>(args, most, stream)
+                          : launch_split<128, kTiles, false>(args, most, stream);
+    default:
+      return args.parents ? launch_split<256, kTiles, true>(args, most, stream)
+                          : launch_split<256, kTiles, false>(args, most, stream);
+  }
+}
+
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream) {
-  if (most <= 16) {
-    switch (dim) {
-      case 64: return launch_split<64, 1>(args, most, stream);
-      case 128: return launch_split<128, 1>(args, most, stream);
-      default: return launch_split<256, 1>(args, most, stream);
-    }
-  }
-  switch (dim) {
-    case 64: return launch_split<64, 2>(args, most, stream);
-    case 128: return launch_split<128, 2>(args, most, stream);
-    default: return launch_split<256, 2>(args, most, stream);
-  }
+  return most <= 16 ? launch_split_rows<1>(args, dim, most, stream)
+                    : launch_split_rows<2>(args, dim, most, stream);
 }
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
