@@ -93,12 +93,13 @@ def build_library(jobs: int = 8) -> Path:
 
 
 def build_probe() -> Path:
-    """bench.py's measurement library: the MFMA/HBM probes (probe.hip) and the persistent
-    GEMM with clock stamps (probe_pp.hip, built with gemm_pp.hip's flags). It links the
-    drop-in library for device_cu_count."""
+    """bench.py's measurement library: the MFMA/HBM probes (probe.hip), the persistent
+    GEMM with clock stamps (probe_pp.hip, built with gemm_pp.hip's flags) and, for tests, the
+    verification of drafts without its waits (probe_verify.hip). It links the drop-in library
+    for device_cu_count."""
     BUILD_DIR.mkdir(exist_ok=True)
     objects = [_compile(CSRC / name, BUILD_DIR / (Path(name).stem + ".o"))
-               for name in ("probe.hip", "probe_pp.hip")]
+               for name in ("probe.hip", "probe_pp.hip", "probe_verify.hip")]
     target = OUT_DIR / "libci8_probe.so"
     tmp = target.with_suffix(".so.tmp")
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objects),

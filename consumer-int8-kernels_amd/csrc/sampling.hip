@@ -2,14 +2,9 @@
 //
 //   p_i = exp2((l_i - m) c) / sum_j exp2((l_j - m) c),   c = log2(e) / temperature, m = max l
 //
-// and rejection sampling of drafted tokens against such rows. A vocabulary is one or two passes over
-// memory and a few operations a value: bound by HBM for many rows, by launches and dependent loads for
-// few, so a row is cut into chunks that fill the GPU, whose sums are joined by a second kernel in a
-// fixed order (no atomics, the same bits every time).
-//
-// Which drafts stand takes one value of p and q a row, all loaded at once, a row a lane. Only where none
-// stands any more is a vocabulary read. Weights, sums and comparisons are in 64 bits: a running sum over
-// 150000 values in 32 would lose tokens of less than 6e-8 of it.
+// and rejection sampling of drafted tokens against such rows. A vocabulary is one pass over memory
+// and a few operations a value: bound by HBM for many rows, by launches and dependent loads for few.
+// No sum depends on what finishes first: the same bits every time.
 #include "ci8_device.h"
 #include "sampling_launch.h"
 #include "sampling_plan.h"
@@ -18,7 +13,6 @@ namespace ci8 {
 namespace {
 
 // Vectors that need not start on their size: a row starts wherever its stride puts it.
-typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) loose_u32x4;
 typedef float __attribute__((ext_vector_type(4), aligned(4))) loose_f32x4;
 
 constexpr float kInf = __builtin_inff();
@@ -43,48 +37,60 @@ __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); 
 __device__ __forceinline__ int smaller(int a, int b) { return min(a, b); }
 
 // ---- token_probs ------------------------------------------------------------------------
+//
+// A workgroup of 1024 threads a row holds the row in registers: it is read once, then its largest, the
+// sum of its weights and the probabilities are computed from there (the exponential twice: weights
+// in 32 bits would not fit beside). Where rows are few, several workgroups share one: each reads all
+// of it, from the L2s, and writes a part; one launch, and nothing to wait for. Rows that are few and
+// long take two kernels over their chunks instead (sampling_plan.h has both sides' times).
+// Measured: 512 rows of 152000 BF16 logits 110 us, 4.2 TB/s of the 5.1 that a copy reaches; 1000 of 50001
+// in FP32 89, 4.5; one of 32000 5.7, 3 of it the launch. Plain stores: nontemporal ones 163.
 
-// Eight values of a row from `at` on; past the end -inf.
+// Registers hold 163840 BF16 or 81920 FP32 values of a row, or 32768 in less code, which a launch of
+// few workgroups has to fetch first: one row of 32000 5.4 us, with room for 163840 10.8.
+constexpr int kFewHeld = 8;
+constexpr int kPackValues = 4, kRowStep = kRowThreads * kPackValues;  // values that all threads take
+static_assert(kRowStep == kProbsPart && kFewVocab <= (kFewHeld + 1) * kRowStep);
+
+// Four values of a row as they lie there: neighbouring lanes load and store what lies side by side.
 template <bool kBf16>
-__device__ __forceinline__ void load8(const void* row, int at, int vocab, float (&x)[8]) {
-  if (at + 8 <= vocab) {
-    if constexpr (kBf16) {
-      const loose_u32x4 raw =
-          *reinterpret_cast<const loose_u32x4*>(static_cast<const uint16_t*>(row) + at);
+struct Pack {
+  static constexpr int kBytes = kBf16 ? 2 : 4;  // of a value
+  uint32_t raw[kBytes];
+  __device__ __forceinline__ void load(const void* row, int at) {
+    typedef uint32_t __attribute__((ext_vector_type(kBytes), aligned(2))) Loose;
+    const Loose x =
+        *reinterpret_cast<const Loose*>(static_cast<const char*>(row) + int64_t(at) * kBytes);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = bf16_lo(raw[j]);
-        x[2 * j + 1] = bf16_hi(raw[j]);
-      }
-    } else {
+    for (int j = 0; j < kBytes; ++j) raw[j] = x[j];
+  }
+  // Past the end -inf.
+  __device__ __forceinline__ void load(const void* row, int at, int vocab) {
+    if (at + 4 <= vocab) return load(row, at);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const loose_f32x4 raw =
-            *reinterpret_cast<const loose_f32x4*>(static_cast<const float*>(row) + at + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * h + j] = raw[j];
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kBf16) {
+        const uint32_t x = at + j < vocab ? static_cast<const uint16_t*>(row)[at + j] : 0xFF80u;
+        raw[j / 2] = j % 2 ? raw[j / 2] | x << 16 : x;
+      } else {
+        raw[j] = at + j < vocab ? static_cast<const uint32_t*>(row)[at + j] : 0xFF800000u;
       }
     }
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (!kBf16)
+      return __uint_as_float(raw[j]);
+    else
+      return j % 2 ? bf16_hi(raw[j / 2]) : bf16_lo(raw[j / 2]);
+  }
+};
+__device__ __forceinline__ void store4(float* row, int at, int vocab, const float (&x)[4]) {
+  if (at + 4 <= vocab) {
+    *reinterpret_cast<loose_f32x4*>(row + at) = loose_f32x4{x[0], x[1], x[2], x[3]};
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = -kInf;
-    if (at + j < vocab)
-      x[j] = kBf16 ? bf16_to_f32(static_cast<const uint16_t*>(row)[at + j])
-                   : static_cast<const float*>(row)[at + j];
-  }
-}
-__device__ __forceinline__ void store8(float* row, int at, int vocab, const float (&x)[8]) {
-  if (at + 8 <= vocab) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<loose_f32x4*>(row + at + 4 * h) =
-          loose_f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 4; ++j)
     if (at + j < vocab) row[at + j] = x[j];
 }
 
@@ -96,153 +102,200 @@ __device__ __forceinline__ float inverse_of(float temperature) {
                           : __builtin_nanf("");
 }
 
-// What a part of a row adds up to: its largest logit, and the sum of the weights against it (against
+// Workgroup (token, part of `length` values). A thread holds kHeld packs, and one more that may pass the
+// end or be of any further step; others between are loaded for each use.
+template <bool kBf16, int kHeld>
+__global__ void __launch_bounds__(kRowThreads) probs_kernel(const ProbsArgs p, int length, int parts) {
+  __shared__ float room[kRowThreads / 64];
+  const int token = blockIdx.x / parts, part = blockIdx.x % parts;
+  const void* const row =
+      static_cast<const char*>(p.logits) + token * p.logit_stride * (kBf16 ? 2 : 4);
+  float* const out = p.probs + token * p.prob_stride;
+  const float temperature = p.temperature ? p.temperature[token] : 1.f;
+  const int vocab = p.vocab, mine = kPackValues * int(threadIdx.x);
+  const int whole = vocab / kRowStep;  // steps that do not pass the end
+  Pack<kBf16> held[kHeld], last;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (i < whole) held[i].load(row, mine + i * kRowStep);
+  last.load(row, mine + whole * kRowStep, vocab);
+  // f(values, place) of all packs of the thread.
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i < whole) f(held[i], mine + i * kRowStep);
+    for (int i = kHeld; i < whole; ++i) {
+      Pack<kBf16> x;
+      x.load(row, mine + i * kRowStep);
+      f(x, mine + i * kRowStep);
+    }
+    f(last, mine + whole * kRowStep);
+  };
+  float top = -kInf;
+  each([&](const Pack<kBf16>& x, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, x[j]);
+  });
+  top = reduce_all<kRowThreads>(top, room, larger);
+  const int begin = part * length, end = min(begin + length, vocab);
+  if (temperature == 0) {
+    // 1 at the first of the largest; NaN if any logit is, nothing where none is above -inf.
+    int first = 0x7FFFFFFF;
+    each([&](const Pack<kBf16>& x, int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (x[j] == top && top > -kInf) first = min(first, at + j);  // past the end is -inf
+        if (x[j] != x[j]) first = -1;
+      }
+    });
+    first = reduce_all<kRowThreads>(first, reinterpret_cast<int*>(room), smaller);
+    for (int at = begin + mine; at < end; at += kRowStep) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = first < 0 ? __builtin_nanf("") : at + j == first ? 1.f : 0.f;
+      store4(out, at, vocab, y);
+    }
+    return;
+  }
+  // Where nothing is above -inf all weights are 0. +inf gives NaN, as inf - inf is.
+  const float c = inverse_of(temperature), against = top == -kInf ? 0.f : top;
+  float sums[2] = {0, 0};
+  each([&](const Pack<kBf16>& x, int) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[j % 2] += __builtin_amdgcn_exp2f((x[j] - against) * c);
+  });
+  const float sum = reduce_all<kRowThreads>(sums[0] + sums[1], room, add<float>);
+  const float scale = sum == 0 ? 0.f : 1.f / sum;
+  each([&](const Pack<kBf16>& x, int at) __attribute__((always_inline)) {
+    if (at - mine < begin || at - mine >= end) return;
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_exp2f((x[j] - against) * c) * scale;
+    store4(out, at, vocab, y);
+  });
+}
+
+// What a chunk of a row adds up to: its largest logit, and the sum of the weights against it (against
 // 0 where nothing is above -inf, so that all are 0); at temperature 0 the place of the first that is
-// largest (negative if a logit is NaN, past all places if nothing is above -inf).
+// largest: negative if a logit is NaN, past all places if nothing is above -inf.
 struct RowPart {
   float top, sum;
 };
 __device__ __forceinline__ float against(float top) { return top == -kInf ? 0.f : top; }
-// Weights of 8 logits against `top`, c as above. +inf is NaN, as inf - inf is.
-__device__ __forceinline__ float weigh8(float (&x)[8], float top, float c) {
-  float s[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = __builtin_amdgcn_exp2f((x[j] - top) * c);
-    s[j % 2] += x[j];
-  }
-  return s[0] + s[1];
-}
 
-template <bool kBf16, int kThreads>
-__device__ __forceinline__ RowPart row_part(const void* row, int begin, int end, float temperature,
-                                            float* room) {
-  RowPart part;
-  float top = -kInf;
-  bool nan = false;
-  float x[8];
-  for (int at = begin + 8 * int(threadIdx.x); at < end; at += 8 * kThreads) {
-    load8<kBf16>(row, at, end, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      top = fmaxf(top, x[j]);
-      nan = nan || x[j] != x[j];
-    }
-  }
-  top = reduce_all<kThreads>(top, room, larger);
-  part.top = top;
-  if (temperature == 0) {
-    int first = 0x7FFFFFFF;
-    for (int at = begin + 8 * int(threadIdx.x); at < end; at += 8 * kThreads) {
-      load8<kBf16>(row, at, end, x);
-#pragma unroll
-      for (int j = 7; j >= 0; --j)
-        if (x[j] == top && top > -kInf) first = min(first, at + j);
-    }
-    first = reduce_all<kThreads>(nan ? -1 : first, reinterpret_cast<int*>(room), smaller);
-    part.sum = __int_as_float(first);
-    return part;
-  }
-  const float c = inverse_of(temperature);
-  float sum = 0;
-  for (int at = begin + 8 * int(threadIdx.x); at < end; at += 8 * kThreads) {
-    load8<kBf16>(row, at, end, x);
-    sum += weigh8(x, against(top), c);
-  }
-  part.sum = reduce_all<kThreads>(sum, room, add<float>);
-  return part;
-}
-
-// Writes [begin, end) of a row: of weights against `top`, whose sum over the row is `sum`; at
-// temperature 0 1 at `first`.
-template <bool kBf16, int kThreads>
-__device__ __forceinline__ void write_part(const ProbsArgs& p, const void* row, int token, int begin,
-                                           int end, float temperature, const RowPart& all) {
-  float* const out = p.probs + token * p.prob_stride;
-  const bool greedy = temperature == 0;
-  const int first = __float_as_int(all.sum);
-  const float c = inverse_of(temperature);
-  // Where nothing is above -inf, all weights are 0 and so is their sum.
-  const float scale = greedy ? 0.f : all.sum == 0 ? 0.f : 1.f / all.sum;
-  float x[8];
-  for (int at = begin + 8 * int(threadIdx.x); at < end; at += 8 * kThreads) {
-    load8<kBf16>(row, at, end, x);
-    if (greedy) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = first < 0 ? __builtin_nanf("") : at + j == first ? 1.f : 0.f;
-    } else {
-      weigh8(x, against(all.top), c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= scale;
-    }
-    store8(out, at, end, x);
-  }
-}
-
+// Workgroup (token, chunk). A thread has kChunkPacks packs of it at most.
 template <bool kBf16>
-__device__ __forceinline__ const void* logit_row(const ProbsArgs& p, int token) {
-  return static_cast<const char*>(p.logits) + token * p.logit_stride * (kBf16 ? 2 : 4);
-}
-__device__ __forceinline__ float temperature_of(const ProbsArgs& p, int token) {
-  return p.temperature ? p.temperature[token] : 1.f;
-}
+struct ChunkOfRow {
+  int token, begin, end;
+  const void* row;
+  float temperature;
+  Pack<kBf16> held[kChunkPacks];
+  __device__ __forceinline__ ChunkOfRow(const ProbsArgs& p, int length, int chunks) {
+    token = blockIdx.x / chunks;
+    begin = int(blockIdx.x % chunks) * length;
+    end = min(begin + length, p.vocab);
+    row = static_cast<const char*>(p.logits) + token * p.logit_stride * (kBf16 ? 2 : 4);
+    temperature = p.temperature ? p.temperature[token] : 1.f;
+    begin += kPackValues * int(threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < kChunkPacks; ++i) held[i].load(row, at(i), end);
+  }
+  __device__ __forceinline__ int at(int i) const { return begin + i * kSampleThreads * kPackValues; }
+};
 
-// Workgroup (token, chunk): the chunk's part goes to the workspace.
 template <bool kBf16>
 __global__ void __launch_bounds__(kSampleThreads)
     probs_parts_kernel(const ProbsArgs p, int length, int chunks) {
   __shared__ float room[kSampleThreads / 64];
-  const int token = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int begin = chunk * length, end = min(begin + length, p.vocab);
-  const RowPart part = row_part<kBf16, kSampleThreads>(logit_row<kBf16>(p, token), begin, end,
-                                                       temperature_of(p, token), room);
+  const ChunkOfRow<kBf16> chunk(p, length, chunks);
+  float top = -kInf;
+#pragma unroll
+  for (int i = 0; i < kChunkPacks; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, chunk.held[i][j]);
+  RowPart part;
+  part.top = top = reduce_all<kSampleThreads>(top, room, larger);
+  if (chunk.temperature == 0) {
+    int first = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = 0; i < kChunkPacks; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = chunk.held[i][j];
+        if (x == top && top > -kInf) first = min(first, chunk.at(i) + j);
+        if (x != x) first = -1;
+      }
+    part.sum = __int_as_float(
+        reduce_all<kSampleThreads>(first, reinterpret_cast<int*>(room), smaller));
+  } else {
+    const float c = inverse_of(chunk.temperature);
+    float sums[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kChunkPacks; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        sums[j % 2] += __builtin_amdgcn_exp2f((chunk.held[i][j] - against(top)) * c);
+    part.sum = reduce_all<kSampleThreads>(sums[0] + sums[1], room, add<float>);
+  }
   if (threadIdx.x == 0) reinterpret_cast<RowPart*>(p.workspace)[blockIdx.x] = part;
 }
 
-// Joins the parts of the row and writes the chunk.
+// Joins the chunks' parts in each of them, and writes it.
 template <bool kBf16>
 __global__ void __launch_bounds__(kSampleThreads)
     probs_write_kernel(const ProbsArgs p, int length, int chunks) {
   __shared__ float room[kSampleThreads / 64];
-  const int token = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int begin = chunk * length, end = min(begin + length, p.vocab);
-  const float temperature = temperature_of(p, token);
-  const RowPart* parts = reinterpret_cast<const RowPart*>(p.workspace) + int64_t(token) * chunks;
-  RowPart all;
-  float top = -kInf;
-  for (int i = threadIdx.x; i < chunks; i += kSampleThreads) top = fmaxf(top, parts[i].top);
-  all.top = top = reduce_all<kSampleThreads>(top, room, larger);
-  if (temperature == 0) {
+  const ChunkOfRow<kBf16> chunk(p, length, chunks);
+  const RowPart* parts = reinterpret_cast<const RowPart*>(p.workspace) + int64_t(chunk.token) * chunks;
+  RowPart mine = {-kInf, 0.f};  // chunks are no more than threads
+  if (int(threadIdx.x) < chunks) mine = parts[threadIdx.x];
+  const float top = reduce_all<kSampleThreads>(mine.top, room, larger);
+  float* const out = p.probs + chunk.token * p.prob_stride;
+  float y[4];
+  if (chunk.temperature == 0) {
+    const int place = __float_as_int(mine.sum);
     int first = 0x7FFFFFFF;
-    for (int i = threadIdx.x; i < chunks; i += kSampleThreads) {
-      const int at = __float_as_int(parts[i].sum);
-      if (at < 0 || parts[i].top == top) first = min(first, at);
+    if (int(threadIdx.x) < chunks && (place < 0 || mine.top == top)) first = place;
+    first = reduce_all<kSampleThreads>(first, reinterpret_cast<int*>(room), smaller);
+#pragma unroll
+    for (int i = 0; i < kChunkPacks; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        y[j] = first < 0 ? __builtin_nanf("") : chunk.at(i) + j == first ? 1.f : 0.f;
+      store4(out, chunk.at(i), chunk.end, y);
     }
-    all.sum = __int_as_float(
-        reduce_all<kSampleThreads>(first, reinterpret_cast<int*>(room), smaller));
-  } else {
-    const float c = inverse_of(temperature);
-    float sum = 0;
-    for (int i = threadIdx.x; i < chunks; i += kSampleThreads)
-      if (parts[i].sum != 0)
-        sum += parts[i].sum * __builtin_amdgcn_exp2f((parts[i].top - against(top)) * c);
-    all.sum = reduce_all<kSampleThreads>(sum, room, add<float>);
+    return;
   }
-  write_part<kBf16, kSampleThreads>(p, logit_row<kBf16>(p, token), token, begin, end, temperature, all);
-}
-
-// A workgroup a row.
-template <bool kBf16>
-__global__ void __launch_bounds__(kRowThreads) probs_rows_kernel(const ProbsArgs p) {
-  __shared__ float room[kRowThreads / 64];
-  const int token = blockIdx.x;
-  const void* const row = logit_row<kBf16>(p, token);
-  const float temperature = temperature_of(p, token);
-  const RowPart all = row_part<kBf16, kRowThreads>(row, 0, p.vocab, temperature, room);
-  write_part<kBf16, kRowThreads>(p, row, token, 0, p.vocab, temperature, all);
+  const float c = inverse_of(chunk.temperature);
+  float sum = mine.sum;
+  if (sum != 0) sum *= __builtin_amdgcn_exp2f((mine.top - against(top)) * c);
+  sum = reduce_all<kSampleThreads>(sum, room, add<float>);
+  const float scale = sum == 0 ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < kChunkPacks; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      y[j] = __builtin_amdgcn_exp2f((chunk.held[i][j] - against(top)) * c) * scale;
+    store4(out, chunk.at(i), chunk.end, y);
+  }
 }
 
 // ---- verify_drafts ----------------------------------------------------------------------
+//
+// Which drafts stand takes one value of p and q a row, all loaded at once, a row a lane; a vocabulary is
+// read where none stands any more, and between the children of a drafter's row. Weights, sums and
+// comparisons are in 64 bits: a running sum over 150000 values in 32 would lose tokens of less than 6e-8
+// of it.
+//
+// Chains and certain choices need sums at the end alone: every wave follows its sequence and adds up a
+// chunk of what is left, then a second kernel finds the chunk and the token. 64 chains of 9 over 152000
+// tokens 22.4 us: the sums 16.5 (78 MB, 4.7 TB/s), the token 8.3, a chain of dependent loads.
+//
+// Trees of a drafter's tokens need a sum for every child but the last that fails. Several workgroups
+// share a sequence: all follow it, each sums its chunk, and sums go from one to the others through the
+// workspace, which a first kernel fills with what is no sum. A workgroup that waits in vain (another may
+// not run yet) adds up the missing chunks itself, so every wait ends, and to the same result. 16 trees
+// of 32 rows over 128000 tokens 29.6 us, 3 to 4 a sum; with one workgroup a sequence 62.7.
 
 constexpr float kMostUniform = 1 - 0x1p-24f;  // the largest number below 1
 
@@ -258,7 +311,7 @@ __device__ __forceinline__ int token_of(const VerifyArgs& p, int row) {
 struct Stop {
   double taken;       // times the drafter's row
   uint64_t rejected;  // rows whose tokens have none
-  int row, pad;
+  int row;
 };
 constexpr int kMostRows = 64;
 
@@ -326,95 +379,6 @@ __device__ __forceinline__ double at_lane(double v, int lane) {
   return __builtin_bit_cast(double, int64_t(uint64_t(high) << 32 | low));
 }
 
-// Follows sequence rows.begin .. as far as its drafts stand. Every wave does so, and all come to the
-// same. kSums: a row may have several children of a drafter's row, so sums over it are needed.
-// path: in lane i the i-th accepted row.
-template <int kThreads, bool kSums>
-__device__ __forceinline__ Stop follow(const VerifyArgs& p, const Rows& rows, int lane, int& path,
-                                       int& accepted, int& token, double* room) {
-  const int count = min(rows.count, kMostRows), row = rows.begin + lane;
-  int parent = -1;
-  float pt = 0, qt = 0, u = 0;
-  token = -1;
-  if (lane < count) {
-    u = fminf(fmaxf(p.uniforms[row], 0.f), kMostUniform);
-    if (lane > 0) {
-      parent = p.parents ? p.parents[row] : lane - 1;
-      if (parent >= lane) parent = -1;
-      token = token_of(p, row);
-    }
-    if (parent >= 0 && token >= 0) {
-      pt = clean(p.target[(rows.begin + parent) * p.target_stride + token]);
-      if (p.draft) qt = clean(p.draft[(rows.begin + parent) * p.draft_stride + token]);
-    }
-  }
-  Stop stop = {0.0, 0, 0, 0};
-  double left = 1;
-  path = lane == 0 ? 0 : -1;
-  accepted = 1;
-  uint64_t children = __ballot(parent == 0);
-  while (children) {
-    const int i = __builtin_ctzll(children);
-    children &= children - 1;
-    const double number = at_lane(double(u), i), q = at_lane(double(qt), i);
-    double w = at_lane(double(pt), i);
-    bool stands;
-    if (p.draft) {
-      w = fmax(w - stop.taken * q, 0.0);
-      stands = number * (left * q) < w;
-    } else {
-      const int id = __builtin_amdgcn_readlane(token, i);
-      if (__ballot((stop.rejected >> lane & 1) && token == id)) w = 0;
-      stands = number * left < w;
-    }
-    if (stands) {
-      if (lane == accepted) path = i;
-      ++accepted;
-      stop = {0.0, 0, i, 0};
-      left = 1;
-      children = __ballot(parent == i);
-    } else if (p.draft) {
-      stop.taken += left;
-      if (kSums && children) {
-        const int64_t at = rows.begin + stop.row;
-        const Weights weights = {p.target + at * p.target_stride, p.draft + at * p.draft_stride,
-                                 stop.taken, nullptr, 0};
-        left = sum_weights<kThreads>(weights, 0, p.vocab, room);
-      }
-    } else {
-      left -= w;
-      stop.rejected |= uint64_t(1) << i;
-    }
-  }
-  return stop;
-}
-
-// One wave: what is known of the sequence before any vocabulary is read.
-__device__ __forceinline__ void write_path(const VerifyArgs& p, const Rows& rows, int seq, int lane,
-                                           int path, int accepted) {
-  for (int i = lane; i < rows.count; i += 64) p.path[rows.begin + i] = i == lane ? path : -1;
-  if (lane == 0) p.accepted[seq] = rows.count ? accepted : 0;
-}
-
-// The workspace: a sum for each chunk of each sequence, then the stops.
-__device__ __forceinline__ double* chunk_sums(const VerifyArgs& p) {
-  return static_cast<double*>(p.workspace);
-}
-__device__ __forceinline__ Stop* stops(const VerifyArgs& p, int chunks) {
-  return reinterpret_cast<Stop*>(chunk_sums(p) + int64_t(p.seqs) * chunks);
-}
-
-// Trees of a drafter's tokens: a workgroup a sequence follows it.
-__global__ void __launch_bounds__(kRowThreads) verify_follow_kernel(const VerifyArgs p, int chunks) {
-  __shared__ double room[kRowThreads / 64];
-  const int seq = blockIdx.x, lane = threadIdx.x & 63;
-  const Rows rows = rows_of(p, seq);
-  int path, accepted, token;
-  const Stop stop = follow<kRowThreads, true>(p, rows, lane, path, accepted, token, room);
-  if (threadIdx.x < 64) write_path(p, rows, seq, lane, path, accepted);
-  if (threadIdx.x == 0) stops(p, chunks)[seq] = stop;
-}
-
 // Tokens of rejected rows in [begin, end) to `skip`; how many.
 __device__ __forceinline__ int skipped(uint64_t rejected, int token, int lane, int begin, int end,
                                        int* skip) {
@@ -422,40 +386,6 @@ __device__ __forceinline__ int skipped(uint64_t rejected, int token, int lane, i
   const uint64_t all = __ballot(mine);
   if (mine) skip[__builtin_popcountll(all & ((uint64_t(1) << lane) - 1))] = token;
   return __builtin_popcountll(all);
-}
-
-__device__ __forceinline__ Weights weights_at(const VerifyArgs& p, const Rows& rows, const Stop& stop,
-                                              const int* skip, int skips) {
-  const int64_t at = rows.begin + stop.row;
-  return {p.target + at * p.target_stride, stop.taken > 0 ? p.draft + at * p.draft_stride : nullptr,
-          stop.taken, skip, skips};
-}
-
-// Workgroup (sequence, chunk): the sum of the chunk's weights where the sequence stops. kFollowed: that
-// is known.
-template <bool kFollowed>
-__global__ void __launch_bounds__(kSampleThreads)
-    verify_sums_kernel(const VerifyArgs p, int length, int chunks) {
-  __shared__ double room[kSampleThreads / 64];
-  __shared__ int skip[kSampleThreads / 64][kMostRows];
-  const int seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x & 63;
-  const Rows rows = rows_of(p, seq);
-  Stop stop;
-  int token = -1;
-  if (kFollowed) {
-    stop = stops(p, chunks)[seq];
-  } else {
-    int path, accepted;
-    stop = follow<kSampleThreads, false>(p, rows, lane, path, accepted, token, room);
-    if (chunk == 0 && threadIdx.x < 64) write_path(p, rows, seq, lane, path, accepted);
-    if (chunk == 0 && threadIdx.x == 0) stops(p, chunks)[seq] = stop;
-  }
-  if (rows.count == 0) return;
-  const int begin = chunk * length, end = min(begin + length, p.vocab), wave = threadIdx.x >> 6;
-  const int skips = skipped(stop.rejected, token, lane, begin, end, skip[wave]);
-  const double sum =
-      sum_weights<kSampleThreads>(weights_at(p, rows, stop, skip[wave], skips), begin, end, room);
-  if (threadIdx.x == 0) chunk_sums(p)[blockIdx.x] = sum;
 }
 
 // Inclusive sums over the workgroup's threads.
@@ -478,10 +408,9 @@ __device__ __forceinline__ double scan_all(double v, double* room) {
 // anything; -1 if none does. before: the sum in front of it.
 template <int kThreads>
 __device__ __forceinline__ int first_past(double mine, double bar, double& before, double* room,
-                                          int* places, bool share) {
+                                          int* places) {
   const double sum = scan_all<kThreads>(mine, room);
-  const double total = share ? bar * reduce_all<kThreads>(mine, room, add<double>) : bar;
-  const int past = sum > total && mine > 0 ? int(threadIdx.x) : 0x7FFFFFFF;
+  const int past = sum > bar && mine > 0 ? int(threadIdx.x) : 0x7FFFFFFF;
   int found = reduce_all<kThreads>(past, places, smaller);
   if (found == 0x7FFFFFFF) {
     const int last = mine > 0 ? -int(threadIdx.x) : 1;
@@ -489,114 +418,346 @@ __device__ __forceinline__ int first_past(double mine, double bar, double& befor
     found = found > 0 ? -1 : -found;
   }
   __syncthreads();
-  if (int(threadIdx.x) == found) room[0] = sum - mine, room[1] = total;
+  if (int(threadIdx.x) == found) room[0] = sum - mine;
   __syncthreads();
   before = found < 0 ? 0 : room[0];
   return found;
 }
 
-// The first token of [begin, end) whose running sum of weights passes `bar` (share: `bar` times their
-// sum); -1 where no token has a weight.
-template <int kThreads>
-__device__ __forceinline__ int pick(const Weights& weights, int begin, int end, double bar, bool share,
-                                    double* room, int* places) {
-  const int each = ((end - begin + kThreads - 1) / kThreads + 3) / 4 * 4;
-  const int first = min(begin + each * int(threadIdx.x), end), last = min(first + each, end);
-  double mine = 0, w[4];
-  for (int at = first; at < last; at += 4) {
-    weights.load(at, last, w);
-    mine += (w[0] + w[1]) + (w[2] + w[3]);
-  }
-  double before;
-  const int found = first_past<kThreads>(mine, bar, before, room, places, share);
-  if (found < 0) return -1;
-  const double level = room[1];
-  if (int(threadIdx.x) == found) {
-    int token = -1;
-    bool past = false;
-    for (int at = first; at < last && !past; at += 4) {
-      weights.load(at, last, w);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        before += w[j];
-        if (!past && w[j] > 0) {
-          token = at + j;
-          past = before > level;
-        }
-      }
-    }
-    places[0] = token;
-  }
-  __syncthreads();
-  return places[0];
+// One wave: what is known of the sequence before any vocabulary is read.
+__device__ __forceinline__ void write_path(const VerifyArgs& p, const Rows& rows, int seq, int lane,
+                                           int path, int accepted) {
+  for (int i = lane; i < rows.count; i += 64) p.path[rows.begin + i] = i == lane ? path : -1;
+  if (lane == 0) p.accepted[seq] = rows.count ? accepted : 0;
 }
 
-// A workgroup a sequence: the chunk that the number falls in, then the token.
-__global__ void __launch_bounds__(kRowThreads)
+constexpr uint64_t kNoSum = ~uint64_t(0);  // a NaN, which no sum is
+
+__global__ void __launch_bounds__(kClearThreads) verify_clear_kernel(uint64_t* sums, int count) {
+  const int i = blockIdx.x * kClearThreads + threadIdx.x;
+  if (i < count) sums[i] = kNoSum;
+}
+
+// A chunk of a sequence's vocabulary, and the sums of all its chunks.
+template <int kThreads>
+struct Cluster {
+  int seq, chunk, chunks, length, vocab;
+  uint64_t* shared_sums;  // of this sequence
+  double* room;           // LDS, a value a wave
+  double* sums;           // LDS, a value a chunk: the last sums
+  int* missing;           // LDS
+  int round;
+
+  __device__ __forceinline__ int begin(int i) const { return i * length; }
+  __device__ __forceinline__ int end(int i) const { return min(i * length + length, vocab); }
+
+  // The sum of weights over the vocabulary. weights_in(begin, end) gives those of a chunk.
+  template <typename F>
+  __device__ __forceinline__ double total(F weights_in) {
+    const double own = sum_weights<kThreads>(weights_in(begin(chunk), end(chunk)), begin(chunk),
+                                             end(chunk), room);
+    if (chunks == 1) {
+      if (threadIdx.x == 0) sums[0] = own;
+      __syncthreads();
+      return own;
+    }
+    uint64_t* const slots = shared_sums + round * chunks;
+    ++round;
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(slots + chunk, __builtin_bit_cast(uint64_t, own), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      *missing = 0;
+    }
+    __syncthreads();
+    if (int(threadIdx.x) < chunks) {
+      uint64_t bits = kNoSum;
+      for (int i = 0; i < kMostPolls && bits == kNoSum; ++i) {
+        bits = __hip_atomic_load(slots + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (bits == kNoSum) __builtin_amdgcn_s_sleep(1);
+      }
+      sums[threadIdx.x] = __builtin_bit_cast(double, bits);
+      if (bits == kNoSum) *missing = 1;
+    }
+    __syncthreads();
+    if (*missing) {
+      for (int i = 0; i < chunks; ++i) {
+        if (__builtin_bit_cast(uint64_t, sums[i]) != kNoSum) continue;
+        const double sum = sum_weights<kThreads>(weights_in(begin(i), end(i)), begin(i), end(i), room);
+        __syncthreads();
+        if (threadIdx.x == 0) sums[i] = sum;
+        __syncthreads();
+      }
+    }
+    double mine = 0;
+    if (int(threadIdx.x) < chunks) mine = sums[threadIdx.x];
+    return reduce_all<kThreads>(mine, room, add<double>);
+  }
+};
+
+// A sequence, as far as its drafts stand. Lane l has row l: its parent, its token and, in the lane's
+// values, what the parent's rows have for it.
+struct Followed {
+  Stop stop;
+  double number;       // of row 0
+  int token;           // of the lane's row
+  int path, accepted;  // path: in lane i the i-th accepted row
+};
+// Every wave of every workgroup that needs it follows the sequence, and all come to the same.
+// left_after(stop, token): what is left of a drafter's row at a stop; only trees of its tokens ask.
+template <typename F>
+__device__ __forceinline__ Followed follow(const VerifyArgs& p, const Rows& rows, int lane,
+                                           F left_after) {
+  const int count = min(rows.count, kMostRows), row = rows.begin + lane;
+  int parent = -1;
+  float pt = 0, qt = 0, u = 0;
+  Followed x = {{0.0, 0, 0}, 0.0, -1, lane == 0 ? 0 : -1, 1};
+  if (lane < count) {
+    u = fminf(fmaxf(p.uniforms[row], 0.f), kMostUniform);
+    if (lane > 0) {
+      parent = p.parents ? p.parents[row] : lane - 1;
+      if (parent >= lane) parent = -1;
+      x.token = token_of(p, row);
+    }
+    if (parent >= 0 && x.token >= 0) {
+      pt = clean(p.target[(rows.begin + parent) * p.target_stride + x.token]);
+      if (p.draft) qt = clean(p.draft[(rows.begin + parent) * p.draft_stride + x.token]);
+    }
+  }
+  x.number = at_lane(double(u), 0);
+  double left = 1;
+  uint64_t children = __ballot(parent == 0);
+  while (children) {
+    const int i = __builtin_ctzll(children);
+    children &= children - 1;
+    const double number = at_lane(double(u), i), q = at_lane(double(qt), i);
+    double w = at_lane(double(pt), i);
+    bool stands;
+    if (p.draft) {
+      w = fmax(w - x.stop.taken * q, 0.0);
+      stands = number * (left * q) < w;
+    } else {
+      const int id = __builtin_amdgcn_readlane(x.token, i);
+      if (__ballot((x.stop.rejected >> lane & 1) && x.token == id)) w = 0;
+      stands = number * left < w;
+    }
+    if (stands) {
+      if (lane == x.accepted) x.path = i;
+      ++x.accepted;
+      x.stop = {0.0, 0, i};
+      left = 1;
+      children = __ballot(parent == i);
+    } else if (p.draft) {
+      x.stop.taken += left;
+      if (children) left = left_after(x.stop, x.token);
+    } else {
+      left -= w;
+      x.stop.rejected |= uint64_t(1) << i;
+    }
+  }
+  return x;
+}
+
+// Weights at a stop in [begin, end); skip: room of the wave for tokens that have none.
+__device__ __forceinline__ Weights weights_at(const VerifyArgs& p, const Rows& rows, const Stop& stop,
+                                              int token, int lane, int begin, int end, int* skip) {
+  const int64_t at = rows.begin + stop.row;
+  const int skips = skipped(stop.rejected, token, lane, begin, end, skip);
+  return {p.target + at * p.target_stride, stop.taken > 0 ? p.draft + at * p.draft_stride : nullptr,
+          stop.taken, skip, skips};
+}
+
+// Writes the first token of [begin, end) whose running sum of weights passes `level`, or the last that
+// has a weight; -1 if none has. One workgroup alone writes a sequence's: stores of two would meet in
+// different L2s.
+template <int kThreads>
+__device__ __forceinline__ void pick(const Weights& weights, int begin, int end, double level,
+                                     double* room, int* places, int64_t* next) {
+  const int each = ((end - begin + kThreads - 1) / kThreads + 3) / 4 * 4;
+  const int first = min(begin + each * int(threadIdx.x), end), last = min(first + each, end);
+  double part = 0, w[4];
+  for (int at = first; at < last; at += 4) {
+    weights.load(at, last, w);
+    part += (w[0] + w[1]) + (w[2] + w[3]);
+  }
+  double sum;
+  const int found = first_past<kThreads>(part, level, sum, room, places);
+  int token = -1;
+  if (int(threadIdx.x) != max(found, 0)) return;
+  bool past = found < 0;
+  for (int at = first; at < last && !past; at += 4) {
+    weights.load(at, last, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum += w[j];
+      if (!past && w[j] > 0) {
+        token = at + j;
+        past = sum > level;
+      }
+    }
+  }
+  *next = token;
+}
+
+// Workgroup (sequence, chunk), where sums may be needed on the way, or a workgroup has it all.
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
+    verify_cluster_kernel(const VerifyArgs p, int length, int chunks, int rounds) {
+  constexpr int kWaves = kThreads / 64;
+  __shared__ double room[kWaves], sums[kMostChunks];
+  __shared__ int places[kWaves], missing, skip[kWaves][kMostRows];
+  const int seq = blockIdx.x / chunks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Cluster<kThreads> cluster = {seq, int(blockIdx.x % chunks), chunks, length, p.vocab,
+                               static_cast<uint64_t*>(p.workspace) + int64_t(seq) * rounds * chunks,
+                               room, sums, &missing, 0};
+  const Rows rows = rows_of(p, seq);
+  auto total = [&](const Stop& stop, int token) {
+    return cluster.total([&](int begin, int end) {
+      return weights_at(p, rows, stop, token, lane, begin, end, skip[wave]);
+    });
+  };
+  Followed x = follow(p, rows, lane, total);
+  if (cluster.chunk == 0 && wave == 0) write_path(p, rows, seq, lane, x.path, x.accepted);
+  auto none = [&]() {
+    if (cluster.chunk == 0 && threadIdx.x == 0) p.next[seq] = -1;
+  };
+  if (rows.count == 0) return none();
+
+  // The chunk that the first row's number falls in, then the token. Where no weight is left, the
+  // target's own.
+  double all = total(x.stop, x.token);
+  if (all == 0 && (x.stop.taken > 0 || x.stop.rejected)) {
+    x.stop.taken = 0;
+    x.stop.rejected = 0;
+    all = total(x.stop, x.token);
+  }
+  if (all == 0) return none();
+  const double bar = x.number * all;
+  double before = 0;
+  if (chunks > 1) {
+    const double mine = int(threadIdx.x) < chunks ? sums[threadIdx.x] : 0;
+    if (first_past<kThreads>(mine, bar, before, room, places) != cluster.chunk) return;
+  }
+  const int begin = cluster.begin(cluster.chunk), end = cluster.end(cluster.chunk);
+  const Weights weights = weights_at(p, rows, x.stop, x.token, lane, begin, end, skip[wave]);
+  pick<kThreads>(weights, begin, end, bar - before, room, places, p.next + seq);
+}
+
+// Chains, and certain choices: sums are needed at the end alone, so a second kernel joins them. A wave
+// adds up a chunk; the workspace has a sum for each, then the stops.
+__device__ __forceinline__ Stop* stops(const VerifyArgs& p, int chunks) {
+  return reinterpret_cast<Stop*>(static_cast<double*>(p.workspace) + int64_t(p.seqs) * chunks);
+}
+__global__ void __launch_bounds__(kSampleThreads)
+    verify_sums_kernel(const VerifyArgs p, int length, int chunks) {
+  __shared__ int skip[kSampleThreads / 64][kMostRows];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, index = blockIdx.x * (kSampleThreads / 64) + wave;
+  const int seq = index / chunks, chunk = index % chunks;
+  if (seq >= p.seqs) return;
+  const Rows rows = rows_of(p, seq);
+  const Followed x = follow(p, rows, lane, [](const Stop&, int) { return 0.0; });
+  if (chunk == 0) {
+    write_path(p, rows, seq, lane, x.path, x.accepted);
+    if (lane == 0) stops(p, chunks)[seq] = x.stop;
+  }
+  if (rows.count == 0) return;
+  const int begin = chunk * length, end = min(begin + length, p.vocab);
+  const Weights weights = weights_at(p, rows, x.stop, x.token, lane, begin, end, skip[wave]);
+  double sum = 0, w[4];
+#pragma unroll 4
+  for (int at = begin + 4 * lane; at < end; at += 256) {
+    weights.load(at, end, w);
+    sum += (w[0] + w[1]) + (w[2] + w[3]);
+  }
+#pragma unroll
+  for (int step = 32; step >= 1; step /= 2) sum += __shfl_xor(sum, step, 64);
+  if (lane == 0) static_cast<double*>(p.workspace)[index] = sum;
+}
+
+// A workgroup a sequence.
+__global__ void __launch_bounds__(kPickThreads)
     verify_pick_kernel(const VerifyArgs p, int length, int chunks) {
-  constexpr int kThreads = kRowThreads;
-  __shared__ double room[kThreads / 64];
-  __shared__ int places[kThreads / 64];
-  __shared__ int skip[kThreads / 64][kMostRows];
+  constexpr int kThreads = kPickThreads, kWaves = kThreads / 64;
+  __shared__ double room[kWaves];
+  __shared__ int places[kWaves], skip[kWaves][kMostRows];
   const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Rows rows = rows_of(p, seq);
   if (rows.count == 0) {
     if (threadIdx.x == 0) p.next[seq] = -1;
     return;
   }
-  const Stop stop = stops(p, chunks)[seq];
-  const double u = fminf(fmaxf(p.uniforms[rows.begin], 0.f), kMostUniform);
-  const double mine = int(threadIdx.x) < chunks ? chunk_sums(p)[int64_t(seq) * chunks + threadIdx.x] : 0;
-  double before;
-  const int chunk = first_past<kThreads>(mine, u, before, room, places, true);
-  int token;
-  if (chunk >= 0) {
-    const double bar = room[1] - before;
-    int id = -1;
-    if (stop.rejected >> lane & 1) id = token_of(p, rows.begin + lane);
-    const int begin = chunk * length, end = min(begin + length, p.vocab);
-    const int skips = skipped(stop.rejected, id, lane, begin, end, skip[wave]);
-    __syncthreads();
-    token = pick<kThreads>(weights_at(p, rows, stop, skip[wave], skips), begin, end, bar, false, room,
-                           places);
-  } else {
-    const Weights all = {p.target + (rows.begin + stop.row) * p.target_stride, nullptr, 0.0, nullptr, 0};
-    token = pick<kThreads>(all, 0, p.vocab, u, true, room, places);
+  const double mine = int(threadIdx.x) < chunks
+                          ? static_cast<const double*>(p.workspace)[int64_t(seq) * chunks + threadIdx.x]
+                          : 0;
+  Stop stop = stops(p, chunks)[seq];
+  const double number = fminf(fmaxf(p.uniforms[rows.begin], 0.f), kMostUniform);
+  int token = -1;
+  if (stop.rejected >> lane & 1) token = token_of(p, rows.begin + lane);
+  const double all = reduce_all<kThreads>(mine, room, add<double>);
+  double bar = number * all, before;
+  const int chunk = first_past<kThreads>(mine, bar, before, room, places);
+  int begin = chunk * length, end = min(begin + length, p.vocab);
+  if (chunk < 0) {
+    // Where no weight is left, the target's own.
+    begin = 0;
+    end = p.vocab;
+    stop.taken = 0;
+    stop.rejected = 0;
+    const Weights weights = weights_at(p, rows, stop, token, lane, begin, end, skip[wave]);
+    bar = number * sum_weights<kThreads>(weights, begin, end, room);
+    before = 0;
   }
-  if (threadIdx.x == 0) p.next[seq] = token;
+  const Weights weights = weights_at(p, rows, stop, token, lane, begin, end, skip[wave]);
+  pick<kThreads>(weights, begin, end, bar - before, room, places, p.next + seq);
 }
 
 }  // namespace
 
 hipError_t launch_token_probs(const ProbsArgs& args, bool bf16, hipStream_t stream) {
   if (args.tokens == 0) return hipSuccess;
-  if (args.tokens >= kManyRows) {
-    const auto kernel = bf16 ? probs_rows_kernel<true> : probs_rows_kernel<false>;
-    kernel<<<uint32_t(args.tokens), kRowThreads, 0, stream>>>(args);
+  const Chunks c = probs_chunks(args.tokens, args.vocab);
+  const uint32_t tokens = uint32_t(args.tokens);
+  if (probs_in_chunks(args.tokens, args.vocab, c, bf16)) {
+    const auto parts = bf16 ? probs_parts_kernel<true> : probs_parts_kernel<false>;
+    parts<<<tokens * c.count, kSampleThreads, 0, stream>>>(args, c.length, c.count);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const auto write = bf16 ? probs_write_kernel<true> : probs_write_kernel<false>;
+    write<<<tokens * c.count, kSampleThreads, 0, stream>>>(args, c.length, c.count);
     return hipGetLastError();
   }
-  const Chunks c = vocab_chunks(args.tokens, args.vocab);
-  const uint32_t grid = uint32_t(args.tokens) * c.count;
-  const auto parts = bf16 ? probs_parts_kernel<true> : probs_parts_kernel<false>;
-  parts<<<grid, kSampleThreads, 0, stream>>>(args, c.length, c.count);
-  if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  const auto write = bf16 ? probs_write_kernel<true> : probs_write_kernel<false>;
-  write<<<grid, kSampleThreads, 0, stream>>>(args, c.length, c.count);
+  // In place a row has one workgroup, which has read a value before it writes there.
+  const bool in_place = args.logits == args.probs;
+  const Chunks parts = in_place ? Chunks{args.vocab, 1} : probs_parts(args.tokens, args.vocab);
+  const bool few = args.vocab < kFewVocab;
+  const auto kernel = bf16 ? (few ? probs_kernel<true, kFewHeld> : probs_kernel<true, 40>)
+                           : (few ? probs_kernel<false, kFewHeld> : probs_kernel<false, 20>);
+  kernel<<<tokens * parts.count, kRowThreads, 0, stream>>>(args, parts.length, parts.count);
   return hipGetLastError();
 }
 
 hipError_t launch_verify_drafts(const VerifyArgs& args, hipStream_t stream) {
   if (args.seqs == 0) return hipSuccess;
-  const Chunks c = vocab_chunks(args.seqs, args.vocab);
-  const bool followed = args.draft && args.parents;
-  if (followed) {
-    verify_follow_kernel<<<uint32_t(args.seqs), kRowThreads, 0, stream>>>(args, c.count);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  const Chunks c = verify_chunks(args.seqs, args.vocab, args.draft && args.parents);
+  const uint32_t workgroups = uint32_t(args.seqs) * c.count;
+  if (c.count == 1) {
+    verify_cluster_kernel<kRowThreads>
+        <<<workgroups, kRowThreads, 0, stream>>>(args, c.length, 1, kMostRounds);
+    return hipGetLastError();
   }
-  const auto sums = followed ? verify_sums_kernel<true> : verify_sums_kernel<false>;
-  sums<<<uint32_t(args.seqs) * c.count, kSampleThreads, 0, stream>>>(args, c.length, c.count);
+  if (args.draft && args.parents) {
+    const int sums = args.seqs * c.count * kMostRounds;
+    verify_clear_kernel<<<(sums + kClearThreads - 1) / kClearThreads, kClearThreads, 0, stream>>>(
+        static_cast<uint64_t*>(args.workspace), sums);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    verify_cluster_kernel<kSampleThreads>
+        <<<workgroups, kSampleThreads, 0, stream>>>(args, c.length, c.count, kMostRounds);
+    return hipGetLastError();
+  }
+  constexpr int kWaves = kSampleThreads / 64;
+  verify_sums_kernel<<<(workgroups + kWaves - 1) / kWaves, kSampleThreads, 0, stream>>>(args, c.length,
+                                                                                       c.count);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  verify_pick_kernel<<<uint32_t(args.seqs), kRowThreads, 0, stream>>>(args, c.length, c.count);
+  verify_pick_kernel<<<uint32_t(args.seqs), kPickThreads, 0, stream>>>(args, c.length, c.count);
   return hipGetLastError();
 }
 

@@ -6,23 +6,67 @@
 namespace ci8 {
 
 constexpr int64_t kMostVocab = 1 << 24, kMostVerified = 1 << 14;
-constexpr int kSampleThreads = 256, kRowThreads = 1024;
+constexpr int kSampleThreads = 256, kRowThreads = 1024, kClearThreads = 256;
 constexpr int64_t kSamplingWorkspaceBytes = 1 << 20;
 
-// A vocabulary is cut into chunks of a multiple of 1024 tokens, 2048 at least, so that few rows are
-// about 1024 workgroups.
+// Parts of a row of `length` values.
 struct Chunks {
   int length, count;
 };
-inline Chunks vocab_chunks(int64_t rows, int64_t vocab) {
-  int64_t length = (rows * vocab + 1023) / 1024;
-  if (length > vocab) length = vocab;
-  if (length < 2048) length = 2048;
-  length = (length + 1023) / 1024 * 1024;
+
+// token_probs: whole multiples of what a workgroup's threads hold at once, as many as fill 256 CUs.
+constexpr int kProbsPart = 4096;
+inline Chunks probs_parts(int64_t tokens, int64_t vocab) {
+  const int64_t steps = (vocab + kProbsPart - 1) / kProbsPart;
+  int64_t parts = tokens < 256 ? 256 / tokens : 1;
+  if (parts > steps) parts = steps;
+  const int64_t each = (steps + parts - 1) / parts;
+  return {int(each * kProbsPart), int((steps + each - 1) / each)};
+}
+
+// Two kernels: chunks of a row of up to kChunkPacks * 1024 values, 256 of them at least where rows are
+// that long.
+constexpr int kChunkPacks = 8;
+inline Chunks probs_chunks(int64_t tokens, int64_t vocab) {
+  const int step = kSampleThreads * 4;
+  int64_t packs = tokens * vocab / step / 256;
+  if (packs < 1) packs = 1;
+  if (packs > kChunkPacks) packs = kChunkPacks;
+  const int64_t length = packs * step;
+  return {int(length), int((vocab + length - 1) / length)};
+}
+// Where they are faster, and their sums fit threads and workspace. us, chunks and whole rows, BF16: 1 x
+// 50001 8.1 and 9.5, 52 x 50001 10.0 and 13.5, 52 x 152000 13.3 and 24.5, 128 x 152000 26.6 and 34.3, 400 x
+// 50001 30.1 and 37.4; but 256 x 50001 19.4 and 18.0, 512 x 152000 124 and 110, 52 x 32000 8.8 and
+// 7.8. FP32: 128 x 152000 46 and 58, but 400 x 81000 75 and 59.
+constexpr int64_t kFewVocab = 9 * kProbsPart;
+inline bool probs_in_chunks(int64_t tokens, int64_t vocab, const Chunks& c, bool bf16) {
+  return vocab >= kFewVocab && (tokens < 192 || (bf16 && tokens > 256 && tokens < 512)) &&
+         c.count <= kSampleThreads && tokens * c.count * 8 <= kSamplingWorkspaceBytes;
+}
+
+// verify_drafts. With `rounds`, where sums may be needed after each row that fails and twice at the end:
+// a workgroup a chunk of 2048 tokens at least, about 1024 of all sequences, whose sums fit the workspace
+// for all rounds. Else a wave a chunk, four times as many. One chunk, and one workgroup, where the
+// vocabulary is small: us, one and several, 6 rows over 8000 tokens 9.5 and 11.2, 64 x 6 9.9 and 15.9; over
+// 16000 10.9 and 10.8, 12.7 and 12.3; over 32000 18.8 and 11.0.
+constexpr int kMostRounds = 64 + 2, kMostChunks = 256, kOneChunk = 10000, kPickThreads = 512;
+inline Chunks verify_chunks(int64_t seqs, int64_t vocab, bool rounds) {
+  if (vocab <= kOneChunk) return {int(vocab), 1};
+  int64_t count = (rounds ? 1024 : 4096) / seqs;
+  const int64_t fits = kSamplingWorkspaceBytes / 8 / (seqs * kMostRounds);
+  if (rounds && count > fits) count = fits;
+  if (count > kMostChunks) count = kMostChunks;
+  if (count > vocab / (rounds ? 2048 : 512)) count = vocab / (rounds ? 2048 : 512);
+  if (count <= 1) return {int(vocab), 1};
+  const int64_t length = ((vocab + count - 1) / count + 3) / 4 * 4;
   return {int(length), int((vocab + length - 1) / length)};
 }
 
-// token_probs: rows from here on take a workgroup each, which needs no workspace.
-constexpr int64_t kManyRows = 512;
+// Times that a workgroup looks for a sum of another, a microsecond or so each, before it computes it.
+#ifndef CI8_MOST_POLLS
+#define CI8_MOST_POLLS (1 << 14)
+#endif
+constexpr int kMostPolls = CI8_MOST_POLLS;
 
 }  // namespace ci8

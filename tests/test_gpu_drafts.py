@@ -137,7 +137,11 @@ def test_a_chain_is_what_attention_gives(attention, dim, group, count, window):
     want, want_lse = torch.empty_like(out), torch.empty_like(lse)
     attention.attention_fp4(q, *cache, dev(table), dev(np.int32(lens)), dev(starts), attention.new_workspace(dim), want,
                             want_lse, 0.1, count, window)
-    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    if group * count <= 128:  # the same parts, joined in the same order
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    parents = np.tile(np.arange(-1, count - 1), 3)
+    for o, l in ((out, lse), (want, want_lse)):
+        check_tree(q, cache, table, lens, starts, parents, 0.1, window, o, l)
 
 
 @pytest.mark.parametrize("hq,count", [(4, 12), (16, 50)])
@@ -431,6 +435,65 @@ def test_verified_tokens_follow_the_target(sampling, drawn, tree):
     got = np.bincount(first, minlength=vocab) / seqs
     assert np.all(np.abs(got - p) <= 5 * np.sqrt(p * (1 - p) / seqs)), (got, p)
     assert (accepted > 1).any() and (accepted == 1).any()
+
+
+@pytest.mark.parametrize("probe", [False, True])
+def test_verify_of_shared_sums(sampling, probe):
+    """Trees whose sums several workgroups share: each from the others', and (the measurement library's
+    build) each adding up all of them itself, as after a wait in vain. Replayed in a graph, where the
+    workspace holds the sums of the replay before."""
+    say("shared sums", probe)
+    rng = np.random.default_rng(7)
+    counts, vocab = [12, 1, 0, 30, 7], 20011
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    rows = starts[-1]
+    target = random_probs(rng, rows, vocab)
+    draft = (target * rng.random((rows, vocab)) ** 0.5).astype(np.float32)
+    draft = (draft / draft.sum(1, keepdims=True)).astype(np.float32)
+    if not probe:
+        tokens, parents = drafts_of(rng, target, draft, starts, True)
+        ws, t, q = sampling.new_workspace().fill_(0), dev(target), dev(draft)
+        ids, par, at = dev(np.int64(tokens)), dev(np.int32(parents)), dev(np.int32(starts))
+        u = torch.zeros(rows, device="cuda")
+        path, accepted, following = (torch.empty(n, dtype=d, device="cuda") for n, d in
+                                     ((rows, torch.int32), (5, torch.int32), (5, torch.int64)))
+        call = lambda: sampling.verify_drafts(t, q, ids, par, at, u, ws, path, accepted, following)  # noqa: E731
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        for trial in range(6):
+            uniforms = rng.random(rows, dtype=np.float32)
+            u.copy_(dev(uniforms))
+            graph.replay()
+            got = [host(x).copy() for x in (path, accepted, following)]
+            check_verify(sampling, t, q, tokens, parents, starts, uniforms)
+            eager = run_verify(sampling, t, q, tokens, parents, starts, uniforms)
+            assert all(np.array_equal(a, b) for a, b in zip(got, eager))
+        return
+    import ctypes
+
+    from consumer_int8 import _abi
+
+    _abi.load()
+    lib = ctypes.CDLL(str(_abi.LIB_PATH.with_name("libci8_probe.so")))
+    lib.probe_verify_drafts.argtypes = [ctypes.c_void_p] * 6 + [ctypes.c_int64] * 3 + [ctypes.c_void_p] * 5
+    for trial in range(3):
+        tokens, parents = drafts_of(rng, target, draft, starts, True)
+        uniforms = rng.random(rows, dtype=np.float32)
+        want = run_verify(sampling, dev(target), dev(draft), tokens, parents, starts, uniforms)
+        held = [dev(x) for x in (target, draft, np.int64(tokens), np.int32(parents), np.int32(starts), uniforms)]
+        out = [torch.empty(n, dtype=d, device="cuda") for n, d in
+               ((rows, torch.int32), (5, torch.int32), (5, torch.int64))]
+        ws = sampling.new_workspace().fill_(math.nan)
+        status = lib.probe_verify_drafts(*(x.data_ptr() for x in held), 5, rows, vocab, ws.data_ptr(),
+                                         *(x.data_ptr() for x in out), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert status == 0 and all(np.array_equal(host(a), b) for a, b in zip(out, want))
 
 
 def test_verify_offsets_past_32_bits(sampling):
