@@ -57,13 +57,14 @@ __device__ __forceinline__ Sequence sequence(const AttentionArgs& p, int seq) {
   return s;
 }
 
-// A tree of at most 64 queries. Lane l gets the set of query l and its ancestors, bit a for query a:
-// sets of parents are joined while the way up from each doubles, six rounds at most. A parent is
-// a query before its own; any other number is none.
-__device__ __forceinline__ uint64_t tree_ancestors(const AttentionArgs& p, const Sequence& s,
-                                                   int lane) {
-  int up = -1;
-  if (lane < s.shown) up = p.parents[s.q_begin + lane];
+// A tree of at most 64 queries. Lane l: the parent of query l as it stands.
+__device__ __forceinline__ int tree_parent(const AttentionArgs& p, const Sequence& s, int lane) {
+  return lane < s.shown ? p.parents[s.q_begin + lane] : -1;
+}
+// Lane l gets the set of query l and its ancestors, bit a for query a: sets of parents are joined
+// while the way up from each doubles, six rounds at most. A parent is a query before its own; any
+// other number is none.
+__device__ __forceinline__ uint64_t tree_ancestors(int up, int lane) {
   if (up >= lane) up = -1;
   uint64_t set = uint64_t(1) << lane;
   while (__any(up >= 0)) {

@@ -190,9 +190,11 @@ __device__ __forceinline__ const AttentionArgs& arguments() {
   return *(const AttentionArgs*)args;
 }
 
+// Whether registers leave no room for the queries of a block; eight waves share them then.
+constexpr bool queries_in_lds(int dim, int tiles) { return dim * tiles >= 512 || tiles == 4; }
 // Workgroups of a CU, by their registers and LDS.
 constexpr int groups_per_cu(int dim, int tiles) {
-  return dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
+  return tiles == 4 ? 1 : dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
 }
 
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone. kTree:
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   __shared__ __align__(16) char shared[kWaves * kWaveBytes];
   __shared__ float tops[kWaves][kRows], sums[kWaves][kRows];
   // The queries' operands stay in registers, or in LDS where those are taken.
-  constexpr bool kQueriesInLds = D == 256 && kTiles == 2;
+  constexpr bool kQueriesInLds = queries_in_lds(D, kTiles);
   constexpr int kSteps = L::kChunks * L::kSteps;
   __shared__ u32x4 queries[kQueriesInLds ? kTiles * kSteps * 64 : 1];
   __shared__ uint64_t tree[kTree ? 64 : 1];  // what each query sees of the tree, bit a for query a
@@ -287,11 +289,9 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
     // Every row attends to [last_low, all_high). Of a tree nothing is known; the sets are for the
     // tiles that have some of it, and depths for a window.
     const int all_high = kTree ? s.shift : s.first_high;
-    if (kTree && (p.window || t_end * kTokens > s.shift)) {
-      const uint64_t set = tree_ancestors(p, s, lane);
-      depth = __builtin_popcountll(set) - 1;
-      tree[kTree ? lane : 0] = tree_seen(p, set);  // every wave the same
-    }
+    const bool some_tree = kTree && (p.window || t_end * kTokens > s.shift);
+    int parent = -1;
+    if (some_tree) parent = tree_parent(p, s, lane);
     u32x4 q[kTiles][L::kChunks][L::kSteps];
     if (kQueriesInLds) __syncthreads();  // the last ones are read
 #pragma unroll
@@ -300,10 +300,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       const bool live = row < s.rows;
       const int query = live ? row / p.group : 0;
       high[n] = live ? s.shift + query + 1 : 0;
-      if constexpr (kTree)
-        low[n] = tree_low(p, s, depth, query);
-      else
-        low[n] = p.window ? max(high[n] - p.window, 0) : 0;
+      low[n] = p.window && !kTree ? max(high[n] - p.window, 0) : 0;
       const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
                             int64_t(kv_head * p.group + (live ? row % p.group : 0)) *
                                 p.q.head_stride;
@@ -382,6 +379,15 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       load(k, k_codes, at_page.k_codes, k_scales, at_page.k_scales, t, 0);
       load(v, v_codes, at_page.v_codes, v_scales, at_page.v_scales, t, 0);
       there = int(in_cache & 3);
+    }
+    if (some_tree) {  // with the first tile on its way
+      const uint64_t set = tree_ancestors(parent, lane);
+      depth = __builtin_popcountll(set) - 1;
+      tree[kTree ? lane : 0] = tree_seen(p, set);  // every wave the same
+      wave_order();
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+        low[n] = tree_low(p, s, depth, max(high[n] - 1 - s.shift, 0) & 63);
     }
     while (t < t_end) {
       const bool more = t + kWaves < t_end;
@@ -744,7 +750,7 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   // of 4 heads of 256 51.4 us, with four 61.7. At D = 256 contexts that are few get one workgroup a CU and
   // so fewer parts to join: one of 131071 tokens of 4 heads 32.8 us, with two 34.8; 12 up to 9000 24.6 and
   // 25.6.
-  constexpr int kWaves = D == 256 && kTiles == 2 ? 8 : 4;
+  constexpr int kWaves = queries_in_lds(D, kTiles) ? 8 : 4;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(groups_per_cu(D, kTiles) <= 8 &&
                     2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
@@ -762,9 +768,11 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   // More threads where a context has many parts. Whole calls with 1024 and with 256, us: one of 131071
   // tokens of 4 heads of 256, 64 parts each, 32.6 and 34.8; 32 up to 8000, 3 or 4 parts, 41.4 and 37.6.
   const bool many = groups > 16 * contexts;
-  const auto join = many ? attention_join_kernel<D, kTiles, 1024> : attention_join_kernel<D, kTiles, 256>;
-  join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : 256, 0,
-         stream>>>(args, most, blocks, groups, by_context);
+  constexpr int kFewThreads = kTiles == 4 ? 512 : 256;
+  const auto join = many ? attention_join_kernel<D, kTiles, 1024>
+                         : attention_join_kernel<D, kTiles, kFewThreads>;
+  join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : kFewThreads,
+         0, stream>>>(args, most, blocks, groups, by_context);
   return hipGetLastError();
 }
 
@@ -788,13 +796,16 @@ static hipError_t launch_split_rows(const AttentionArgs& args, int dim, int most
 
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream) {
+  if (args.parents && most > 64 && dim == 64) return launch_split<64, 4, true>(args, most, stream);
+  if (args.parents && most > 64 && dim == 128) return launch_split<128, 4, true>(args, most, stream);
   return most <= 16 ? launch_split_rows<1>(args, dim, most, stream)
                     : launch_split_rows<2>(args, dim, most, stream);
 }
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  const RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
+  RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
+  if (args.parents) rows = tree_split(rows, args.group, args.max_q, dim);
   if (rows.split) {
     if (const hipError_t e = launch_attention_split(args, dim, rows.few, stream); e != hipSuccess)
       return e;
