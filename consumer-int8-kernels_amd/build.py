@@ -35,7 +35,7 @@ ARCH = "gfx950"
 HIP_SOURCES = ["quantize.hip", "gemm.hip", "gemm_small.hip", "gemm_ring.hip", "gemm_pp.hip", "gemv.hip", "gemv_stream.hip", "silu.hip",
                "allspark.hip", "q8block.hip", "gguf_q8.hip", "gguf_ring.hip",
                "gemm_grouped.hip", "grouped_ring.hip", "noalloc.hip", "gemm_bytes.hip",
-               "norm_rope.hip", "attention_split.hip", "attention_prompt.hip",
+               "norm_rope.hip", "attention_split.hip", "attention_prompt.hip", "attention_tree.hip",
                "move_fp4.hip", "sampling.hip"]
 HOST_SOURCES = ["abi.cpp", "attention_abi.cpp", "sampling_abi.cpp"]
 

@@ -90,11 +90,25 @@ __device__ __forceinline__ int tree_low(const AttentionArgs& p, const Sequence& 
                                         int query) {
   return p.window ? max(s.shift + __shfl(depth, query, 64) + 1 - p.window, 0) : 0;
 }
-// Whether a row of a tree, which sees tokens up to `high`, sees one of them: those before the tree,
-// and those that its query's set in LDS names.
-__device__ __forceinline__ bool tree_sees(const uint64_t* seen, int high, int token, int shift) {
+// What a row of a tree, which attends to [low, high), sees of the 32 tokens from `first` on, bit i for
+// token first + i: those before the tree, and those that its query's set in LDS names. Shifts of 64
+// bits by a vector register are kept out: with the amount in the last register that a wave has they
+// gave wrong bits here now and then.
+__device__ __forceinline__ uint32_t tree_sees(const uint64_t* seen, int low, int high, int first,
+                                              int shift) {
   const uint64_t set = seen[max(high - 1 - shift, 0) & 63];
-  return (token < shift) | ((set >> (uint32_t(token - shift) & 63) & 1) != 0);
+  const uint32_t near = uint32_t(set), far = uint32_t(set >> 32);
+  const int ahead = first - shift;  // the same in all lanes
+  uint32_t bits = ~0u;
+  if (ahead >= 32)
+    bits = ahead < 64 ? far >> (ahead - 32) : 0;
+  else if (ahead >= 0)
+    bits = __builtin_amdgcn_alignbit(far, near, uint32_t(ahead));
+  else if (ahead > -32)
+    bits = near << -ahead | ((1u << -ahead) - 1);
+  const int passed = low - first;
+  if (passed > 0) bits = passed < 32 ? bits >> passed << passed : 0;
+  return high > first ? bits : 0;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -78,6 +78,7 @@ hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream);
 hipError_t launch_attention_prompt(const AttentionArgs& args, int dim, int few,
                                    hipStream_t stream);
+hipError_t launch_attention_tree(const AttentionArgs& args, int dim, hipStream_t stream);
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream);
 
 }  // namespace ci8

@@ -72,13 +72,10 @@ inline RowSplit row_split(int64_t tokens, int64_t seqs, int group, int64_t max_q
   return {few, group <= few, most > few};
 }
 
-// Trees: up to kMostTreeRows a sequence are few.
-constexpr int kMostTreeRows = 512;
-inline RowSplit tree_split(const RowSplit& usual, int group, int64_t max_q, int dim) {
-  const int64_t most = max_q * group;
-  if (dim == 256 || most > kMostTreeRows) return usual;
-  return {int(most), true, false};
-}
+// Trees: up to kFewTreeRows a sequence go to the split kernel as they are few, more to the tree kernel in
+// blocks.
+constexpr int kFewTreeRows = 32;
+constexpr int tree_rows(int dim) { return dim == 256 ? 32 : 64; }
 
 // Units of the prompt kernel's work at most: its row tiles (each but a sequence's last is full) for
 // each key head. The kernel has as many workgroups, and one more a CU where contexts may be cut.

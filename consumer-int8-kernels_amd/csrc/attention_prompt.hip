@@ -114,77 +114,6 @@ __device__ __forceinline__ Cut cut_units(const AttentionArgs& p, int few, int ro
   return c;
 }
 
-// Trees, where units are no more than the CUs and sequences no more than a wave's lanes: contexts
-// differ, and so do units (the last row tile of a sequence may have few waves of rows), so each unit
-// is cut by what it costs, into as many parts as leave the longest part shortest with one for each CU.
-// Lane l counts sequence l's.
-struct TreeCut {
-  bool apart;       // else units are cut as prompts' are
-  int tiles;        // row tiles of a key head
-  int full, last;   // parts of a full row tile, and of the last one
-  int parts, units; // of this and all sequences before it, all key heads
-};
-// Costs, in sixteenths of a tile of full rows. A row tile with one wave a SIMD or fewer takes 9 of 16.
-constexpr int kFullCost = 16, kFewCost = 9, kBeginCost = 48;
-template <int D>
-__device__ __forceinline__ TreeCut cut_tree(const AttentionArgs& p, int few, int cus, int most_splits,
-                                            int lane) {
-  using S = Shape<D>;
-  TreeCut c = {};
-  if (p.seqs > 64 || most_splits <= 1) return c;
-  int tiles = 0, waves = 0;
-  if (lane < p.seqs) {
-    const Sequence s = sequence(p, lane);
-    c.tiles = row_tiles(s, few, S::kRows);
-    const int low = p.window ? max(s.shift + 1 - p.window, 0) : 0;
-    tiles = (s.high + S::kTokens - 1) / S::kTokens - low / S::kTokens;
-    waves = c.tiles ? (s.rows - (c.tiles - 1) * S::kRows + 31) / 32 : 0;
-  }
-  const int heads = p.cache.heads;
-  c.units = wave_scan(c.tiles) * heads;
-  if (at_lane(c.units, 63) > cus) return c;
-  c.apart = true;
-  const int full = tiles * kFullCost + kBeginCost;
-  const int last = tiles * (waves > 4 ? kFullCost : kFewCost) + kBeginCost;
-  const int others = max(c.tiles - 1, 0);
-  // Their sum may pass 32 bits.
-  const int64_t total = (int64_t(wave_sum(c.tiles ? others * (full >> 12) + (last >> 12) : 0)) << 12) +
-                        wave_sum(c.tiles ? others * (full & 4095) + (last & 4095) : 0);
-  int quota = max(int(total * heads / cus), 4 * kFullCost + kBeginCost);
-  for (;; quota += quota / 32 + 1) {
-    c.full = (full + quota - 1) / quota;
-    c.last = (last + quota - 1) / quota;
-    c.parts = wave_scan(c.tiles ? others * c.full + c.last : 0) * heads;
-    if (at_lane(c.parts, 63) <= cus) return c;
-  }
-}
-
-// A part of a unit. seq < 0: there is none.
-struct TreePart {
-  int seq, row0, head, split, splits, first;  // first: the unit's first part
-};
-// Of the part or the unit that `index` counts to.
-__device__ __forceinline__ TreePart find_tree_part(const TreeCut& c, int heads, int index, bool unit) {
-  TreePart x = {-1, 0, 0, 0, 0, 0};
-  const uint64_t hit = __ballot((unit ? c.units : c.parts) > index);
-  if (!hit) return x;
-  x.seq = __builtin_ctzll(hit);
-  const int others = at_lane(c.tiles, x.seq) - 1;
-  const int full = at_lane(c.full, x.seq), last = at_lane(c.last, x.seq);
-  const int parts = at_lane(c.parts, x.seq) - heads * (others * full + last);  // before it
-  int inside = index - (unit ? at_lane(c.units, x.seq) - heads * (others + 1) : parts);
-  const int in_front = heads * others * (unit ? 1 : full);
-  const bool at_last = inside >= in_front;
-  if (at_last) inside -= in_front;
-  x.splits = at_last ? last : full;
-  x.split = unit ? 0 : inside % x.splits;
-  const int number = unit ? inside : inside / x.splits;  // of its kind
-  x.row0 = at_last ? others : number / heads;
-  x.head = number % heads;
-  x.first = parts + (at_last ? heads * others * full : 0) + number * x.splits;
-  return x;
-}
-
 // Parts of the workspace: [cut unit][split][row][D] and the statistics after them.
 __device__ __forceinline__ float* part_sums(const AttentionArgs& p, int64_t row, int dim) {
   return p.workspace + row * dim;
@@ -193,8 +122,7 @@ __device__ __forceinline__ float* part_stats(const AttentionArgs& p, int64_t row
   return p.workspace + int64_t(kAttentionWorkspaceRows) * dim + row * 2;
 }
 
-// kTree: queries are a tree of drafted tokens.
-template <int D, bool kTree>
+template <int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads)
     attention_prompt_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
   using S = Shape<D>;
@@ -209,7 +137,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   constexpr int kValues = kKeyBuffers * S::kKeyBytes;
   __shared__ uint8_t poison[kPoisonBuffers][kTokens][S::kBlocks];  // NaN blocks of edge tiles
   __shared__ int poisoned[kPoisonBuffers];  // the last such tile that has any
-  __shared__ uint64_t tree[kTree ? 64 : 1];  // what each query sees of the tree, bit a for query a
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6);
   const int column = lane & 31, half = lane >> 5;
@@ -224,32 +151,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
       split = part % splits;
     }
   }
-  int kv_head = unit % heads, seq, row0;
-  TreeCut cut = {};
-  if (kTree) cut = cut_tree<D>(p, few, cus, most_splits, lane);
-  if (kTree && cut.apart) {
-    const TreePart x = find_tree_part(cut, heads, blockIdx.x, false);
-    kv_head = x.head;
-    seq = x.seq;
-    row0 = x.row0 * S::kRows;
-    split = x.split;
-    splits = x.splits;
-    part = blockIdx.x;
-  } else {
-    const RowTile where = find_row_tile(p, few, S::kRows, unit / heads, lane);
-    seq = where.seq;
-    // The last rows see the most: they go first.
-    row0 = (where.tiles - 1 - where.tile) * S::kRows;
-  }
-  if (seq < 0) return;
-  const Sequence s = sequence(p, seq);
+  const int kv_head = unit % heads;
+  const RowTile where = find_row_tile(p, few, S::kRows, unit / heads, lane);
+  if (where.seq < 0) return;
+  const Sequence s = sequence(p, where.seq);
+  // The last rows see the most: they go first.
+  const int row0 = (where.tiles - 1 - where.tile) * S::kRows;
   const int last_row = min(row0 + S::kRows, s.rows) - 1;
 
-  // Tokens that any row of the workgroup attends to, and those that all attend to: of a tree none,
-  // and its first positions are those right behind the context.
-  const int first_high = kTree ? s.shift : s.shift + row0 / p.group + 1;
-  const int high = max(s.shift + last_row / p.group + 1, 0);
-  const int tile_low = p.window ? max(first_high + (kTree ? 1 : 0) - p.window, 0) : 0;
+  // Tokens that any row of the workgroup attends to, and those that all attend to.
+  const int first_high = s.shift + row0 / p.group + 1, high = max(s.shift + last_row / p.group + 1, 0);
+  const int tile_low = p.window ? max(first_high - p.window, 0) : 0;
   const int last_low = p.window ? max(high - p.window, 0) : 0;
   int t_begin = tile_low / kTokens, t_end = (high + kTokens - 1) / kTokens;
   if (splits > 1) {
@@ -260,7 +172,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   }
 
   const int context_page = max(s.context - 1, 0) >> p.cache.page_shift;
-  const int32_t* const table = p.page_table + int64_t(seq) * p.table_width;
+  const int32_t* const table = p.page_table + int64_t(where.seq) * p.table_width;
   // Staging. A thread converts 32 channels of one token a pack; a wave's packs are all of the keys
   // or all of the values, of one page or two. Pages are looked up a tile ahead of the codes, these
   // are loaded a tile ahead of their use. Past the last tile this goes on with tokens that are
@@ -364,22 +276,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
   // The lane's rows and their tokens [low, high). Lanes past the last row repeat it; their results
   // go nowhere.
   int row_low[kTiles], row_high[kTiles];
-  int depth = 0;
-  if (kTree) {
-    const uint64_t set = tree_ancestors(tree_parent(p, s, lane), lane);
-    depth = __builtin_popcountll(set) - 1;
-    tree[kTree ? lane : 0] = tree_seen(p, set);  // every wave the same
-  }
   u32x4 q[kTiles][kHeld];
   const int wave_row = row0 + wave * 32 * kTiles;
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
     const int row = min(wave_row + 32 * n + column, s.rows - 1), query = row / p.group;
     row_high[n] = s.shift + query + 1;
-    if constexpr (kTree)
-      row_low[n] = tree_low(p, s, depth, query);
-    else
-      row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
+    row_low[n] = p.window ? max(row_high[n] - p.window, 0) : 0;
     const uint16_t* src = p.q.data + int64_t(s.q_begin + query) * p.q.token_stride +
                           int64_t(kv_head * p.group + row % p.group) * p.q.head_stride;
 #pragma unroll
@@ -396,7 +299,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     load_codes(ahead, pages_ahead, t_begin + 1, t_begin);
   }
   // Tokens [all_low, all_high) that all of the wave's rows attend to.
-  const int all_high = kTree ? s.shift : s.shift + min(wave_row, s.rows - 1) / p.group + 1;
+  const int all_high = s.shift + min(wave_row, s.rows - 1) / p.group + 1;
   const int any_high = s.shift + min(wave_row + 32 * kTiles - 1, s.rows - 1) / p.group + 1;
   const int all_low = p.window ? max(any_high - p.window, 0) : 0;
 
@@ -501,8 +404,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         for (int i = 0; i < 16; ++i) {
           const int at = 8 * (i / 4) + i % 4, token = first + at + 4 * half;
           const bool seen = (token >= row_low[n]) & (token < row_high[n]) &
-                            (at < 16 ? low_there : high_there) &
-                            (!kTree || tree_sees(tree, row_high[n], token, s.shift));
+                            (at < 16 ? low_there : high_there);
           x[n][i] = seen ? x[n][i] : -__builtin_inff();
         }
         most[n] = largest(x[n]);
@@ -578,8 +480,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
         if (poison[t % kPoisonBuffers][token][m]) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n] &&
-                (!kTree || tree_sees(tree, row_high[n], t * kTokens + token, s.shift)))
+            if (t * kTokens + token >= row_low[n] && t * kTokens + token < row_high[n])
               o[n][m] += __builtin_nanf("");
         }
   };
@@ -633,22 +534,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
     }
   }
   int buffer[3] = {0, 1, 2};  // of the keys of this tile and the next two
-  // Waves that have no rows stage tiles for those that have: 156 rows of 256 channels behind contexts up to
-  // 131071 tokens, where 5 of 8 have some, 361 us, 433 with all of them computing. Prompts have few.
-  const bool idle = kTree && wave_row >= s.rows;
-  if (kTree && idle) {
-    for (int t = t_begin; t < t_end; ++t) {
-      store_tiles(staged, buffer[2], t + 1);
-      load_codes(staged, pages, t + 3, t + 2);
-      load_pages(pages, t + 4, t + 3);
-      __syncthreads();
-      const int first = buffer[0];
-      buffer[0] = buffer[1];
-      buffer[1] = buffer[2];
-      buffer[2] = first;
-    }
-    return;
-  }
   for (int t = t_begin; t < t_end; ++t) {
 #pragma unroll
     for (int b = 0; b < kHalves; ++b) {
@@ -736,39 +621,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads)
 
 // Joins the parts of the rows of cut units: D / 4 lanes a row.
 constexpr int kJoinThreads = 512;
-template <int D, bool kTree>
+template <int D>
 __global__ void __launch_bounds__(kJoinThreads)
     attention_prompt_join_kernel(const AttentionArgs p, int few, int cus, int most_splits) {
   constexpr int kRows = Shape<D>::kRows, kLanes = D / 4, kSlices = kRows * kLanes / kJoinThreads;
   const int lane = threadIdx.x & 63, slice = blockIdx.x % kSlices, cut = blockIdx.x / kSlices;
+  const Cut c = cut_units(p, few, kRows, cus, most_splits, lane);
+  const int unit = c.whole + cut;
+  if (unit >= c.units) return;
+  const RowTile where = find_row_tile(p, few, kRows, unit / p.cache.heads, lane);
+  const Sequence s = sequence(p, where.seq);
   const int r = slice * (kJoinThreads / kLanes) + int(threadIdx.x) / kLanes;
   const int channel = threadIdx.x % kLanes * 4;
-  int seq, row0, kv_head, splits;
-  int64_t first;
-  TreeCut trees = {};
-  if (kTree) trees = cut_tree<D>(p, few, cus, most_splits, lane);
-  if (kTree && trees.apart) {
-    const TreePart x = find_tree_part(trees, p.cache.heads, cut, true);
-    if (x.seq < 0 || x.splits == 1) return;
-    seq = x.seq;
-    row0 = x.row0 * kRows;
-    kv_head = x.head;
-    splits = x.splits;
-    first = int64_t(x.first) * kRows + r;
-  } else {
-    const Cut c = cut_units(p, few, kRows, cus, most_splits, lane);
-    const int unit = c.whole + cut;
-    if (unit >= c.units) return;
-    const RowTile where = find_row_tile(p, few, kRows, unit / p.cache.heads, lane);
-    seq = where.seq;
-    row0 = (where.tiles - 1 - where.tile) * kRows;
-    kv_head = unit % p.cache.heads;
-    splits = c.splits;
-    first = int64_t(cut) * splits * kRows + r;
-  }
-  const Sequence s = sequence(p, seq);
-  const int row = row0 + r;
+  const int row = (where.tiles - 1 - where.tile) * kRows + r;
   if (row >= s.rows) return;
+  const int64_t first = int64_t(cut) * c.splits * kRows + r;
   float top = kLowest, total = 0;
   f32x4 x = {0, 0, 0, 0};
   // Parts i .. i + n - 1, on their way together; past the last they are that one again, and count 0.
@@ -777,7 +644,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     f32x4 sums[n];
 #pragma unroll
     for (int j = 0; j < n; ++j) {
-      const int64_t at = first + int64_t(min(i + j, splits - 1)) * kRows;
+      const int64_t at = first + int64_t(min(i + j, c.splits - 1)) * kRows;
       stats[j] = *reinterpret_cast<const f32x2*>(part_stats(p, at, D));
       sums[j] = *reinterpret_cast<const f32x4*>(part_sums(p, at, D) + channel);
     }
@@ -790,19 +657,19 @@ __global__ void __launch_bounds__(kJoinThreads)
     x *= old;
 #pragma unroll
     for (int j = 0; j < n; ++j)
-      if (i + j < splits) {
+      if (i + j < c.splits) {
         const float factor = __builtin_amdgcn_exp2f(stats[j][0] - most);
         total += stats[j][1] * factor;
         x += sums[j] * factor;
       }
   };
   int i = 0;
-  for (; i + 8 <= splits; i += 8) add(i, std::integral_constant<int, 8>());
-  for (; i < splits; i += 2) add(i, std::integral_constant<int, 2>());
-  write_row4(p, D, s.q_begin, row, kv_head, channel, x, top, total);
+  for (; i + 8 <= c.splits; i += 8) add(i, std::integral_constant<int, 8>());
+  for (; i < c.splits; i += 2) add(i, std::integral_constant<int, 2>());
+  write_row4(p, D, s.q_begin, row, unit % p.cache.heads, channel, x, top, total);
 }
 
-template <int D, bool kTree>
+template <int D>
 hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream) {
   using S = Shape<D>;
   const int found = device_cu_count(), cus = found > 0 && found <= 256 ? found : 256;
@@ -819,15 +686,14 @@ hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream)
   if (splits > cus) splits = cus;
   if (splits < 1) splits = 1;
   const int64_t grid = units + (splits > 1 ? cus : 0);
-  attention_prompt_kernel<D, kTree>
+  attention_prompt_kernel<D>
       <<<uint32_t(grid), S::kThreads, 0, stream>>>(args, few, cus, int(splits));
   if (splits == 1) return hipGetLastError();
   if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  // A unit that is cut has two parts or more. A tree's units are counted with those that are not.
+  // A unit that is cut has two parts or more.
   constexpr int kSlices = S::kRows * (D / 4) / kJoinThreads;
-  const int most_cut = !kTree ? cus / 2 : int(units < cus ? units : cus);
-  attention_prompt_join_kernel<D, kTree>
-      <<<uint32_t(most_cut * kSlices), kJoinThreads, 0, stream>>>(args, few, cus, int(splits));
+  attention_prompt_join_kernel<D>
+      <<<uint32_t(cus / 2 * kSlices), kJoinThreads, 0, stream>>>(args, few, cus, int(splits));
   return hipGetLastError();
 }
 
@@ -835,15 +701,9 @@ hipError_t launch_prompt(const AttentionArgs& args, int few, hipStream_t stream)
 
 hipError_t launch_attention_prompt(const AttentionArgs& args, int dim, int few, hipStream_t stream) {
   switch (dim) {
-    case 64:
-      return args.parents ? launch_prompt<64, true>(args, few, stream)
-                          : launch_prompt<64, false>(args, few, stream);
-    case 128:
-      return args.parents ? launch_prompt<128, true>(args, few, stream)
-                          : launch_prompt<128, false>(args, few, stream);
-    default:
-      return args.parents ? launch_prompt<256, true>(args, few, stream)
-                          : launch_prompt<256, false>(args, few, stream);
+    case 64: return launch_prompt<64>(args, few, stream);
+    case 128: return launch_prompt<128>(args, few, stream);
+    default: return launch_prompt<256>(args, few, stream);
   }
 }
 

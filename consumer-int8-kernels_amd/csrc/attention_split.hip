@@ -35,21 +35,11 @@
 // to 266 us, 5.4 to 5.6 TB/s (a stream of reads alone reaches 5.9 to 6.06); 32 up to 8000 40 us, 3.7
 // TB/s with the join (5 us) and the way into the pipeline counted; one of 517 tokens 7.4 us, nearly all
 // the launch.
-#include "attention_device.h"
-#include "attention_plan.h"
+#include "attention_runs.h"
 #include "launch.h"
 
 namespace ci8 {
 namespace {
-
-constexpr int kTokens = 32;  // tokens a wave takes at once
-
-// Keeps LDS accesses of a wave's lanes in program order; the LDS itself does.
-__device__ __forceinline__ void wave_order() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 template <int D>
 struct Layout {
@@ -85,116 +75,9 @@ __device__ __forceinline__ void load_rows(Raw<D>& r, const uint8_t* codes, const
   }
 }
 
-// What the split kernel has of a sequence: blocks of rows, none if those are more than `most`, which
-// are the prompt kernel's, and the tiles of each, at least one (it writes the rows that attend to
-// nothing). Each block of a key head has its own context.
-__device__ __forceinline__ int row_blocks(const Sequence& s, int most, int block_rows) {
-  return s.rows > most ? 0 : (s.rows + block_rows - 1) / block_rows;
-}
-__device__ __forceinline__ int block_tiles(const Sequence& s) { return max(s.tiles(kTokens), 1); }
-// What it costs to begin a context, in tiles: queries and pages on their way in and sums out take a
-// workgroup 9000 clocks, a tile 800 with three workgroups a CU. Not counted, workgroups that had four
-// short contexts ran 73000 clocks where others ran 47000: 32 contexts up to 8000 41 us, counted 37.7,
-// 64 from 100 to 4000 58 and 39.
-constexpr int kBegin = 10;
-
-// A run: [begin, end) of the row of all sequences' costs, one after the other for each key head and
-// block of rows.
-struct Run {
-  int64_t begin, end, quota;
-};
-struct Place {
-  int seq, head, block, blocks, at, cost;  // at: of its cost
-};
-
-// Of 64 sequences from `base` on, one a lane: blocks of a key head, cost of a block, and sums of
-// both's products up to each lane's.
-struct Counted {
-  int base, blocks, cost, sum;
-};
-__device__ __forceinline__ Counted count_costs(const AttentionArgs& p, int most, int block_rows,
-                                               int begin, int lane, int base) {
-  Counted c = {base, 0, 1, 0};
-  if (base + lane < p.seqs) {
-    const Sequence s = sequence(p, base + lane);
-    c.blocks = row_blocks(s, most, block_rows);
-    c.cost = block_tiles(s) + begin;
-  }
-  c.sum = wave_scan(c.blocks * c.cost);
-  return c;
-}
-// Costs of all; `first` are those of the first 64 sequences.
-__device__ __forceinline__ int64_t all_costs(const AttentionArgs& p, int most, int block_rows,
-                                             int begin, int lane, const Counted& first) {
-  int64_t total = at_lane(first.sum, 63);
-  for (int base = 64; base < p.seqs; base += 64)
-    total += at_lane(count_costs(p, most, block_rows, begin, lane, base).sum, 63);
-  return total * p.cache.heads;
-}
-
-// Where `at` of all costs lies; it is less than their sum. `first`: of the first 64 sequences.
-__device__ __forceinline__ Place find_place(const AttentionArgs& p, int most, int block_rows,
-                                            int begin, int lane, int64_t at, const Counted& first) {
-  const int heads = p.cache.heads;
-  Counted c = first;
-  int64_t before = 0;
-  for (;;) {
-    const uint64_t hit = __ballot(before + int64_t(c.sum) * heads > at);
-    if (hit || c.base + 64 >= p.seqs) {
-      const int which = hit ? __builtin_ctzll(hit) : 0;
-      Place place;
-      place.seq = uniform(c.base + which);
-      place.cost = at_lane(c.cost, which);
-      place.blocks = max(at_lane(c.blocks, which), 1);
-      const int in_front = at_lane(c.sum, which) - place.cost * place.blocks;
-      const int64_t inside = at - before - int64_t(in_front) * heads;
-      const int context = uniform(int(inside / place.cost));
-      place.at = uniform(int(inside % place.cost));
-      place.head = uniform(context / place.blocks);
-      place.block = uniform(context % place.blocks);
-      return place;
-    }
-    before += int64_t(at_lane(c.sum, 63)) * heads;
-    c = count_costs(p, most, block_rows, begin, lane, c.base + 64);
-  }
-}
-
-// Parts in the workspace: of workgroup w, part 2w continues a context, part 2w + 1 begins one.
-// Sums of rows [part][row][D] first, then their [reference, sum], then what the workgroup that
-// begins a context says of it: one for each context (0 parts: its output is written), or, where
-// contexts are more than workgroups, for each workgroup, which begins one at most that another
-// continues.
-struct Joint {
-  int parts, first, q_begin, row0, rows, head, unused[2];
-};
-template <int D, int kTiles>
-__device__ __forceinline__ float* part_sums(const AttentionArgs& p, int part) {
-  return p.workspace + int64_t(part) * (16 * kTiles * D);
-}
-template <int D, int kTiles>
-__device__ __forceinline__ float* part_stats(const AttentionArgs& p, int part) {
-  return p.workspace + int64_t(kAttentionWorkspaceRows) * D + part * (16 * kTiles * 2);
-}
-template <int D>
-__device__ __forceinline__ Joint* joints(const AttentionArgs& p) {
-  // the last 64 KiB of the [rows, 2] region
-  return reinterpret_cast<Joint*>(p.workspace + int64_t(kAttentionWorkspaceRows) * (D + 2)) - 2048;
-}
-
-// The kernel's first argument, read anew: what one part of a long kernel needs of it is not held
-// in registers through the others.
-__device__ __forceinline__ const AttentionArgs& arguments() {
-  auto* args =
-      (const __attribute__((address_space(4))) AttentionArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(args));
-  return *(const AttentionArgs*)args;
-}
-
-// Whether registers leave no room for the queries of a block; eight waves share them then.
-constexpr bool queries_in_lds(int dim, int tiles) { return dim * tiles >= 512 || tiles == 4; }
 // Workgroups of a CU, by their registers and LDS.
 constexpr int groups_per_cu(int dim, int tiles) {
-  return tiles == 4 ? 1 : dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
+  return dim == 64 ? (tiles == 1 ? 4 : 2) : dim == 128 ? (tiles == 1 ? 3 : 2) : 3 - tiles;
 }
 
 // kTiles tiles of 16 rows. kSplit: equal runs of all tiles; else workgroup (seq, head) alone. kTree:
@@ -212,7 +95,7 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   __shared__ __align__(16) char shared[kWaves * kWaveBytes];
   __shared__ float tops[kWaves][kRows], sums[kWaves][kRows];
   // The queries' operands stay in registers, or in LDS where those are taken.
-  constexpr bool kQueriesInLds = queries_in_lds(D, kTiles);
+  constexpr bool kQueriesInLds = D == 256 && kTiles == 2;
   constexpr int kSteps = L::kChunks * L::kSteps;
   __shared__ u32x4 queries[kQueriesInLds ? kTiles * kSteps * 64 : 1];
   __shared__ uint64_t tree[kTree ? 64 : 1];  // what each query sees of the tree, bit a for query a
@@ -466,13 +349,15 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
       for (int n = 0; n < kTiles; ++n) {
         float most = -__builtin_inff();
         if (edge) {
+          uint32_t sees = 0;
+          if constexpr (kTree) sees = tree_sees(tree, low[n], high[n], t * kTokens, s.shift);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int token = t * kTokens + 16 * h + 4 * group4 + j;
-              const bool seen = (there >> h & 1) & (token >= low[n]) & (token < high[n]) &
-                                (!kTree || tree_sees(tree, high[n], token, s.shift));
+              const int at = 16 * h + 4 * group4 + j, token = t * kTokens + at;
+              const bool seen = kTree ? (there >> h & 1) & (sees >> at & 1)
+                                      : (there >> h & 1) & (token >= low[n]) & (token < high[n]);
               score[n][h][j] = seen ? score[n][h][j] : -__builtin_inff();
             }
         }
@@ -518,8 +403,8 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
           const uint32_t blocks = uint32_t(__shfl(int(poisoned[token / 16]), token % 16, 64));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            if (t * kTokens + token >= low[n] && t * kTokens + token < high[n] &&
-                (!kTree || tree_sees(tree, high[n], t * kTokens + token, s.shift))) {
+            if (kTree ? tree_sees(tree, low[n], high[n], t * kTokens, s.shift) >> token & 1
+                      : t * kTokens + token >= low[n] && t * kTokens + token < high[n]) {
 #pragma unroll
               for (int m = 0; m < D / 16; ++m)
                 o[n][m] += blocks >> (m / 2) & 1 ? __builtin_nanf("") : 0.f;
@@ -615,110 +500,6 @@ __global__ void __launch_bounds__(64 * kWaves, kSplit ? groups_per_cu(D, kTiles)
   }
 }
 
-// Joins the parts of a context (by_context: the blockIdx.x-th, else what workgroup blockIdx.x of the
-// split kernel began): 32 channels a workgroup, 8 lanes a row; groups of rows * 8 lanes take every so
-// many parts. Bound by the latency of its dependent reads, 1 to 2 us each: the sums of the first
-// parts are on their way while the statistics are read, by a row's own lanes where parts are few and
-// by whole waves where many.
-constexpr int kJoinChannels = 32;
-template <int D, int kTiles, int kThreads>
-__global__ void __launch_bounds__(kThreads)
-    attention_join_kernel(const AttentionArgs p, int most, int most_blocks, int workgroups,
-                          bool by_context) {
-  constexpr int kRows = 16 * kTiles, kLanes = kJoinChannels / 4, kEarly = 4, kFew = 8;
-  static_assert(kRows * kLanes <= kThreads);
-  Joint joint = joints<D>(p)[blockIdx.x];
-  // Contexts that the split kernel does not have say nothing.
-  if (by_context) {
-    const int seq = int(blockIdx.x) / most_blocks / p.cache.heads;
-    if (int(blockIdx.x) % most_blocks >= row_blocks(sequence(p, seq), most, kRows)) return;
-  }
-  if (joint.parts <= 0) return;
-  // Whatever stands there (a workspace that another stream writes), accesses stay in bounds.
-  joint.first = min(max(joint.first, 0), workgroups - 1);
-  joint.parts = min(joint.parts, workgroups - joint.first);
-  joint.rows = min(max(joint.rows, 1), min(kRows, p.tokens * p.group));
-  joint.row0 = min(max(joint.row0, 0), min(most, p.tokens * p.group - joint.rows));
-  joint.q_begin = min(max(joint.q_begin, 0),
-                      p.tokens - (joint.row0 + joint.rows + p.group - 1) / p.group);
-  joint.head = min(max(joint.head, 0), p.cache.heads - 1);
-  __shared__ f32x4 sums[kThreads];
-  __shared__ float tops[kRows], totals[kRows];
-  auto part = [&](int i) { return 2 * (joint.first + i) + (i == 0); };
-  const int width = joint.rows * kLanes, groups = kThreads / width;
-  const int group = threadIdx.x / width, row = threadIdx.x % width / kLanes;
-  const int channel = blockIdx.y * kJoinChannels + threadIdx.x % kLanes * 4;
-  auto sum_at = [&](int i) {
-    return *reinterpret_cast<const f32x4*>(part_sums<D, kTiles>(p, part(i)) + row * D + channel);
-  };
-  auto stats_at = [&](int i, int r) {
-    return *reinterpret_cast<const f32x2*>(part_stats<D, kTiles>(p, part(i)) + 2 * r);
-  };
-  f32x4 early[kEarly];
-  f32x2 early_stats[kEarly];
-#pragma unroll
-  for (int e = 0; e < kEarly; ++e) {
-    early[e] = f32x4{0, 0, 0, 0};
-    early_stats[e] = f32x2{kLowest, 0};
-    const int i = group + e * groups;
-    if (group < groups && i < joint.parts) {
-      early[e] = sum_at(i);
-      early_stats[e] = stats_at(i, row);
-    }
-  }
-  float top = kLowest, total = 0;
-  if (joint.parts <= kFew) {
-    f32x2 stats[kFew];
-#pragma unroll
-    for (int i = 0; i < kFew; ++i) stats[i] = stats_at(min(i, joint.parts - 1), row);
-#pragma unroll
-    for (int i = 0; i < kFew; ++i) top = fmaxf(top, stats[i][0]);
-#pragma unroll
-    for (int i = 0; i < kFew; ++i)
-      total += i < joint.parts ? stats[i][1] * __builtin_amdgcn_exp2f(stats[i][0] - top) : 0.f;
-  } else {
-    const int lane = threadIdx.x & 63;
-    for (int r = threadIdx.x >> 6; r < joint.rows; r += kThreads / 64) {
-      float m = kLowest, l = 0;
-      for (int i = lane; i < joint.parts; i += 64) {
-        const f32x2 stats = stats_at(i, r);
-        const float most = fmaxf(m, stats[0]);
-        l = l * __builtin_amdgcn_exp2f(m - most) +
-            stats[1] * __builtin_amdgcn_exp2f(stats[0] - most);
-        m = most;
-      }
-      float most = m;
-#pragma unroll
-      for (int step = 32; step >= 1; step /= 2) most = fmaxf(most, __shfl_xor(most, step, 64));
-      l *= __builtin_amdgcn_exp2f(m - most);
-#pragma unroll
-      for (int step = 32; step >= 1; step /= 2) l += __shfl_xor(l, step, 64);
-      if (lane == 0) {
-        tops[r] = most;
-        totals[r] = l;
-      }
-    }
-    __syncthreads();
-    top = tops[row];
-    total = totals[row];
-  }
-  f32x4 x = {0, 0, 0, 0};
-  if (group < groups) {
-#pragma unroll
-    for (int e = 0; e < kEarly; ++e)
-      x += early[e] * __builtin_amdgcn_exp2f(early_stats[e][0] - top);
-#pragma unroll 4
-    for (int i = group + kEarly * groups; i < joint.parts; i += groups)
-      x += sum_at(i) * __builtin_amdgcn_exp2f(stats_at(i, row)[0] - top);
-  }
-  sums[threadIdx.x] = x;
-  __syncthreads();
-  if (group == 0) {
-    for (int g = 1; g < min(groups, joint.parts); ++g) x += sums[g * width + threadIdx.x];
-    write_row4(p, D, joint.q_begin, joint.row0 + row, joint.head, channel, x, top, total);
-  }
-}
-
 // Up to this many tiles of the longest context a workgroup takes a whole context: fewer where contexts
 // leave most of the GPU idle. Whole and split, us: 16 contexts up to 2000 tokens of 8 heads of 128 14.3
 // and 15.3, 64 of them 22.1 and 29.4, 4 13.5 and 12.1, one of 1100 9.6 and 11.8; 16 of 4 heads of 256
@@ -750,7 +531,7 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   // of 4 heads of 256 51.4 us, with four 61.7. At D = 256 contexts that are few get one workgroup a CU and
   // so fewer parts to join: one of 131071 tokens of 4 heads 32.8 us, with two 34.8; 12 up to 9000 24.6 and
   // 25.6.
-  constexpr int kWaves = queries_in_lds(D, kTiles) ? 8 : 4;
+  constexpr int kWaves = D == 256 && kTiles == 2 ? 8 : 4;
   const int groups = D == 256 && contexts < 64 ? cus : cus * groups_per_cu(D, kTiles);
   static_assert(groups_per_cu(D, kTiles) <= 8 &&
                     2 * 256 * groups_per_cu(D, kTiles) * 16 * kTiles * 2 <=
@@ -768,11 +549,9 @@ hipError_t launch_split(const AttentionArgs& args, int most, hipStream_t stream)
   // More threads where a context has many parts. Whole calls with 1024 and with 256, us: one of 131071
   // tokens of 4 heads of 256, 64 parts each, 32.6 and 34.8; 32 up to 8000, 3 or 4 parts, 41.4 and 37.6.
   const bool many = groups > 16 * contexts;
-  constexpr int kFewThreads = kTiles == 4 ? 512 : 256;
-  const auto join = many ? attention_join_kernel<D, kTiles, 1024>
-                         : attention_join_kernel<D, kTiles, kFewThreads>;
-  join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : kFewThreads,
-         0, stream>>>(args, most, blocks, groups, by_context);
+  const auto join = many ? attention_join_kernel<D, kTiles, 1024> : attention_join_kernel<D, kTiles, 256>;
+  join<<<dim3(by_context ? uint32_t(contexts) : groups, D / kJoinChannels), many ? 1024 : 256, 0,
+         stream>>>(args, most, blocks, groups, by_context);
   return hipGetLastError();
 }
 
@@ -796,16 +575,15 @@ static hipError_t launch_split_rows(const AttentionArgs& args, int dim, int most
 
 hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
                                   hipStream_t stream) {
-  if (args.parents && most > 64 && dim == 64) return launch_split<64, 4, true>(args, most, stream);
-  if (args.parents && most > 64 && dim == 128) return launch_split<128, 4, true>(args, most, stream);
   return most <= 16 ? launch_split_rows<1>(args, dim, most, stream)
                     : launch_split_rows<2>(args, dim, most, stream);
 }
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
-  if (args.parents) rows = tree_split(rows, args.group, args.max_q, dim);
+  if (args.parents && int64_t(args.max_q) * args.group > kFewTreeRows)
+    return launch_attention_tree(args, dim, stream);
+  const RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
   if (rows.split) {
     if (const hipError_t e = launch_attention_split(args, dim, rows.few, stream); e != hipSuccess)
       return e;
