@@ -241,6 +241,8 @@ int attend(const ci8_heads* q, const ci8_fp4_cache* cache, const int32_t* page_t
   if (i128(table_width) * cache->page_size > (1 << 26) - 4096 ||
       i128(seqs) * table_width * 4 > kMaxExtent)
     return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large");
+  if (parents && !ci8::tree_fits(table_width * cache->page_size, max_q, q->heads / cache->heads, int(dim)))
+    return abi_fail(CI8_ERR_TOO_LARGE, "Page table too large for a tree of that many rows");
   if (!aligned(page_table, 4) || !aligned(context_lens, 4) || !aligned(q_starts, 4) ||
       !aligned(parents, 4) || !aligned(workspace, 16) || !aligned(out, 16) || !aligned(lse, 4))
     return abi_fail(CI8_ERR_ALIGNMENT, "attention_fp4 requires aligned buffers");

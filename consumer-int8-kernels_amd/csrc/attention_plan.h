@@ -76,6 +76,14 @@ inline RowSplit row_split(int64_t tokens, int64_t seqs, int group, int64_t max_q
 // blocks.
 constexpr int kFewTreeRows = 32;
 constexpr int tree_rows(int dim) { return dim == 256 ? 32 : 64; }
+// What it costs to begin a context, in tiles of one wave.
+constexpr int kTreeBegin = 40;
+// Costs of 64 sequences' blocks are summed in 32 bits, and up to twice as much where each context takes a
+// whole number of runs. Behind the longest page table that is 8 blocks.
+inline bool tree_fits(int64_t tokens, int64_t max_q, int64_t group, int dim) {
+  const int64_t blocks = (max_q * group + tree_rows(dim) - 1) / tree_rows(dim);
+  return blocks * (tokens / 32 + 1 + kTreeBegin) < (int64_t(1) << 31) / (64 * 2);
+}
 
 // Units of the prompt kernel's work at most: its row tiles (each but a sequence's last is full) for
 // each key head. The kernel has as many workgroups, and one more a CU where contexts may be cut.

@@ -68,9 +68,6 @@ __device__ __forceinline__ uint32_t anew(uint32_t v) {
   return v;
 }
 
-// What it costs to begin a context, in tiles of one wave.
-constexpr int kTreeBegin = 40;
-
 template <int D, bool kSplit>
 __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
     attention_tree_kernel(const AttentionArgs, int most, int most_blocks, int min_quota,

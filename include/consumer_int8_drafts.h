@@ -28,7 +28,9 @@ extern "C" {
 /* attention_fp4_tree: ci8_attention_fp4 for trees. All rows of sequence s are in the cache, row i of n
  * as token context_lens[s] - n + i; its position is context_lens[s] - n + its depth. It attends to the
  * tokens before the tree whose position its window reaches, to its ancestors that the window
- * reaches, and to itself. max_q is at most 64. All else is as ci8_attention_fp4 says. */
+ * reaches, and to itself. max_q is at most 64. Blocks of 64 rows (max_q times the query heads of a
+ * key head; 32 rows at dim 256) times (table_width * page_size / 32 + 41) stay under 2^24. All else is as
+ * ci8_attention_fp4 says. */
 int ci8_attention_fp4_tree(const ci8_heads* q, const ci8_fp4_cache* cache,
                            const int32_t* page_table, int64_t table_width,
                            const int32_t* context_lens, const int32_t* q_starts,

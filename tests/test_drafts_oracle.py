@@ -135,6 +135,9 @@ def test_tree_refusals(lib):
                 dict(scale=float("nan"))]:
         refused(lib, call(**bad), geometry, "Invalid attention")
     refused(lib, call(width=1 << 28), large, "Page table too large")
+    wide = dict(q=heads(n=64), c=cache(n=1, page=1024), max_q=9, width=65532)
+    refused(lib, call(**wide), large, "Page table too large for a tree of that many rows")  # 9 blocks
+    refused(lib, call(**{**wide, "max_q": 8, "out": FAKE << 15}), overlap, "must not overlap anything else")
     refused(lib, call(parents=(FAKE << 15) + 2), alignment, "attention_fp4 requires aligned")
     refused(lib, call(out=FAKE << 15), overlap, "must not overlap anything else")
     refused(lib, call(lse=FAKE << 15), overlap, "must not overlap anything else")
