@@ -60,6 +60,10 @@ def check_tree(q, cache, table, lens, starts, parents, scale, window, out, lse):
             mine = slice(h * group, (h + 1) * group)
             o, l, mean, off = OD.attention64(qh[rows, mine].reshape(-1, dim), k, v, seen, scale)
             do, dl = OA.attention_bounds(o, l, mean, off)
+            # Numbers below 2^-126 are 0 to the exponential, the products and the roundings: for each token a
+            # weight (its largest is 1 or more, which the sum of weights divides by), its product, the sum it
+            # is added to and the sum's factor where parts join, and the output.
+            do = do + (n * (np.abs(v).max(initial=0) + 3) + 1) * 2.0**-126
             got_o, got_l = oh[rows, mine].reshape(o.shape), lh[rows, mine].reshape(l.shape)
             empty = np.isneginf(l)
             assert np.array_equal(np.isneginf(got_l), empty) and (got_o[empty] == 0).all()
@@ -586,3 +590,133 @@ def test_refusals_of_tensors(attention, sampling):
                    (7, i32[:3]), (8, i32), (9, one), (7, parents), (5, t.cpu()), (8, i32[:1])]:
         with pytest.raises(RuntimeError):
             sampling.verify_drafts(*good[:i], bad, *good[i + 1:])
+
+
+# ---- more sequences, other streams, graphs -----------------------------------------------
+
+MANY = [
+    # dim, query heads, key heads, page, context lengths, rows, window: trees of more than 32 rows that are cut
+    # into runs, with as many contexts as workgroups and with more, and more than 64 sequences
+    (128, 40, 40, 64, [3000, 2400, 9], [64, 40, 9], 0),
+    (64, 40, 40, 32, [2500, 33, 2400, 2400, 700, 64, 2330], [64, 33, 64, 33, 50, 64, 1], 0),
+    (128, 10, 2, 16, [40] * 40 + [2600] + [17] * 39, [7] * 80, 0),
+    (256, 4, 1, 16, [40] * 65 + [2600, 1], [9] * 66 + [1], 0),
+    (128, 128, 1, 128, [700], [64], 0),   # 128 blocks of rows
+    (64, 100, 1, 16, [2600, 30], [64, 30], 33),
+    (64, 2, 2, 16, [50] * 70 + [4000], [3] * 71, 0),  # at most 32 rows, likewise
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(str(x)[:20].replace(" ", "") for x in c))
+def test_tree_attention_of_many(attention, case):
+    test_tree_attention(attention, case)
+
+
+def step_of_all(attention, sampling, seed):
+    """Tensors of one call of each operator, and the calls."""
+    rng = np.random.default_rng(seed)
+    dim, hq, hk, page, counts, lens = 128, 16, 2, 16, [9, 1, 20], [500, 40, 2500]
+    n, vocab = sum(counts), 33000
+    pages = sum(-(-x // page) for x in lens) + 2
+    cache = random_cache(attention, rng, pages, hk, page, dim)
+    table = tables(rng, lens, pages, page)
+    starts = np.int32(np.concatenate([[0], np.cumsum(counts)]))
+    t = dict(q=bf16_randn(rng, n, hq, dim).cuda(), table=dev(table), lens=dev(np.int32(lens)), starts=dev(starts),
+             parents=dev(np.int32(np.concatenate([random_tree(rng, c, 0.5) for c in counts]))),
+             logits=torch.from_numpy(3 * rng.standard_normal((n, vocab)).astype(np.float32)).cuda(),
+             draft=torch.from_numpy(random_probs(rng, n, vocab)).cuda(),
+             tokens=dev(rng.integers(0, vocab, n)), uniforms=dev(rng.random(n).astype(np.float32)),
+             slots=dev(rng.permutation(pages * page)[:n].astype(np.int64)),
+             out=torch.empty(n, hq, dim, dtype=torch.bfloat16, device="cuda"), lse=torch.empty(n, hq, device="cuda"),
+             probs=torch.empty(n, vocab, device="cuda"), path=torch.empty(n, dtype=torch.int32, device="cuda"),
+             accepted=torch.empty(3, dtype=torch.int32, device="cuda"),
+             next=torch.empty(3, dtype=torch.int64, device="cuda"), **cache._asdict())
+    spaces = attention.new_workspace(dim), sampling.new_workspace()
+
+    def run():
+        attention.attention_fp4_tree(t["q"], *cache, t["table"], t["lens"], t["starts"], t["parents"], spaces[0], t["out"],
+                                     t["lse"], dim ** -0.5, 20, 0)
+        sampling.token_probs(t["logits"], None, spaces[1], t["probs"])
+        sampling.verify_drafts(t["probs"], t["draft"], t["tokens"], t["parents"], t["starts"], t["uniforms"], spaces[1],
+                               t["path"], t["accepted"], t["next"])
+        attention.move_fp4(*cache, t["path"], t["slots"], t["starts"])
+
+    def results():
+        return [t[name].clone() for name in ("out", "lse", "probs", "path", "accepted", "next", *cache._fields)]
+
+    return t, run, results
+
+
+def refill(t, other):
+    for name in ("q", "parents", "logits", "draft", "tokens", "uniforms", "k_codes", "k_scales", "v_codes", "v_scales"):
+        t[name].copy_(other[name])
+
+
+def test_graphs_of_all_replay_with_other_inputs(attention, sampling):
+    t, run, results = step_of_all(attention, sampling, 1)
+    others = [step_of_all(attention, sampling, seed)[0] for seed in (2, 3)]
+    original = {name: x.clone() for name, x in t.items()}
+    wants = []
+    for inputs in (original, *others):
+        refill(t, inputs)
+        run()
+        wants.append(results())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    torch.cuda.synchronize()
+    for turn in range(2):
+        for inputs, want in zip((original, *others), wants):
+            refill(t, inputs)
+            for name in ("out", "lse", "probs", "path", "accepted", "next"):
+                t[name].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(results(), want)), turn
+
+
+def test_streams_side_by_side(attention, sampling):
+    """Two streams at once, each with its own workspaces, against the calls one after the other."""
+    calls = [step_of_all(attention, sampling, seed) for seed in (4, 5)]
+    saved = [{name: x.clone() for name, x in t.items()} for t, _, _ in calls]
+    wants = []
+    for t, run, results in calls:
+        run()
+        wants.append(results())
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for (t, _, _), old in zip(calls, saved):
+            refill(t, old)
+        torch.cuda.synchronize()
+        for stream, (_, run, _) in zip(streams, calls):
+            with torch.cuda.stream(stream):
+                run()
+        torch.cuda.synchronize()
+        for (_, _, results), want in zip(calls, wants):
+            assert all(torch.equal(a, b) for a, b in zip(results(), want))
+
+
+def test_tree_and_move_past_32_bits(attention):
+    """Pages whose bytes start past 2^32: 1.1 million of 4 KiB."""
+    rng = np.random.default_rng(32)
+    dim, hq, hk, page, pages = 128, 4, 1, 64, 1_100_000
+    cache = attention.new_cache(pages, hk, page, dim)
+    used = [pages - 1, 3, pages - 20, pages - 7]
+    small = random_cache(attention, rng, 4, hk, page, dim)
+    for big, part in zip(cache, small):
+        big[used] = part
+    lens, counts = [200], [12]
+    parents = random_tree(rng, 12, 0.5)
+    q = bf16_randn(rng, 12, hq, dim).cuda()
+    out, lse = run_tree(attention, q, cache, np.int32([used]), lens, [0, 12], parents, 0.1, 12, 0)
+    want, want_lse = run_tree(attention, q, small, np.int32([[0, 1, 2, 3]]), lens, [0, 12], parents, 0.1, 12, 0)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    rows, starts = np.int32([0, 3, 2, 3]), np.int32([0, 4])
+    here = np.int64([used[0] * page + 1, used[1] * page + 2, used[2] * page, used[3] * page + 63])
+    there = np.int64([1, page + 2, 2 * page, 3 * page + 63])
+    attention.move_fp4(*cache, dev(rows), dev(here), dev(starts))
+    attention.move_fp4(*small, dev(rows), dev(there), dev(starts))
+    for big, part in zip(cache, small):
+        assert torch.equal(big[used], part)
