@@ -130,15 +130,15 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
   const uint32_t code_at = page_row * (D / 2) + half * (D / 4);
   const uint32_t scale_at = (page_row * S::kScaleBytes + half * S::kBlocks) & ~3u;
   char* const tile = shared + wave * S::kWaveBytes;
-  auto store_at = [&]() {
-    const int lane = int(anew(threadIdx.x & 63)), token = lane % 32, half = lane / 32;
-    return uint32_t(token * (2 * D) + ((half * D) ^ (16 * (token % 8))));
-  };
-  auto read_at = [&]() {
-    const int lane = int(anew(threadIdx.x & 63)), half = lane / 32, row = 4 * half + lane % 16 / 4;
-    return uint32_t(row * (2 * D) + 64 * half +
-                    16 * ((2 * (lane / 16 % 2) + lane % 4 / 2) ^ (row & 3)) + lane % 2 * 8);
-  };
+  uint32_t store_at, read_at, scale_byte;  // the last: of the lane's first scale in its word
+  {
+    const uint32_t lane = threadIdx.x & 63, half = lane / 32;
+    const uint32_t token = lane % 32, row = 4 * half + lane % 16 / 4;
+    store_at = token * (2 * D) + ((half * D) ^ (16 * (token % 8)));
+    read_at = row * (2 * D) + 64 * half + 16 * ((2 * (lane / 16 % 2) + lane % 4 / 2) ^ (row & 3)) +
+              lane % 2 * 8;
+    scale_byte = (token * S::kScaleBytes + half * S::kBlocks) % 4;
+  }
 
   for (int64_t at = run.begin; at < run.end;) {
     const int seq = place.seq, kv_head = place.head;
@@ -224,11 +224,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
         fill(column < 16 ? code : code2, column < 16 ? scale : scale2);
       }
     };
-    // The byte of the lane's first scale in its word, and eight channels of step j by it.
-    auto scale_byte = [&]() {
-      const int lane = int(anew(threadIdx.x & 63));
-      return uint32_t(lane % 32 * S::kScaleBytes + lane / 32 * S::kBlocks) % 4;
-    };
+    // Eight channels of step j, with the lane's first scale at `byte` of its word.
     auto converted = [&](const TreeRaw<D>& raw, int j, uint32_t byte) __attribute__((always_inline)) {
       return fp4_to_bf16x8(raw.codes[j], fp4_scale_in(raw.scales, fp4_scale_turn(byte + j / 4)));
     };
@@ -290,7 +286,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
       bf16x8 key;
-      const uint32_t key_byte = scale_byte();
+      const uint32_t key_byte = anew(scale_byte);
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         if (i % kTiles == 0) key = __builtin_bit_cast(bf16x8, converted(k, i / kTiles, key_byte));
@@ -312,7 +308,7 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
         const bool real = (there >> (column / 16) & 1) && token < s.context;
 #pragma unroll
         for (int b = 0; b < S::kBlocks; ++b) {
-          const uint32_t shift = (scale_byte() + b) * 8;
+          const uint32_t shift = (anew(scale_byte) + b) * 8;
           if (!real || (v.scales >> shift & 0xFF) >= 253) {
             if (real) poisoned |= 1u << (half * S::kBlocks + b);
 #pragma unroll
@@ -332,14 +328,14 @@ __global__ void __launch_bounds__(TreeShape<D>::kThreads, 2)
         }
       }
       wave_order();
-      const uint32_t value_byte = scale_byte(), to = store_at();
+      const uint32_t value_byte = anew(scale_byte), to = anew(store_at);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
         *reinterpret_cast<u32x4*>(tile + (to ^ (16 * j))) = converted(v, j, value_byte);
       wave_order();
       load(v, p.cache.v, t_next, i);
       // The first values' operands come while the scores are weighed.
-      const uint32_t from = read_at();
+      const uint32_t from = anew(read_at);
       auto value = [&](int i) {
         const char* at = tile + ((from ^ (64 * (i / 2))) + 16 * (i % 2) * (2 * D));
         const u32x2 a = lds_read_transposed(at), b = lds_read_transposed(at + 8 * (2 * D));
