@@ -14,22 +14,23 @@
 //
 // Two waves a SIMD, eight a workgroup, which share the queries in LDS; the sums of the rows take half of
 // the registers. Every block of a key head reads and converts its tokens anew, from the caches between
-// it and HBM: what bounds it is the time that a SIMD's two waves need for a tile by turns, of which the
-// MFMAs are a third: 64 rows of 128 channels take a wave 3600 clocks a tile, 620 for S, 1170 to convert V
-// and store it, 850 to weigh, 780 for O. Larger blocks convert less, but four tiles of rows at 512
-// registers a wave took longer (one wave a SIMD has nobody to hide behind), and so did workgroups that
-// share converted tokens through LDS, with their barriers.
+// it and HBM: what bounds it is the issue of a SIMD's two waves. 64 rows of 128 channels take a wave 3600
+// clocks a tile, 1024 of them MFMAs; over a long call vector instructions are half of all clocks, MFMAs a
+// third. Larger blocks convert less, but four tiles of rows at 512 registers a wave took longer (one wave a
+// SIMD has nobody to hide behind), and so did workgroups that share converted tokens through LDS, with
+// their barriers.
 //
 // Queries of S and values of O are read from LDS some products ahead, with the compiler kept from
-// moving the reads back together; addresses are computed anew in each tile, since registers held for
-// them through the loop were spilled.
+// moving the reads back together; addresses are computed anew in each tile from one number for each kind,
+// since registers held for all of them through the loop were spilled.
 //
 // What a row sees of 32 tokens is one word of bits (tree_sees), in tiles on the edge only.
 //
-// Measured, us, 8 x 64 tokens behind up to 16000 of 40 query and 8 key heads of 128: 161, 43 % of the rate
+// Measured, us, 8 x 64 tokens behind up to 16000 of 40 query and 8 key heads of 128: 153, 54 % of the rate
 // that a large product of matrices reaches (split kernel in blocks of 64 rows 182, workgroups that share
-// converted tokens 228); 16 x 16 tokens behind up to 8000 of 32 and 8 heads 51, 4 x 26 behind up to
-// 131071 of 24 and 4 heads of 256 365; 32 x 11 of 28 and 4 heads with a window of 1024 21.
+// converted tokens 228); 16 x 16 tokens behind up to 8000 of 32 and 8 heads 50, 4 x 26 behind up to
+// 131071 of 24 and 4 heads of 256 346 (blocks of 128 rows that share converted tokens 360); 32 x 11 of 28
+// and 4 heads with a window of 1024 21.
 #include "attention_runs.h"
 #include "launch.h"
 

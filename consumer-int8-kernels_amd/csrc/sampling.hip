@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kSampleThreads)
 // share a sequence: all follow it, each sums its chunk, and sums go from one to the others through the
 // workspace, which a first kernel fills with what is no sum. A workgroup that waits in vain (another may
 // not run yet) adds up the missing chunks itself, so every wait ends, and to the same result. 16 trees
-// of 32 rows over 128000 tokens 29.6 us, 3 to 4 a sum; with one workgroup a sequence 62.7.
+// of 32 rows over 128000 tokens 30 to 35 us, 3 to 4 a sum; with one workgroup a sequence 62.7.
 
 constexpr float kMostUniform = 1 - 0x1p-24f;  // the largest number below 1
 
