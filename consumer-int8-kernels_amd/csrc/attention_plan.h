@@ -72,9 +72,11 @@ inline RowSplit row_split(int64_t tokens, int64_t seqs, int group, int64_t max_q
   return {few, group <= few, most > few};
 }
 
-// Trees: up to kFewTreeRows a sequence go to the split kernel as they are few, more to the tree kernel in
-// blocks.
-constexpr int kFewTreeRows = 32;
+// Trees: up to so many rows a sequence go to the split kernel as they are few, more to the tree kernel in
+// blocks. us, split and tree kernel: 16 trees behind up to 8000, 32 rows of 8 heads of 128 35.6 and 48.4, 12
+// rows 30.7 and 46.4, 21 of 4 heads 29.6 and 30.7; one behind 600, 21 rows of 2 heads of 64 9.6 and 10.8;
+// but 18 rows of 4 heads of 256 38.5 and 35.9, 30 40.3 and 37.1, one behind 600 16.7 and 16.7.
+constexpr int few_tree_rows(int dim) { return dim == 256 ? 16 : 32; }
 constexpr int tree_rows(int dim) { return dim == 256 ? 32 : 64; }
 // What it costs to begin a context, in tiles of one wave.
 constexpr int kTreeBegin = 40;

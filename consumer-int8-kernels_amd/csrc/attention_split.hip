@@ -568,8 +568,10 @@ static hipError_t launch_split_rows(const AttentionArgs& args, int dim, int most
       return args.parents ? launch_split<128, kTiles, true>(args, most, stream)
                           : launch_split<128, kTiles, false>(args, most, stream);
     default:
-      return args.parents ? launch_split<256, kTiles, true>(args, most, stream)
-                          : launch_split<256, kTiles, false>(args, most, stream);
+      static_assert(few_tree_rows(256) <= 16, "trees of two tiles are the tree kernel's");
+      if constexpr (kTiles == 1)
+        if (args.parents) return launch_split<256, kTiles, true>(args, most, stream);
+      return launch_split<256, kTiles, false>(args, most, stream);
   }
 }
 
@@ -581,7 +583,7 @@ hipError_t launch_attention_split(const AttentionArgs& args, int dim, int most,
 
 hipError_t launch_attention_fp4(const AttentionArgs& args, int dim, hipStream_t stream) {
   if (args.tokens == 0 || args.seqs == 0) return hipSuccess;
-  if (args.parents && int64_t(args.max_q) * args.group > kFewTreeRows)
+  if (args.parents && int64_t(args.max_q) * args.group > few_tree_rows(dim))
     return launch_attention_tree(args, dim, stream);
   const RowSplit rows = row_split(args.tokens, args.seqs, args.group, args.max_q);
   if (rows.split) {
