@@ -172,6 +172,10 @@ bool shares_cache(const ci8_fp4_cache& c, const Extents& e, const void* p, int64
          overlap(c.v_codes, e.bytes[2], p, bytes) || overlap(c.v_scales, e.bytes[3], p, bytes);
 }
 
+bool has_buffers(const ci8_fp4_cache& c) {
+  return c.k_codes && c.k_scales && c.v_codes && c.v_scales;
+}
+
 ci8::HeadsView view(const ci8_heads& v) {
   return {static_cast<uint16_t*>(v.data), int(v.heads), v.token_stride, v.head_stride};
 }
@@ -429,6 +433,8 @@ int ci8_move_fp4(const ci8_fp4_cache* cache, const int32_t* rows, const int64_t*
   if (int s = check_cache(cache, dim, e)) return s;
   if (!(seqs >= 0 && seqs <= 65535))
     return abi_fail(CI8_ERR_GEOMETRY, "Invalid move: expected at most 65535 sequences");
+  if (seqs > 0 && tokens > 0 && !(rows && slots && q_starts && has_buffers(*cache)))
+    return abi_fail(CI8_ERR_GEOMETRY, "Invalid move: a buffer is missing");
   if (!aligned(rows, 4) || !aligned(slots, 8) || !aligned(q_starts, 4))
     return abi_fail(CI8_ERR_ALIGNMENT, "move_fp4 requires aligned buffers");
   if (int s = check_cache_written(*cache, e)) return s;
