@@ -422,6 +422,10 @@ int ci8_attention_fp4_tree(const ci8_heads* q, const ci8_fp4_cache* cache,
     return abi_fail(CI8_ERR_GEOMETRY, "A tree needs q_starts and parents");
   if (max_q > ci8::kMostTree)
     return abi_fail(CI8_ERR_TOO_LARGE, "A tree has at most 64 queries");
+  if (seqs > 0 && tokens > 0 && q && cache &&
+      !(q->data && has_buffers(*cache) && context_lens && workspace && out &&
+        (page_table || table_width == 0)))
+    return abi_fail(CI8_ERR_GEOMETRY, "Invalid attention: a buffer is missing");
   return attend(q, cache, page_table, table_width, context_lens, q_starts, parents, seqs, tokens, dim,
                 workspace, out, lse, scale, max_q, window, stream);
 }
