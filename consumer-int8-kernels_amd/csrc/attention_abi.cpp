@@ -290,8 +290,8 @@ int attend(const ci8_heads* q, const ci8_fp4_cache* cache, const int32_t* page_t
   args.tokens = int(tokens);
   args.group = int(q->heads / cache->heads);
   args.max_q = int(max_q < tokens ? max_q : tokens);
-  // A workgroup a unit, and one more for each of up to 256 CUs.
-  if (ci8::row_split(tokens, seqs, args.group, args.max_q).prompt &&
+  // The prompt kernel, which has no trees: a workgroup a unit, and one more for each of up to 256 CUs.
+  if (!parents && ci8::row_split(tokens, seqs, args.group, args.max_q).prompt &&
       !ci8::launch_fits(
           ci8::prompt_units(tokens, seqs, args.group, args.max_q, args.cache.heads) + 256,
           ci8::kPromptThreads))
