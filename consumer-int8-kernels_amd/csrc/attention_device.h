@@ -66,7 +66,7 @@ __device__ __forceinline__ int tree_parent(const AttentionArgs& p, const Sequenc
 // other number is none.
 __device__ __forceinline__ uint64_t tree_ancestors(int up, int lane) {
   if (up >= lane) up = -1;
-  uint64_t set = uint64_t(1) << lane;
+  uint64_t set = lane_set(lane);
   while (__any(up >= 0)) {
     const int from = max(up, 0);
     const uint32_t low = __shfl(int(set), from, 64), high = __shfl(int(set >> 32), from, 64);
@@ -91,9 +91,8 @@ __device__ __forceinline__ int tree_low(const AttentionArgs& p, const Sequence& 
   return p.window ? max(s.shift + __shfl(depth, query, 64) + 1 - p.window, 0) : 0;
 }
 // What a row of a tree, which attends to [low, high), sees of the 32 tokens from `first` on, bit i for
-// token first + i: those before the tree, and those that its query's set in LDS names. Shifts of 64
-// bits by a vector register are kept out: with the amount in the last register that a wave has they
-// gave wrong bits here now and then.
+// token first + i: those before the tree, and those that its query's set in LDS names. From halves of 32
+// bits, as lane_set.
 __device__ __forceinline__ uint32_t tree_sees(const uint64_t* seen, int low, int high, int first,
                                               int shift) {
   const uint64_t set = seen[max(high - 1 - shift, 0) & 63];

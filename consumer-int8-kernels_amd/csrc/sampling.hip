@@ -394,9 +394,9 @@ __device__ __forceinline__ double at_lane(double v, int lane) {
 // Tokens of rejected rows in [begin, end) to `skip`; how many.
 __device__ __forceinline__ int skipped(uint64_t rejected, int token, int lane, int begin, int end,
                                        int* skip) {
-  const bool mine = (rejected >> lane & 1) && token >= begin && token < end;
+  const bool mine = has_lane(rejected, lane) && token >= begin && token < end;
   const uint64_t all = __ballot(mine);
-  if (mine) skip[__builtin_popcountll(all & ((uint64_t(1) << lane) - 1))] = token;
+  if (mine) skip[lanes_before(all)] = token;
   return __builtin_popcountll(all);
 }
 
@@ -549,7 +549,7 @@ __device__ __forceinline__ Followed follow(const VerifyArgs& p, const Rows& rows
       stands = number * (left * q) < w;
     } else {
       const int id = __builtin_amdgcn_readlane(x.token, i);
-      if (__ballot((x.stop.rejected >> lane & 1) && x.token == id)) w = 0;
+      if (__ballot(has_lane(x.stop.rejected, lane) && x.token == id)) w = 0;
       stands = number * left < w;
     }
     if (stands) {
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(kPickThreads)
   Stop stop = stops(p, chunks)[seq];
   const double number = fminf(fmaxf(p.uniforms[rows.begin], 0.f), kMostUniform);
   int token = -1;
-  if (stop.rejected >> lane & 1) token = token_of(p, rows.begin + lane);
+  if (has_lane(stop.rejected, lane)) token = token_of(p, rows.begin + lane);
   const double all = reduce_all<kThreads>(mine, room, add<double>);
   double bar = number * all, before;
   const int chunk = first_past<kThreads>(mine, bar, before, room, places);
