@@ -25,12 +25,14 @@ inline Chunks probs_parts(int64_t tokens, int64_t vocab) {
 }
 
 // Two kernels: chunks of a row of up to kChunkPacks * 1024 values, 256 of them at least where rows are
-// that long.
+// that long, and 256 of a row at most, a thread of the second kernel each. One row of 262208 BF16
+// logits 8.6 us in 129 chunks, 29 as a whole row; of 1000000 8.3 and 101.
 constexpr int kChunkPacks = 8;
 inline Chunks probs_chunks(int64_t tokens, int64_t vocab) {
   const int step = kSampleThreads * 4;
+  const int64_t least = (vocab + step * kSampleThreads - 1) / (step * kSampleThreads);
   int64_t packs = tokens * vocab / step / 256;
-  if (packs < 1) packs = 1;
+  if (packs < least) packs = least;
   if (packs > kChunkPacks) packs = kChunkPacks;
   const int64_t length = packs * step;
   return {int(length), int((vocab + length - 1) / length)};

@@ -6,6 +6,7 @@ import subprocess
 import pytest
 
 from tests.conftest import PKG
+from tests.test_drafts_plan import plan  # noqa: F401
 
 
 def test_a_wait_in_vain_costs_no_more_than_the_sums(tmp_path):
@@ -19,3 +20,12 @@ def test_a_wait_in_vain_costs_no_more_than_the_sums(tmp_path):
     subprocess.run([gxx, "-std=c++17", f"-I{PKG / 'csrc'}", str(tmp_path / "p.cpp"), "-o", str(tmp_path / "p")], check=True)
     polls = int(subprocess.run([str(tmp_path / "p")], check=True, capture_output=True, text=True).stdout)
     assert 100 <= polls and polls * 0.16 <= 94
+
+
+def test_one_long_row_is_cut_into_chunks(plan):  # noqa: F811
+    """Up to 256 chunks of 8192 values, whatever their number would be in smaller ones."""
+    sizes = [36864, 262144, 262145, 262208, 300001, 524287, 524289, 10**6, 2000003, 1 << 21]
+    for vocab, (*_, length, chunks, bf16, fp32) in zip(sizes, plan("probs", [(1, v) for v in sizes])):
+        assert bf16 and fp32 and chunks <= 256 and length * chunks >= vocab, (vocab, length, chunks)
+    for *_, bf16, fp32 in plan("probs", [(1, (1 << 21) + 1), (1, 36863)]):
+        assert not bf16 and not fp32

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from tests.helpers import guard_intact, with_guard
 from tests.test_gpu_attention import bf16_randn, random_cache, say
 from tests.test_gpu_drafts import attention, check_probs, check_tree, random_tree, run_tree, sampling  # noqa: F401
 
@@ -43,3 +44,15 @@ def test_trees_of_many_sequences_and_heads(attention):  # noqa: F811
     q = bf16_randn(rng, 64, hk * group, dim).cuda()
     out, lse = run_tree(attention, q, cache, table, lens, starts, parents, 0.1, 64, 0)
     check_tree(q, cache, table, lens, starts, parents, 0.1, 0, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [262209, 1000003, 1 << 21, (1 << 21) + 5])
+def test_probs_of_one_long_row(sampling, vocab, dtype):  # noqa: F811
+    say("one long row", vocab, dtype)
+    rng = np.random.default_rng(vocab)
+    x = torch.from_numpy((3 * rng.standard_normal((1, vocab))).astype(np.float32)).to(dtype).cuda()
+    for t in (None, [0.0], [0.7]):
+        out, guard = with_guard((1, vocab), torch.float32, 5.0)
+        check_probs(sampling, x, t, out)
+        assert guard_intact(guard, 5.0)
