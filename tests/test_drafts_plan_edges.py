@@ -1,4 +1,5 @@
-"""Constants of the launches of speculative decoding's operators that bound what a call may cost."""
+"""Launches of speculative decoding's operators: constants that bound what a call may cost, and which kernels
+the sizes of tests/test_gpu_drafts_edges.py go to."""
 
 import shutil
 import subprocess
@@ -29,3 +30,11 @@ def test_one_long_row_is_cut_into_chunks(plan):  # noqa: F811
         assert bf16 and fp32 and chunks <= 256 and length * chunks >= vocab, (vocab, length, chunks)
     for *_, bf16, fp32 in plan("probs", [(1, (1 << 21) + 1), (1, 36863)]):
         assert not bf16 and not fp32
+
+
+def test_sizes_of_edge_cases_have_chunks(plan):  # noqa: F811
+    for length, count, each, rounds in plan("verify", [(seqs, 20011) for seqs in (1, 7, 23)]):
+        assert count > 1 and rounds > 1 and count * length > 20011 - length
+    few = plan("probs", [(rows, 40003) for rows in (1, 5, 200, 300)])
+    assert [(bool(bf16), bool(fp32)) for *_, bf16, fp32 in few] == [(True, True)] * 2 + [(False, False), (True, False)]
+    assert all(parts > 4 for _, _, _, parts, _, _ in few)
