@@ -11,8 +11,8 @@ verify_drafts(target_probs, draft_probs, tokens, parents, q_starts, uniforms, wo
     then drafted ones, at most 63 of them; INT64 tokens [T]; INT32 parents [T] name each row's parent,
     a row before it, by its number in the sequence (None: the row before). FP32 target_probs and
     draft_probs [T,V]: in each row what follows its token, by the target and by the drafter. With
-    draft_probs, a row's children were drawn from its row there, independently; without (None), they
-    are certain choices, such as a drafter's best. FP32 uniforms [T] in [0, 1), one a row.
+    draft_probs, a row's children were drawn from its row there, independently (with replacement);
+    without (None), they are certain choices, such as a drafter's best. FP32 uniforms [T] in [0, 1), one a row.
     From row 0 on the children of the last accepted row are tried in order, and one stands by
     rejection sampling with its row's number; where none does, the next token is drawn from what the
     rejections leave of the target's row with the number of row 0. So the tokens are distributed as if

@@ -26,11 +26,15 @@
 //
 // What a row sees of 32 tokens is one word of bits (tree_sees), in tiles on the edge only.
 //
-// Measured, us, 8 x 64 tokens behind up to 16000 of 40 query and 8 key heads of 128: 153, 54 % of the rate
-// that a large product of matrices reaches (split kernel in blocks of 64 rows 182, workgroups that share
-// converted tokens 228); 16 x 16 tokens behind up to 8000 of 32 and 8 heads 50, 4 x 26 behind up to
-// 131071 of 24 and 4 heads of 256 346 (blocks of 128 rows that share converted tokens 360); 32 x 11 of 28
-// and 4 heads with a window of 1024 21.
+// Weights are rounded to BF16 for the second product, and their sum is of the FP32 weights, as in
+// attention_split.hip and for its reason: outputs are 0.0019 to 0.0021 from 64 bits where FP32 weights give
+// 0.0017, which is the outputs' own rounding.
+//
+// Measured, us, and in turn with it the split kernel in blocks of 64 rows: 8 x 64 tokens behind up to 16000
+// of 40 query and 8 key heads of 128 151 and 169, 60 % of the rate that a large product of matrices reaches
+// (workgroups that share converted tokens took 228 when the blocks took 182); 16 x 16 tokens behind up to
+// 8000 of 32 and 8 heads 49 and 53; 32 x 11 of 28 and 4 heads with a window of 1024 21 and 26. 4 x 26 behind
+// up to 131071 of 24 and 4 heads of 256 348, and workgroups that share converted tokens 347.
 #include "attention_runs.h"
 #include "launch.h"
 
@@ -532,6 +536,10 @@ hipError_t launch_tree(const AttentionArgs& args, hipStream_t stream) {
   static_assert(2 * 256 * S::kRows * 2 <= kAttentionWorkspaceRows * 2 - 2048 * 8,
                 "parts, statistics and descriptions fit the workspace");
   const bool by_context = contexts <= groups;
+  // With more than three workgroups a context, as in the split kernel. us, contexts apart and runs of all, by
+  // contexts for 256 workgroups: 80 (10 x 16 tokens of 8 heads of 128) 36 and no less; 88 37 and 43, 128 49 and
+  // 50; but 160 of 5 blocks 95 and 87, 192 69 and 62, 248 85 and 73; of 4 heads of 256, 5 blocks, 100 105 and
+  // 102, 120 154 and 128.
   const bool apart = few && args.seqs <= 64;
   attention_tree_kernel<D, true><<<groups, S::kThreads, 0, stream>>>(
       args, most, blocks, 2 * S::kWaves, by_context, apart);

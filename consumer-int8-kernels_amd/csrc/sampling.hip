@@ -46,7 +46,7 @@ __device__ __forceinline__ int smaller(int a, int b) { return min(a, b); }
 // of it, from the L2s, and writes a part; one launch, and nothing to wait for. Rows that are few and
 // long take two kernels over their chunks instead (sampling_plan.h has both sides' times).
 // Measured: 512 rows of 152000 BF16 logits 110 us, 4.2 TB/s of the 5.1 that a copy reaches; 1000 of 50001
-// in FP32 89, 4.5; one of 32000 5.7, 3 of it the launch. Plain stores: nontemporal ones 163.
+// in FP32 89, 4.5; one of 32000 5.8, 3 of it the launch. Plain stores: nontemporal ones 163.
 
 // Registers hold 163840 BF16 or 81920 FP32 values of a row, or 32768 in less code, which a launch of
 // few workgroups has to fetch first: one row of 32000 5.4 us, with room for 163840 10.8.
@@ -307,7 +307,8 @@ __global__ void __launch_bounds__(kSampleThreads)
 // share a sequence: all follow it, each sums its chunk, and sums go from one to the others through the
 // workspace, which a first kernel fills with what is no sum. A workgroup that waits in vain (another may
 // not run yet) adds up the missing chunks itself, so every wait ends, and to the same result. 16 trees
-// of 32 rows over 128000 tokens 30 to 35 us, 3 to 4 a sum; with one workgroup a sequence 62.7.
+// of 32 rows over 128000 tokens take as long as the one that asks for most sums before its last: 25 us with
+// two of them, 31 to 35 with four, 43 with six, so 4 a sum; with one workgroup a sequence 62.7.
 
 constexpr float kMostUniform = 1 - 0x1p-24f;  // the largest number below 1
 

@@ -37,10 +37,13 @@ inline Chunks probs_chunks(int64_t tokens, int64_t vocab) {
   const int64_t length = packs * step;
   return {int(length), int((vocab + length - 1) / length)};
 }
-// Where they are faster, and their sums fit threads and workspace. us, chunks and whole rows, BF16: 1 x
-// 50001 8.1 and 9.5, 52 x 50001 10.0 and 13.5, 52 x 152000 13.3 and 24.5, 128 x 152000 26.6 and 34.3, 400 x
-// 50001 30.1 and 37.4; but 256 x 50001 19.4 and 18.0, 512 x 152000 124 and 110, 52 x 32000 8.8 and
-// 7.8. FP32: 128 x 152000 46 and 58, but 400 x 81000 75 and 59.
+// For few rows, and where whole rows of BF16 leave part of a second round of 256 workgroups empty, if the
+// sums fit threads and workspace. us, chunks and whole rows, BF16: 1 x 50001 8.1 and 9.5, 52 x 50001 10.0 and
+// 13.5, 52 x 152000 13.3 and 24.5, 128 x 152000 26.6 and 34.3, 400 x 50001 30.1 and 37.4; but 256 x 50001 19.4
+// and 18.0, 512 x 152000 124 and 110, 52 x 32000 8.8 and 7.8. FP32: 128 x 152000 46 and 58, but 400 x 81000
+// 75 and 59. The rule leaves out what later rounds leave empty (BF16 513 x 152000 114 and 128, 520 x 50001 35
+// and 42, but 700 x 152000 163 and 159) and that whole FP32 rows past 81920 values are read three times
+// (300 x 152000 84 and 119, 256 x 152000 72 and 71): such calls would gain by chunks.
 constexpr int64_t kFewVocab = 9 * kProbsPart;
 inline bool probs_in_chunks(int64_t tokens, int64_t vocab, const Chunks& c, bool bf16) {
   return vocab >= kFewVocab && (tokens < 192 || (bf16 && tokens > 256 && tokens < 512)) &&

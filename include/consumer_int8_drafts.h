@@ -73,6 +73,7 @@ int ci8_token_probs(const void* logits, int64_t logit_bits, int64_t logit_stride
  *     new w (so w / S is max(w / S - q, 0), made to sum to 1, of the w before);
  *   without, children are certain choices: w = p, S = 1; child x stands if u S < w(x); if not, S
  *     loses w(x) and w(x) becomes 0.
+ * Children drawn without replacement are neither: what is returned would not be so distributed.
  * Where none stands, or c has no child, the next token is the first whose running sum of w passes u
  * times the sum of w, with u the number of the sequence's row 0; where w is zero everywhere, p takes
  * its place; where p is, too, the next token is -1. In 64 bits throughout.
